@@ -81,6 +81,8 @@ SYMBOLS = [
     "gs_ot_value_f32", "gs_scale_cols_f32", "gs_ot_divdiff_f32", "gs_clamp_finite_f32", "gs_gcond_set_structure", "gs_gcond_set_block_structure",
     "gs_comm_unique_id", "gs_comm_probe", "gs_comm_create_rccl", "gs_comm_create_callback", "gs_comm_create_null", "gs_comm_ipc_arena", "gs_comm_create_ipc", "gs_comm_ipc_error", "gs_comm_check", "gs_comm_destroy", "gs_comm_rank", "gs_comm_world",
     "gs_comm_allreduce", "gs_comm_set_timing", "gs_comm_read_timing", "gs_comm_read_timing2", "gs_gcond_outer_step_sharded", "gs_gcond_outer_step_sharded_ex",
+    "gs_embedding_fwd", "gs_embedding_bwd_scratch_bytes", "gs_embedding_bwd", "gs_gated_fwd_scratch_bytes", "gs_gated_fwd",
+    "gs_gated_bwd_scratch_bytes", "gs_gated_bwd", "gs_distill_fwd", "gs_distill_bwd", "gs_distill_loss_grad",
 ]
 
 # gs_allreduce_fn of include/gslim.h: int fn(void* user, void* buf, long count, int dtype, gs_stream_t stream)
@@ -229,6 +231,19 @@ def lib():
     L.gs_gcond_set_h1_bits.argtypes = [i]
     L.gs_gcond_set_aux_priority.argtypes = [i]
     L.gs_gcond_set_dw1_generated.argtypes = [i]
+    L.gs_embedding_fwd.argtypes = [vp, l, l, i, i, vp, l, f, vp, l, vp]
+    L.gs_embedding_bwd_scratch_bytes.argtypes = [l, l, i]
+    L.gs_embedding_bwd_scratch_bytes.restype = C.c_size_t
+    L.gs_embedding_bwd.argtypes = [vp, l, i, vp, l, l, i, f, i, vp, l, i, vp, vp]
+    L.gs_gated_fwd_scratch_bytes.argtypes = [l, l, l, i]
+    L.gs_gated_fwd_scratch_bytes.restype = C.c_size_t
+    L.gs_gated_fwd.argtypes = [vp, l, vp, vp, l, i, l, l, l, i, vp, l, vp, vp, vp]
+    L.gs_gated_bwd_scratch_bytes.argtypes = [l, l, l, i]
+    L.gs_gated_bwd_scratch_bytes.restype = C.c_size_t
+    L.gs_gated_bwd.argtypes = [vp, l, vp, l, vp, vp, l, vp, i, l, l, l, i, vp, l, vp, vp, l, vp, vp]
+    L.gs_distill_fwd.argtypes = [vp, l, i, l, i, vp, vp, i, f, vp, vp, vp]
+    L.gs_distill_bwd.argtypes = [vp, l, i, l, i, vp, vp, i, f, vp, vp, vp, l, vp]
+    L.gs_distill_loss_grad.argtypes = [vp, l, i, l, i, vp, vp, i, f, vp, vp, vp, l, vp]
     _lib = L
     return L
 

@@ -1,0 +1,66 @@
+// Element types of the operators that take rows in 32 or 16 bits (GS_TYPE_* of gslim.h), and how their kernels read and write them.
+#pragma once
+#include "gs_common.h"
+
+template <int T>
+struct GsElt;
+template <>
+struct GsElt<GS_TYPE_F32> {
+  typedef float type;
+};
+template <>
+struct GsElt<GS_TYPE_F16> {
+  typedef _Float16 type;
+};
+template <>
+struct GsElt<GS_TYPE_BF16> {
+  typedef __bf16 type;
+};
+
+// N elements that are aligned to one element only: a row of odd width starts anywhere, and the global memory path takes 16-byte
+// accesses at any element's address (a wave's access then touches one cache line more).
+template <typename E, int N>
+struct GsVec {
+  typedef E type __attribute__((ext_vector_type(N), aligned(sizeof(E))));
+};
+template <typename E>
+struct GsVec<E, 1> {
+  typedef E type;
+};
+
+// p[0 .. N) as floats, the elements from `n` on as `fill`
+template <typename E, int N>
+__device__ __forceinline__ void gs_load(const E* __restrict__ p, long n, float fill, float* __restrict__ v) {
+  if (n >= N) {
+    const typename GsVec<E, N>::type r = *(const typename GsVec<E, N>::type*)p;
+    if constexpr (N == 1) {
+      v[0] = (float)r;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = (float)r[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : fill;
+  }
+}
+
+template <typename E, int N>
+__device__ __forceinline__ void gs_store(E* __restrict__ p, long n, const float* __restrict__ v) {
+  if (n >= N) {
+    typename GsVec<E, N>::type r;
+    if constexpr (N == 1) {
+      r = (E)v[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = (E)v[i];
+    }
+    *(typename GsVec<E, N>::type*)p = r;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) p[i] = (E)v[i];
+  }
+}
+
+static inline int gs_type_bytes(int t) { return t == GS_TYPE_F32 ? 4 : (t == GS_TYPE_F16 || t == GS_TYPE_BF16 ? 2 : 0); }

@@ -1,0 +1,246 @@
+"""Operators for training a student on a teacher's top logits, on rows in fp32, fp16 or bf16 (csrc/gs_embedding.hip, gs_gated.hip,
+gs_distill.hip; the C entry points are in include/gslim.h):
+
+    embedding, embedding_grad                  rows of a table by token / node id, scaled; the table's gradient
+    gated_ffn, gated_ffn_grad                  h = act(x Wg^T) * (x Wu^T) and its backward pass
+    distill, distill_grad, distill_loss_grad   tau^2 KL(teacher's top logits || student) per row and its gradient
+
+Gradients are explicit calls, like everywhere in this package: no autograd.  Every call runs on the current stream of its tensors'
+device (which need not be the current device) and takes its outputs and scratch from torch's allocator there, so it can be captured
+into a graph, and calls on two streams or in two graphs share nothing.  A tensor that another stream writes or frees has to be
+synchronised by the caller, as for any torch call.  Matrices may have any row stride; their rows have to be dense.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from ._lib import check, ptr, vp
+
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+MAX_TOP = 1024
+
+
+def _need(ok, message):
+    if not ok:
+        raise ValueError(f"graphslim_amd.ops: {message}")
+
+
+def _device(**tensors):
+    """The one GPU all of them are on."""
+    dev = None
+    for name, t in tensors.items():
+        _need(isinstance(t, torch.Tensor), f"{name} is a tensor (got {type(t).__name__})")
+        _need(t.device.type == "cuda", f"{name} is on {t.device}: there is no CPU path")
+        _need(dev is None or t.device == dev, f"{name} is on {t.device}, other arguments on {dev}")
+        dev = t.device
+    return dev
+
+
+def _matrix(name, t, cols=None, rows=None, dtype=None):
+    """Row stride of a 2-D tensor with dense rows."""
+    _need(t.dim() == 2, f"{name} has two dimensions (got {tuple(t.shape)})")
+    _need(t.dtype in TYPES, f"{name} is fp32, fp16 or bf16 (got {t.dtype})")
+    _need(dtype is None or t.dtype == dtype, f"{name} is {t.dtype}, other arguments {dtype}")
+    _need(cols is None or t.shape[1] == cols, f"{name} has {t.shape[1]} columns, {cols} are wanted")
+    _need(rows is None or t.shape[0] == rows, f"{name} has {t.shape[0]} rows, {rows} are wanted")
+    _need(t.shape[1] > 0, f"{name} has no columns")
+    _need(t.shape[1] == 1 or t.stride(1) == 1, f"the rows of {name} are not dense (strides {t.stride()})")
+    if t.shape[0] <= 1:
+        return t.shape[1]
+    _need(t.stride(0) >= t.shape[1], f"the rows of {name} overlap (strides {t.stride()})")
+    return t.stride(0)
+
+
+def _vector(name, t, n, dtype):
+    _need(t.dtype == dtype, f"{name} is {dtype} (got {t.dtype})")
+    _need(tuple(t.shape) == (n,) and t.is_contiguous(), f"{name} is a dense vector of {n} (got {tuple(t.shape)}, strides {t.stride()})")
+
+
+def _ids(ids):
+    _need(ids.dtype == torch.int32, f"ids are int32 (got {ids.dtype})")
+    _need(ids.is_contiguous(), f"ids are dense (strides {ids.stride()})")
+
+
+def _scratch(nbytes, dev):
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=dev)
+
+
+def _stream(dev):
+    return vp(torch.cuda.current_stream(dev).cuda_stream)
+
+
+# ------------------------------------------------------------------------------------------------
+# embedding
+# ------------------------------------------------------------------------------------------------
+
+
+def embedding(table, ids, scale=1.0, out=None):
+    """scale * table[ids], of shape ids.shape + (width,); an id outside the table is padding and gives zeros.  `out`: a
+    [ids.numel(), width] matrix that receives the rows and is returned as it is."""
+    dev = _device(table=table, ids=ids)
+    ld = _matrix("table", table)
+    _need(table.shape[0] > 0, "table has no rows")
+    _ids(ids)
+    n, F = ids.numel(), table.shape[1]
+    if out is None:
+        res = torch.empty(n, F, dtype=table.dtype, device=dev)
+        ldo = F
+    else:
+        _device(table=table, out=out)
+        ldo = _matrix("out", out, F, n, table.dtype)
+        res = out
+    with torch.cuda.device(dev):
+        check(_lib.lib().gs_embedding_fwd(ptr(table), ld, table.shape[0], F, TYPES[table.dtype], ptr(ids), n, float(scale), ptr(res), ldo,
+                                          _stream(dev)))
+    return res if out is not None else res.view(*ids.shape, F)
+
+
+def embedding_grad(d_out, ids, n_rows, scale=1.0, out=None, accumulate=False, dtype=None):
+    """Gradient [n_rows, width] of `embedding`'s table: scale times the sum of d_out's rows of each id, in ascending order.  d_out:
+    ids.shape + (width,), or [ids.numel(), width] with any row stride.  dtype: that of d_out (default) or torch.float32.  `out`
+    receives the gradient; with accumulate=True it is added to what `out` holds."""
+    dev = _device(d_out=d_out, ids=ids)
+    _ids(ids)
+    n = ids.numel()
+    if d_out.dim() != 2:
+        _need(d_out.dim() >= 1 and tuple(d_out.shape[:-1]) == tuple(ids.shape),
+              f"d_out is {tuple(d_out.shape)}, ids are {tuple(ids.shape)}")
+        _need(d_out.is_contiguous(), f"d_out is dense, or a matrix (strides {d_out.stride()})")
+        d_out = d_out.view(n, d_out.shape[-1])
+    ldd = _matrix("d_out", d_out, rows=n)
+    n_rows, F = int(n_rows), d_out.shape[1]
+    _need(n_rows > 0, f"a table of {n_rows} rows")
+    if out is None:
+        _need(not accumulate, "accumulate=True adds to `out`, which is missing")
+        dtype = d_out.dtype if dtype is None else dtype
+        _need(dtype in (d_out.dtype, torch.float32), f"the gradient is {d_out.dtype} or torch.float32 (got {dtype})")
+        out = torch.empty(n_rows, F, dtype=dtype, device=dev)
+    else:
+        _device(d_out=d_out, out=out)
+        _need(dtype in (None, out.dtype), f"out is {out.dtype}, dtype {dtype}")
+        _need(out.dtype in (d_out.dtype, torch.float32), f"the gradient is {d_out.dtype} or torch.float32 (got {out.dtype})")
+    ldw = _matrix("out", out, F, n_rows)
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        scratch = _scratch(L.gs_embedding_bwd_scratch_bytes(n, n_rows, F), dev)
+        check(L.gs_embedding_bwd(ptr(d_out), ldd, TYPES[d_out.dtype], ptr(ids), n, n_rows, F, float(scale), int(bool(accumulate)), ptr(out),
+                                 ldw, TYPES[out.dtype], ptr(scratch), _stream(dev)))
+    return out
+
+
+# ------------------------------------------------------------------------------------------------
+# gated feed-forward block
+# ------------------------------------------------------------------------------------------------
+
+
+def _gated_args(x, w_gate, w_up, act):
+    _need(act in ACTIVATIONS, f"act is one of {', '.join(ACTIVATIONS)} (got {act!r})")
+    dev = _device(x=x, w_gate=w_gate, w_up=w_up)
+    ldx = _matrix("x", x)
+    M, D = x.shape
+    ldw = _matrix("w_gate", w_gate, D, dtype=x.dtype)
+    F = w_gate.shape[0]
+    _need(F > 0, "w_gate has no rows")
+    ldu = _matrix("w_up", w_up, D, F, x.dtype)
+    _need(ldw == ldu, f"w_gate and w_up have one row stride (got {ldw} and {ldu})")
+    return dev, ldx, ldw, M, D, F
+
+
+def gated_ffn(x, w_gate, w_up, act="silu", save=False):
+    """act(x w_gate^T) * (x w_up^T) for x [M, D] and w_gate, w_up [F, D].  save=True returns (h, saved): `saved` holds the two
+    projections, [2, M, F] in fp32, for `gated_ffn_grad`."""
+    dev, ldx, ldw, M, D, F = _gated_args(x, w_gate, w_up, act)
+    h = torch.empty(M, F, dtype=x.dtype, device=dev)
+    saved = torch.empty(2, M, F, dtype=torch.float32, device=dev) if save else None
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        scratch = _scratch(L.gs_gated_fwd_scratch_bytes(M, D, F, TYPES[x.dtype]), dev)
+        check(L.gs_gated_fwd(ptr(x), ldx, ptr(w_gate), ptr(w_up), ldw, TYPES[x.dtype], M, D, F, ACTIVATIONS[act], ptr(h), F, ptr(saved),
+                             ptr(scratch), _stream(dev)))
+    return (h, saved) if save else h
+
+
+def gated_ffn_grad(d_h, x, w_gate, w_up, saved, act="silu"):
+    """(d_x, d_w_gate, d_w_up) of `gated_ffn` for the gradient d_h [M, F] of its result; `saved` as the forward call gave it."""
+    dev, ldx, ldw, M, D, F = _gated_args(x, w_gate, w_up, act)
+    _device(x=x, d_h=d_h, saved=saved)
+    lddh = _matrix("d_h", d_h, F, M, x.dtype)
+    _need(saved.dtype == torch.float32 and tuple(saved.shape) == (2, M, F) and saved.is_contiguous(),
+          f"saved is what gated_ffn(save=True) gave: [2, {M}, {F}] in fp32 (got {saved.dtype}, {tuple(saved.shape)}, strides {saved.stride()})")
+    d_x = torch.empty(M, D, dtype=x.dtype, device=dev)
+    d_wg, d_wu = (torch.empty(F, D, dtype=x.dtype, device=dev) for _ in range(2))
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        scratch = _scratch(L.gs_gated_bwd_scratch_bytes(M, D, F, TYPES[x.dtype]), dev)
+        check(L.gs_gated_bwd(ptr(d_h), lddh, ptr(x), ldx, ptr(w_gate), ptr(w_up), ldw, ptr(saved), TYPES[x.dtype], M, D, F,
+                             ACTIVATIONS[act], ptr(d_x), D, ptr(d_wg), ptr(d_wu), D, ptr(scratch), _stream(dev)))
+    return d_x, d_wg, d_wu
+
+
+# ------------------------------------------------------------------------------------------------
+# distillation
+# ------------------------------------------------------------------------------------------------
+
+
+def _distill_args(logits, top_values, top_ids, tau):
+    dev = _device(logits=logits, top_values=top_values, top_ids=top_ids)
+    ldz = _matrix("logits", logits)
+    n, V = logits.shape
+    _need(top_values.dim() == 2 and top_values.shape[0] == n and top_values.is_contiguous(),
+          f"top_values are dense, one row a row of logits (got {tuple(top_values.shape)}, strides {top_values.stride()})")
+    _need(top_values.dtype == logits.dtype, f"top_values are {top_values.dtype}, logits {logits.dtype}")
+    k = top_values.shape[1]
+    _need(1 <= k <= MAX_TOP, f"1 to {MAX_TOP} teacher entries a row (got {k})")
+    _need(tuple(top_ids.shape) == (n, k), f"top_ids are {tuple(top_ids.shape)}, top_values {(n, k)}")
+    _ids(top_ids)
+    tau = float(tau)
+    _need(0 < tau < math.inf, f"a temperature of {tau}")
+    return dev, (ptr(logits), ldz, TYPES[logits.dtype], n, V, ptr(top_values), ptr(top_ids), k, tau), n
+
+
+def _grad_out(logits, out):
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _device(logits=logits, out=out)
+    return out, _matrix("out", out, logits.shape[1], logits.shape[0], logits.dtype)
+
+
+def distill(logits, top_values, top_ids, tau=1.0):
+    """(loss, lse), one fp32 value a row: loss = tau^2 KL(p || q) with p the softmax of the teacher's top logits / tau over the
+    row's entries and q that of logits / tau over all classes; lse = log sum exp(logits / tau), which `distill_grad` takes.
+    An entry whose class (top_ids) is none of the logits', or whose value is -inf, is not there; a row without any has loss 0."""
+    dev, args, n = _distill_args(logits, top_values, top_ids, tau)
+    loss, lse = (torch.empty(n, dtype=torch.float32, device=dev) for _ in range(2))
+    with torch.cuda.device(dev):
+        check(_lib.lib().gs_distill_fwd(*args, ptr(loss), ptr(lse), _stream(dev)))
+    return loss, lse
+
+
+def distill_grad(logits, top_values, top_ids, lse, d_loss, tau=1.0, out=None):
+    """Gradient of sum(d_loss * loss) with respect to the logits, in their type; rows with d_loss 0 or without teacher entries get 0.
+    out=logits overwrites them."""
+    dev, args, n = _distill_args(logits, top_values, top_ids, tau)
+    _device(logits=logits, lse=lse, d_loss=d_loss)
+    _vector("lse", lse, n, torch.float32)
+    _vector("d_loss", d_loss, n, torch.float32)
+    out, ldd = _grad_out(logits, out)
+    with torch.cuda.device(dev):
+        check(_lib.lib().gs_distill_bwd(*args, ptr(lse), ptr(d_loss), ptr(out), ldd, _stream(dev)))
+    return out
+
+
+def distill_loss_grad(logits, top_values, top_ids, d_loss, tau=1.0, out=None):
+    """(loss, gradient) in one call, for row weights d_loss that are known beforehand (1 / n for a mean): the logits are read once
+    where a row fits the registers of a workgroup."""
+    dev, args, n = _distill_args(logits, top_values, top_ids, tau)
+    _device(logits=logits, d_loss=d_loss)
+    _vector("d_loss", d_loss, n, torch.float32)
+    out, ldd = _grad_out(logits, out)
+    loss = torch.empty(n, dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        check(_lib.lib().gs_distill_loss_grad(*args, ptr(d_loss), ptr(loss), ptr(out), ldd, _stream(dev)))
+    return loss, out

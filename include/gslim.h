@@ -299,6 +299,61 @@ int gs_ot_divdiff_f32(float* K, const float* lam, const float* g, const float* g
                       gs_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Training a student on a teacher's top logits: rows of a table by id and the table's gradient, the gated feed-forward block, the
+ * distillation loss.  Rows are held in 32 or 16 bits (`type`: one of GS_TYPE_*); everything is computed and summed in fp32 and
+ * rounded once when it is stored, and every sum has a fixed order (no float atomics: two runs are bitwise equal).  Row strides are in
+ * elements; rows may start at any element's address.  `scratch` is device memory of at least the bytes that the call's
+ * *_scratch_bytes function names, 16-byte aligned; nothing in it is kept between calls, and calls that may run at the same time
+ * (on different streams, or in different captured graphs) need scratch of their own.  No call allocates, synchronises or copies to
+ * the host: all of them can be captured into a graph.
+ * ------------------------------------------------------------------------------------------- */
+#define GS_TYPE_F32 0
+#define GS_TYPE_F16 1
+#define GS_TYPE_BF16 2
+
+/* out[t] = scale * W[ids[t]] (W: [n_rows][ldw], F columns); an id outside [0, n_rows) is padding and gives a row of zeros.
+ * The typed, scaled form of gs_gather_rows_f32. */
+int gs_embedding_fwd(const void* W, long ldw, long n_rows, int F, int type, const int* ids, long n, float scale, void* out, long ldo,
+                     gs_stream_t stream);
+/* dW[v] = scale * sum of dout[t] over the t with ids[t] == v, in ascending t (+ dW[v] when `accumulate`); rows that no id names get
+ * 0 (or stay).  type_dw: that of dout, or GS_TYPE_F32.  gs_segment_sum_rows_f32 with the permutation built on the device. */
+size_t gs_embedding_bwd_scratch_bytes(long n, long n_rows, int F);
+int gs_embedding_bwd(const void* dout, long ldd, int type, const int* ids, long n, long n_rows, int F, float scale, int accumulate,
+                     void* dW, long ldw, int type_dw, void* scratch, gs_stream_t stream);
+
+/* Gated feed-forward block: h = act(x Wg^T) * (x Wu^T), x [M][D], Wg and Wu [F][D] (one stride), h [M][F].  `saved` (may be NULL)
+ * receives x Wg^T and x Wu^T, [2][M][F] in fp32, for the backward call: two roundings to 16 bits there would cost more accuracy than
+ * the one of the result. */
+#define GS_ACT_SILU 0
+#define GS_ACT_GELU 1      /* the exact one: x Phi(x) */
+#define GS_ACT_RELU 2
+#define GS_ACT_SIGMOID 3
+size_t gs_gated_fwd_scratch_bytes(long M, long D, long F, int type);
+int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, long ldw, int type, long M, long D, long F, int act,
+                 void* h, long ldh, float* saved, void* scratch, gs_stream_t stream);
+/* dg = dh * u * act'(g), du = dh * act(g) (rounded to the operands' type: the products take them there); dx = dg Wg + du Wu,
+ * dw_gate = dg^T x, dw_up = du^T x. */
+size_t gs_gated_bwd_scratch_bytes(long M, long D, long F, int type);
+int gs_gated_bwd(const void* dh, long lddh, const void* x, long ldx, const void* w_gate, const void* w_up, long ldw, const float* saved,
+                 int type, long M, long D, long F, int act, void* dx, long lddx, void* dw_gate, void* dw_up, long lddw, void* scratch,
+                 gs_stream_t stream);
+
+/* Distillation from a teacher's top logits.  Z: student logits [n][ldz] over V classes; top_val, top_cls: [n][k] teacher logits and
+ * their classes, contiguous (k <= 1024).  p = softmax(top_val / tau) over a row's entries, q = softmax(Z / tau) over the classes:
+ *   loss[i] = tau^2 sum_j p_j (log p_j - log q_{c_j}),   dZ[i][v] = d_loss[i] tau (q_v - sum_{j : c_j = v} p_j).
+ * An entry whose class is outside [0, V) or whose logit is -inf is not there.  A row without entries has loss 0 and gradient 0, and
+ * its logits do not matter; a row with d_loss 0 has gradient 0.  Where all logits of a row are -inf, q is 0.  The soft-label
+ * counterpart of gs_softmax_nll_grad_f32; dZ may be Z.
+ * gs_distill_fwd also writes lse[i] = log sum_v exp(Z[i][v] / tau), which gs_distill_bwd takes; gs_distill_loss_grad is both at
+ * once for row weights that are known beforehand (1 / n). */
+int gs_distill_fwd(const void* Z, long ldz, int type, long n, int V, const void* top_val, const int* top_cls, int k, float tau,
+                   float* loss, float* lse, gs_stream_t stream);
+int gs_distill_bwd(const void* Z, long ldz, int type, long n, int V, const void* top_val, const int* top_cls, int k, float tau,
+                   const float* lse, const float* d_loss, void* dZ, long ldd, gs_stream_t stream);
+int gs_distill_loss_grad(const void* Z, long ldz, int type, long n, int V, const void* top_val, const int* top_cls, int k, float tau,
+                         const float* d_loss, float* loss, void* dZ, long ldd, gs_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * The GCond engine: one object per GPU holding the learnable synthetic graph (X~, PGE), the
  * per-epoch SGC model and all scratch.  One gs_gcond_outer_step == one iteration of the loop body
  * condensation/gcond.py:47-72 (PGE forward + dense_gcn_norm, train_class over all classes
