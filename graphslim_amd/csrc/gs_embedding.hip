@@ -29,42 +29,454 @@ __global__ __launch_bounds__(256) void gs_embedding_fwd_kernel(const typename Gs
   gs_store<E, N>(out + t * ldo + f, F - f, v);
 }
 
-// One wave per (table row, 64 N columns): it walks all ids and adds the rows of its own, in order.
-template <int T, int TO>
-__global__ __launch_bounds__(256) void gs_embedding_bwd_kernel(const typename GsElt<T>::type* __restrict__ dout, long ldd,
-                                                               const int* __restrict__ ids, long n, long V, int F, float scale,
-                                                               int accumulate, typename GsElt<TO>::type* __restrict__ dW, long ldw) {
-  typedef typename GsElt<T>::type E;
-  typedef typename GsElt<TO>::type EO;
-  constexpr int N = 16 / sizeof(E);
-  const int lane = threadIdx.x & 63;
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= V) return;
-  const int f = (blockIdx.y * 64 + lane) * N;
-  float acc[N];
+// ---- the gradient ---------------------------------------------------------------------------------------------------------------
+// The table is cut into buckets of R consecutive rows.  The tokens of a bucket, sorted by row (stable, so ascending within a row), are
+// walked by the waves of one workgroup, each on columns of its own: a run of one row is summed in registers and written once, rows
+// without tokens are written as zeros, and nothing is joined between waves.
+//   few tokens:  one launch, every workgroup picks its bucket's tokens out of all ids itself.
+//   many:        gs_embedding_count / _place sort the tokens by bucket first; a bucket of more than EM_SPAN tokens (a frequent id) is
+//                cut into spans with a workgroup each, whose sums gs_embedding_join adds in the spans' order.
+constexpr int EM_TILE = 1024;      // ids per workgroup of the sort: four a thread, all loaded at once
+constexpr int EM_WAVES = 8;        // waves of a workgroup that sums
+constexpr int EM_SPAN = 256;       // tokens of a bucket per workgroup
+constexpr int EM_MAX_BUCKETS = 2048;
+constexpr int EM_MAX_R = 1024;     // rows of a bucket at most
+constexpr long EM_MAX_V = (long)EM_MAX_R * EM_MAX_BUCKETS;
+constexpr long EM_DIRECT = 6144;   // tokens up to which one launch does it all
+
+struct EmbPlan {
+  int R, nb, nbp;      // rows per bucket (a power of two), buckets, rounded up to 8
+  int tiles, extra;    // sort tiles; workgroups for the second and further spans
+  bool direct;
+  size_t cnt, start, xs, list, ptrs, part, bytes;
+};
+
+EmbPlan emb_plan(long n, long V, int F) {
+  EmbPlan p;
+  p.R = 4;
+  while ((V + p.R - 1) / p.R > 1024 && p.R < 64) p.R *= 2;
+  while ((V + p.R - 1) / p.R > EM_MAX_BUCKETS) p.R *= 2;
+  p.nb = gs_cdiv(V, p.R);
+  p.direct = n <= EM_DIRECT && p.R <= 64;
+  p.tiles = gs_cdiv(n, EM_TILE);
+  p.extra = (int)(n / EM_SPAN);
+  size_t o = 0;
+  auto take = [&](size_t bytes) { size_t at = o; o += (bytes + 255) / 256 * 256; return at; };
+  p.nbp = (p.nb + 7) / 8 * 8;
+  p.cnt = take((size_t)p.tiles * p.nbp * 4);
+  p.start = take((size_t)(p.nb + 1) * 4);
+  p.xs = take((size_t)(p.nb + 1) * 4);
+  p.list = take((size_t)n * 8);
+  p.ptrs = take((size_t)2 * p.extra * p.R * 4);
+  p.part = take((size_t)2 * p.extra * (p.R < EM_SPAN ? p.R : EM_SPAN) * F * 4);
+  p.bytes = p.direct ? 0 : o;
+  return p;
+}
+
+// lanes of this wave whose `key` (below 2^bits) is mine, among those with `on`
+__device__ __forceinline__ unsigned long long emb_match(int key, bool on, int bits) {
+  unsigned long long m = __ballot(on);
+  for (int b = 0; b < bits; ++b) {
+    const bool set = (key >> b) & 1;
+    const unsigned long long have = __ballot(set);
+    m &= set ? have : ~have;
+  }
+  return m;
+}
+
+// cnt[tile][bucket]: tokens of the tile in the bucket (rows of nbp = nb rounded up to 8 counts)
+__global__ __launch_bounds__(256) void gs_embedding_count_kernel(const int* __restrict__ ids, long n, long V, int rshift, int nbp,
+                                                                 int* __restrict__ cnt) {
+  __shared__ int h[EM_MAX_BUCKETS];
+  const long t0 = (long)blockIdx.x * EM_TILE;
+  int id[EM_TILE / 256];
 #pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  for (long base = 0; base < n; base += 64) {
-    unsigned long long hit = __ballot(base + lane < n && ids[min(base + lane, n - 1)] == row);
-    while (hit) {
-      const long t = base + __ffsll(hit) - 1;
-      hit &= hit - 1;
-      if (f < F) {
-        float v[N];
-        gs_load<E, N>(dout + t * ldd + f, F - f, 0.f, v);
+  for (int i = 0; i < EM_TILE / 256; ++i) {
+    const long t = t0 + i * 256 + threadIdx.x;
+    id[i] = t < n ? ids[t] : -1;
+  }
+  for (int b = threadIdx.x; b < nbp; b += 256) h[b] = 0;
+  __syncthreads();
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] += v[i];
+  for (int i = 0; i < EM_TILE / 256; ++i)
+    if (id[i] >= 0 && id[i] < V) atomicAdd(&h[id[i] >> rshift], 1);
+  __syncthreads();
+  for (int b = threadIdx.x; b < nbp; b += 256) cnt[(long)blockIdx.x * nbp + b] = h[b];
+}
+
+// Stable: a tile's place in a bucket follows from the counts of the tiles before it, a wave's from those of the waves before it, a
+// lane's from the lanes before it.  start[b]: where bucket b begins in the list; xs[b]: further spans of the buckets before b.
+__global__ __launch_bounds__(256) void gs_embedding_place_kernel(const int* __restrict__ ids, long n, long V, int rshift, int nb, int nbp,
+                                                                 int bits, const int* __restrict__ cnt, int tiles,
+                                                                 int* __restrict__ start, int* __restrict__ xs, int2* __restrict__ list) {
+  __shared__ int pos[4][EM_MAX_BUCKETS];     // per wave: the next place of each bucket
+  __shared__ int wsum[4], wext[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int Q = EM_TILE / 256;
+  const long t0 = (long)blockIdx.x * EM_TILE + wave * (EM_TILE / 4) + lane;
+  int id[Q];
+#pragma unroll
+  for (int i = 0; i < Q; ++i) {
+    id[i] = t0 + i * 64 < n ? ids[t0 + i * 64] : -1;
+    if (id[i] >= V) id[i] = -1;
+  }
+  for (int b = tid; b < nb; b += 256) pos[0][b] = pos[1][b] = pos[2][b] = pos[3][b] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < Q; ++i)
+    if (id[i] >= 0) atomicAdd(&pos[wave][id[i] >> rshift], 1);
+  constexpr int PER = EM_MAX_BUCKETS / 256;  // consecutive buckets of a thread, so that its prefix is a running one
+  static_assert(PER == 8, "two 16-byte loads");
+  int before[PER] = {}, all[PER] = {}, mine = 0, ext = 0;
+  if (tid * PER < nbp) {
+    const int4* c = (const int4*)(cnt + tid * PER);
+#pragma unroll 4
+    for (int t = 0; t < tiles; ++t) {
+      const int4 u = c[(long)t * (nbp / 4)], v = c[(long)t * (nbp / 4) + 1];
+      const int x[PER] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        all[j] += x[j];
+        before[j] += t < (int)blockIdx.x ? x[j] : 0;
       }
     }
   }
-  if (f >= F) return;
-  EO* o = dW + row * ldw + f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    acc[i] *= scale;
-    if (accumulate && f + i < F) acc[i] += (float)o[i];
+  for (int j = 0; j < PER; ++j) {
+    mine += all[j];
+    ext += all[j] > 0 ? (all[j] - 1) / EM_SPAN : 0;
   }
-  gs_store<EO, N>(o, F - f, acc);
+  int inc = mine, einc = ext;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int a = __shfl_up(inc, o, 64), e = __shfl_up(einc, o, 64);
+    if (lane >= o) { inc += a; einc += e; }
+  }
+  if (lane == 63) { wsum[wave] = inc; wext[wave] = einc; }
+  __syncthreads();
+  int base = inc - mine, ebase = einc - ext;
+  for (int w = 0; w < wave; ++w) { base += wsum[w]; ebase += wext[w]; }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int b = tid * PER + j;
+    if (b >= nb) break;
+    if (blockIdx.x == 0) { start[b] = base; xs[b] = ebase; }
+    int at = base + before[j];
+    for (int w = 0; w < 4; ++w) {
+      const int c = pos[w][b];
+      pos[w][b] = at;
+      at += c;
+    }
+    base += all[j];
+    ebase += all[j] > 0 ? (all[j] - 1) / EM_SPAN : 0;
+    if (blockIdx.x == 0 && b == nb - 1) { start[nb] = base; xs[nb] = ebase; }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < Q; ++i) {
+    const bool on = id[i] >= 0;
+    const int b = on ? id[i] >> rshift : 0;
+    const unsigned long long same = emb_match(b, on, bits);
+    if (on) {
+      volatile int* p = &pos[wave][b];
+      const int at = *p;
+      list[at + __popcll(same & ((1ull << lane) - 1))] = make_int2((int)(t0 + i * 64), id[i]);
+      if ((same >> lane) == 1) *p = at + __popcll(same);     // the last lane of its kind, after all have read (one wave, in order)
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+struct EmbSum {
+  const int* ids;        // direct: all ids
+  const int* start;      // sorted: as gs_embedding_place_kernel left them
+  const int* xs;
+  const int2* list;
+  int* ptrs;             // [2 extra][R]: place of a row's sum in its span's slot or -1, where a bucket has several spans
+  float* part;           // [2 extra][slot rows][F]: their sums
+  const void* dout;
+  long ldd;
+  void* dW;
+  long ldw;
+  long n, V;
+  int F, R, rshift, nb, extra, slot_rows, cap, cw;
+  float scale;
+  int accumulate;
+};
+
+// A lane's N columns begin at f0, a multiple of N; the last lane's would reach beyond the row, so it loads the row's last N columns
+// (from f on) and stores those from f0 on.  So every load is a whole vector, and a batch of them stays in flight.
+template <typename E, int N>
+__device__ __forceinline__ void emb_store(E* __restrict__ row, int f, int f0, const float* __restrict__ v) {
+  if (f == f0) {
+    gs_store<E, N>(row + f, N, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (f + i >= f0) row[f + i] = (E)v[i];
+  }
+}
+
+template <int TO, int N>
+__device__ __forceinline__ void emb_write(const EmbSum& a, long row, int f, int f0, float* acc) {
+  typedef typename GsElt<TO>::type EO;
+  EO* o = (EO*)a.dW + row * a.ldw;
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] *= a.scale;
+  if (a.accumulate) {
+    float old[N];
+    gs_load<EO, N>(o + f, N, 0.f, old);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] += old[i];
+  }
+  emb_store<EO, N>(o, f, f0, acc);
+}
+
+// One workgroup of EM_WAVES waves per span of a bucket's tokens and 64 N cw columns: cw waves side by side on the columns, EM_WAVES / cw
+// groups of them on consecutive parts of the sorted tokens, so that a frequent row is walked by several waves.  A run that crosses
+// from one part into the next is summed by the wave that it begins in, from what the others leave in LDS, in order.
+// Blocks [0, extra) are the further spans, the longest work, and begin first.
+template <int T, int TO, int N, bool DIRECT>
+__global__ __launch_bounds__(EM_WAVES * 64) void gs_embedding_sum_kernel(EmbSum a) {
+  typedef typename GsElt<T>::type E;
+  typedef typename GsElt<TO>::type EO;
+  typedef typename GsVec<E, N>::type V;
+  constexpr int U = 8, W = EM_WAVES;                   // rows of dout in flight per lane
+  extern __shared__ int dyn[];
+  int* ptr = dyn;                                      // [R + 1] where a row's tokens begin
+  int* cnt = ptr + a.R + 1;                            // [W][R] per wave: tokens of a row, then the next one's place
+  int* st = cnt + W * a.R;                             // [cap] tokens in order of their rows
+  unsigned short* sr = (unsigned short*)(st + a.cap);  // [cap] their rows in the bucket
+  unsigned short* place = sr + a.cap;                  // [R] rows with tokens before this one
+  __shared__ float slot_sum[W][64][N];                 // a wave's part of a run that began before its part
+  __shared__ int found[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int b, span = 0, spans = 1, i0 = 0, i1 = (int)a.n, slot = 0;
+  if (DIRECT) {
+    b = blockIdx.x;
+  } else {
+    if ((int)blockIdx.x < a.extra) {                   // which bucket this further span is of
+      if (tid == 0) found[0] = -1;
+      __syncthreads();
+      const int e = blockIdx.x;
+      for (int q = tid; q < a.nb; q += W * 64)
+        if (a.xs[q] <= e && e < a.xs[q + 1]) { found[0] = q; found[1] = e - a.xs[q] + 1; }
+      __syncthreads();
+      if (found[0] < 0) return;
+      b = found[0];
+      span = found[1];
+      slot = e;
+    } else {
+      b = blockIdx.x - a.extra;
+      slot = a.extra + a.xs[b];
+    }
+    spans = a.xs[b + 1] - a.xs[b] + 1;
+    i0 = a.start[b] + span * EM_SPAN;
+    i1 = min(i0 + EM_SPAN, a.start[b + 1]);
+  }
+  const long row0 = (long)b << a.rshift;
+  const int rows = (int)min((long)a.R, a.V - row0);
+  // stable counting sort of items [i0, i1) by row: each wave takes a share, in order
+  const int len = i1 - i0, q = ((len + W - 1) / W + 63) / 64 * 64;
+  const int w0 = min(i0 + wave * q, i1), w1 = min(w0 + q, i1);
+  auto item = [&](int i, int& t) -> int {              // its row in the bucket, or -1
+    if (i >= w1) return -1;
+    if (DIRECT) {
+      t = i;
+      const long r = (long)a.ids[i] - row0;
+      return r >= 0 && r < rows ? (int)r : -1;
+    }
+    const int2 v = a.list[i];
+    t = v.x;
+    return (int)(v.y - row0);
+  };
+  for (int i = tid; i < W * a.R; i += W * 64) cnt[i] = 0;
+  __syncthreads();
+  constexpr int P = DIRECT ? 8 : 1;                    // items in flight per lane
+  for (int i = w0; i < w1; i += 64 * P) {
+    int t, r[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) r[j] = item(i + j * 64 + lane, t);
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+      if (r[j] >= 0) atomicAdd(&cnt[wave * a.R + r[j]], 1);
+  }
+  __syncthreads();
+  if (wave == 0) {                                     // exclusive prefix, row by row and within a row wave by wave
+    int run = 0, kept = 0;
+    for (int base = 0; base < a.R; base += 64) {
+      const int r = base + lane;
+      int c[W], sum = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) { c[w] = r < a.R ? cnt[w * a.R + r] : 0; sum += c[w]; }
+      int inc = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(inc, o, 64); if (lane >= o) inc += v; }
+      const unsigned long long have = __ballot(sum > 0);
+      int at = run + inc - sum;
+      if (r < a.R) {
+        ptr[r] = at;
+        place[r] = (unsigned short)(kept + __popcll(have & ((1ull << lane) - 1)));
+#pragma unroll
+        for (int w = 0; w < W; ++w) { cnt[w * a.R + r] = at; at += c[w]; }
+      }
+      run += __shfl(inc, 63, 64);
+      kept += __popcll(have);
+    }
+    if (lane == 0) ptr[a.R] = run;
+  }
+  __syncthreads();
+  for (int i = w0; i < w1; i += 64 * P) {
+    int t[P], r[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) r[j] = item(i + j * 64 + lane, t[j]);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      if (!__ballot(r[j] >= 0)) continue;
+      const unsigned long long same = emb_match(r[j], r[j] >= 0, a.rshift);
+      if (r[j] >= 0) {
+        volatile int* p = &cnt[wave * a.R + r[j]];
+        const int at = *p;
+        const int to = at + __popcll(same & ((1ull << lane) - 1));
+        st[to] = t[j];
+        sr[to] = (unsigned short)r[j];
+        if ((same >> lane) == 1) *p = at + __popcll(same);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  __syncthreads();
+  const int total = ptr[a.R];
+  const bool whole = spans == 1;
+  if (!whole && blockIdx.y == 0)
+    for (int r = tid; r < a.R; r += W * 64) a.ptrs[(long)slot * a.R + r] = ptr[r] < ptr[r + 1] ? place[r] : -1;
+
+  const int tw = wave / a.cw, groups = W / a.cw;
+  const int f0 = ((int)blockIdx.y * a.cw + wave % a.cw) * 64 * N + lane * N, f = min(f0, a.F - N);
+  const bool on = f0 < a.F;
+  const int p0 = (int)((long)total * tw / groups), p1 = (int)((long)total * (tw + 1) / groups);
+  const E* src = (const E*)a.dout + f;
+  float* part = a.part + (long)slot * a.slot_rows * a.F;
+  float acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  const int before = p0 > 0 ? __builtin_amdgcn_readfirstlane(sr[p0 - 1]) : -1;
+  int cur = -1, next = before + 1;                     // row being summed, first row not written yet
+  bool foreign = false;                                // cur's run began before this part
+  auto fill = [&](int upto) {                          // zeros for the rows without tokens below `upto`
+    if (whole && !a.accumulate && on) {
+      const float z[N] = {};
+      for (; next < upto; ++next) emb_store<EO, N>((EO*)a.dW + (row0 + next) * a.ldw, f, f0, z);
+    }
+  };
+  auto finish = [&]() {                                // the sum of row cur
+    if (cur >= 0) {
+      if (foreign) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) slot_sum[wave][lane][i] = acc[i];
+      } else if (on) {
+        if (whole) emb_write<TO, N>(a, row0 + cur, f, f0, acc);
+        else emb_store<float, N>(part + (long)place[cur] * a.F, f, f0, acc);
+      }
+      next = cur + 1;
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    }
+  };
+  for (int base = p0; base < p1; base += U) {
+    V v[U];
+    int r[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int at = min(base + j, p1 - 1);
+      const int t = __builtin_amdgcn_readfirstlane(st[at]);
+      r[j] = __builtin_amdgcn_readfirstlane(sr[at]);
+      v[j] = *(const V*)(src + (long)t * a.ldd);
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (base + j < p1) {
+        if (r[j] != cur) {
+          finish();
+          foreign = cur < 0 && r[j] == before;
+          cur = r[j];
+          fill(cur);
+        }
+        if constexpr (N == 1) {
+          acc[0] += (float)v[j];
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) acc[i] += (float)v[j][i];
+        }
+      }
+    }
+  }
+  const bool open = p0 < p1 && p1 < total && __builtin_amdgcn_readfirstlane(sr[p1]) == cur;   // goes on in the next part
+  if (!open || foreign) finish();
+  __syncthreads();
+  if (open && !foreign) {
+    for (int g = tw + 1; g < groups; ++g) {
+      const int q0 = (int)((long)total * g / groups), q1 = (int)((long)total * (g + 1) / groups);
+      if (q0 == q1) continue;
+      if (sr[q0] != cur) break;
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] += slot_sum[g * a.cw + wave % a.cw][lane][i];
+      if (sr[q1 - 1] != cur) break;
+    }
+    finish();
+  }
+  if (p1 == total && (p0 < p1 || (total == 0 && tw == 0))) fill(rows);
+}
+
+// Buckets of several spans: the sums of each row in the spans' order, a wave per row.  Blocks (e, ., .) work if e is a bucket's first
+// further span.
+template <int TO, int N>
+__global__ __launch_bounds__(256) void gs_embedding_join_kernel(EmbSum a) {
+  __shared__ int found;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int e = blockIdx.x;
+  if (tid == 0) found = -1;
+  __syncthreads();
+  for (int q = tid; q < a.nb; q += 256)
+    if (a.xs[q] == e && a.xs[q + 1] > e) found = q;
+  __syncthreads();
+  if (found < 0) return;
+  const int b = found, spans = a.xs[b + 1] - e + 1;
+  const long row0 = (long)b << a.rshift;
+  const int r = blockIdx.z * 4 + wave;
+  if (r >= (int)min((long)a.R, a.V - row0)) return;
+  const int f0 = blockIdx.y * 64 * N + lane * N, f = min(f0, a.F - N);
+  float acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  bool any = false;
+  for (int base = 0; base < spans; base += 64) {
+    const int s = base + lane;                         // a lane looks up one span's place for the row
+    const int slot = s == 0 ? a.extra + e : e + s - 1;
+    const int at = s < spans ? a.ptrs[(long)slot * a.R + r] : -1;
+    unsigned long long have = __ballot(at >= 0);
+    any |= have != 0;
+    while (have) {
+      constexpr int U = 4;
+      float v[U][N];
+      unsigned long long left = have;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int l = left ? __ffsll(left) - 1 : __ffsll(have) - 1;
+        const long at_l = (long)__shfl(slot, l, 64) * a.slot_rows + __shfl(at, l, 64);
+        gs_load<float, N>(a.part + at_l * a.F + f, N, 0.f, v[j]);
+        left &= left - 1;
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        if (!have) break;
+        have &= have - 1;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += v[j][i];
+      }
+    }
+  }
+  if (f0 < a.F && (any || !a.accumulate)) emb_write<TO, N>(a, row0 + r, f, f0, acc);
 }
 
 template <int T>
@@ -78,15 +490,52 @@ int emb_fwd(const void* W, long ldw, long V, int F, const int* ids, long n, floa
   return GS_OK;
 }
 
-template <int T, int TO>
-int emb_bwd(const void* dout, long ldd, const int* ids, long n, long V, int F, float scale, int accumulate, void* dW, long ldw,
-            hipStream_t s) {
-  typedef typename GsElt<T>::type E;
-  const dim3 grid((unsigned)gs_cdiv(V, 4), (unsigned)gs_cdiv(F, 64 * 16 / sizeof(E)));
-  gs_embedding_bwd_kernel<T, TO><<<grid, dim3(256), 0, s>>>((const E*)dout, ldd, ids, n, V, F, scale, accumulate,
-                                                          (typename GsElt<TO>::type*)dW, ldw);
+template <int T, int TO, int N>
+int emb_sum(const EmbPlan& p, EmbSum a, hipStream_t s) {
+  a.cw = 1;
+  while (a.cw < EM_WAVES && a.cw * 64 * N < a.F) a.cw *= 2;
+  const unsigned gy = (unsigned)gs_cdiv(a.F, a.cw * 64 * N);
+  a.cap = p.direct ? (int)(a.n > 0 ? a.n : 1) : EM_SPAN;
+  const size_t lds = (size_t)a.cap * 6 + (size_t)((EM_WAVES + 1) * p.R + 1) * 4 + (size_t)p.R * 2 + 2;
+  const dim3 block(EM_WAVES * 64);
+  if (p.direct) {
+    gs_embedding_sum_kernel<T, TO, N, true><<<dim3((unsigned)p.nb, gy), block, lds, s>>>(a);
+  } else {
+    gs_embedding_sum_kernel<T, TO, N, false><<<dim3((unsigned)(p.extra + p.nb), gy), block, lds, s>>>(a);
+    GS_LAUNCH_CHECK();
+    if (p.extra > 0)
+      gs_embedding_join_kernel<TO, N><<<dim3((unsigned)p.extra, (unsigned)gs_cdiv(a.F, 64 * N), (unsigned)gs_cdiv(p.R, 4)), dim3(256), 0, s>>>(a);
+  }
   GS_LAUNCH_CHECK();
   return GS_OK;
+}
+
+template <int T, int TO>
+int emb_bwd(const void* dout, long ldd, const int* ids, long n, long V, int F, float scale, int accumulate, void* dW, long ldw,
+            char* scratch, hipStream_t s) {
+  const EmbPlan p = emb_plan(n, V, F);
+  EmbSum a = {};
+  a.ids = ids; a.dout = dout; a.ldd = ldd; a.dW = dW; a.ldw = ldw; a.n = n; a.V = V; a.F = F; a.scale = scale; a.accumulate = accumulate;
+  a.R = p.R; a.nb = p.nb; a.extra = p.extra; a.slot_rows = p.R < EM_SPAN ? p.R : EM_SPAN;
+  while ((1 << a.rshift) < p.R) ++a.rshift;
+  if (!p.direct) {
+    int* start = (int*)(scratch + p.start);
+    int* xs = (int*)(scratch + p.xs);
+    int2* list = (int2*)(scratch + p.list);
+    int* cnt = (int*)(scratch + p.cnt);
+    int bits = 0;
+    while ((1 << bits) < p.nb) ++bits;
+    gs_embedding_count_kernel<<<dim3((unsigned)p.tiles), dim3(256), 0, s>>>(ids, n, V, a.rshift, p.nbp, cnt);
+    GS_LAUNCH_CHECK();
+    gs_embedding_place_kernel<<<dim3((unsigned)p.tiles), dim3(256), 0, s>>>(ids, n, V, a.rshift, p.nb, p.nbp, bits, cnt, p.tiles, start, xs, list);
+    GS_LAUNCH_CHECK();
+    a.start = start; a.xs = xs; a.list = list; a.ptrs = (int*)(scratch + p.ptrs); a.part = (float*)(scratch + p.part);
+  }
+  // columns per lane: 16 bytes of dout where the width has them, so that more waves share a frequent row
+  constexpr int N = T == GS_TYPE_F32 ? 4 : 8;
+  if (F >= 64 * N) return emb_sum<T, TO, N>(p, a, s);
+  if (F >= 128) return emb_sum<T, TO, 2>(p, a, s);
+  return emb_sum<T, TO, 1>(p, a, s);
 }
 
 int emb_check(const char* who, long n, long V, int F, int type, long ld0, long ld1) {
@@ -110,19 +559,24 @@ extern "C" int gs_embedding_fwd(const void* W, long ldw, long V, int F, int type
   return emb_fwd<GS_TYPE_BF16>(W, ldw, V, F, ids, n, scale, out, ldo, s);
 }
 
-extern "C" size_t gs_embedding_bwd_scratch_bytes(long n, long V, int F) { return 0; }
+extern "C" size_t gs_embedding_bwd_scratch_bytes(long n, long V, int F) {
+  return n < 0 || V < 1 || F < 1 || V > EM_MAX_V || n > 0x7fffffffL ? 0 : emb_plan(n, V, F).bytes;
+}
 
 extern "C" int gs_embedding_bwd(const void* dout, long ldd, int type, const int* ids, long n, long V, int F, float scale, int accumulate,
                                 void* dW, long ldw, int type_dw, void* scratch, gs_stream_t stream) {
   GS_TRY(emb_check("gs_embedding_bwd", n, V, F, type, ldd, ldw));
   if (type_dw != type && type_dw != GS_TYPE_F32)
     GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: the gradient is held in the type of d_out or in fp32 (got %d for %d)", type_dw, type);
+  if (V > EM_MAX_V) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_embedding_bwd: tables of at most %ld rows (got %ld)", EM_MAX_V, V);
   if (!dW || (n > 0 && (!dout || !ids))) GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: null pointer");
+  if (gs_embedding_bwd_scratch_bytes(n, V, F) > 0 && (!scratch || ((size_t)scratch & 15)))
+    GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: the scratch is missing or not 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;
-  if (type == GS_TYPE_F32) return emb_bwd<GS_TYPE_F32, GS_TYPE_F32>(dout, ldd, ids, n, V, F, scale, accumulate, dW, ldw, s);
+  if (type == GS_TYPE_F32) return emb_bwd<GS_TYPE_F32, GS_TYPE_F32>(dout, ldd, ids, n, V, F, scale, accumulate, dW, ldw, (char*)scratch, s);
   if (type == GS_TYPE_F16)
-    return type_dw == GS_TYPE_F16 ? emb_bwd<GS_TYPE_F16, GS_TYPE_F16>(dout, ldd, ids, n, V, F, scale, accumulate, dW, ldw, s)
-                                  : emb_bwd<GS_TYPE_F16, GS_TYPE_F32>(dout, ldd, ids, n, V, F, scale, accumulate, dW, ldw, s);
-  return type_dw == GS_TYPE_BF16 ? emb_bwd<GS_TYPE_BF16, GS_TYPE_BF16>(dout, ldd, ids, n, V, F, scale, accumulate, dW, ldw, s)
-                                 : emb_bwd<GS_TYPE_BF16, GS_TYPE_F32>(dout, ldd, ids, n, V, F, scale, accumulate, dW, ldw, s);
+    return type_dw == GS_TYPE_F16 ? emb_bwd<GS_TYPE_F16, GS_TYPE_F16>(dout, ldd, ids, n, V, F, scale, accumulate, dW, ldw, (char*)scratch, s)
+                                  : emb_bwd<GS_TYPE_F16, GS_TYPE_F32>(dout, ldd, ids, n, V, F, scale, accumulate, dW, ldw, (char*)scratch, s);
+  return type_dw == GS_TYPE_BF16 ? emb_bwd<GS_TYPE_BF16, GS_TYPE_BF16>(dout, ldd, ids, n, V, F, scale, accumulate, dW, ldw, (char*)scratch, s)
+                                 : emb_bwd<GS_TYPE_BF16, GS_TYPE_F32>(dout, ldd, ids, n, V, F, scale, accumulate, dW, ldw, (char*)scratch, s);
 }

@@ -17,60 +17,83 @@ import math
 import torch
 
 from . import _lib
-from ._lib import check, ptr, vp
+from ._lib import check
 
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 MAX_TOP = 1024
 
 
-def _need(ok, message):
-    if not ok:
-        raise ValueError(f"graphslim_amd.ops: {message}")
+def _refuse(message):
+    raise ValueError(f"graphslim_amd.ops: {message}")
 
 
 def _device(**tensors):
     """The one GPU all of them are on."""
     dev = None
     for name, t in tensors.items():
-        _need(isinstance(t, torch.Tensor), f"{name} is a tensor (got {type(t).__name__})")
-        _need(t.device.type == "cuda", f"{name} is on {t.device}: there is no CPU path")
-        _need(dev is None or t.device == dev, f"{name} is on {t.device}, other arguments on {dev}")
+        if not isinstance(t, torch.Tensor):
+            _refuse(f"{name} is a tensor (got {type(t).__name__})")
+        if t.device.type != "cuda":
+            _refuse(f"{name} is on {t.device}: there is no CPU path")
+        if not (dev is None or t.device == dev):
+            _refuse(f"{name} is on {t.device}, other arguments on {dev}")
         dev = t.device
     return dev
 
 
 def _matrix(name, t, cols=None, rows=None, dtype=None):
     """Row stride of a 2-D tensor with dense rows."""
-    _need(t.dim() == 2, f"{name} has two dimensions (got {tuple(t.shape)})")
-    _need(t.dtype in TYPES, f"{name} is fp32, fp16 or bf16 (got {t.dtype})")
-    _need(dtype is None or t.dtype == dtype, f"{name} is {t.dtype}, other arguments {dtype}")
-    _need(cols is None or t.shape[1] == cols, f"{name} has {t.shape[1]} columns, {cols} are wanted")
-    _need(rows is None or t.shape[0] == rows, f"{name} has {t.shape[0]} rows, {rows} are wanted")
-    _need(t.shape[1] > 0, f"{name} has no columns")
-    _need(t.shape[1] == 1 or t.stride(1) == 1, f"the rows of {name} are not dense (strides {t.stride()})")
+    if t.dim() != 2:
+        _refuse(f"{name} has two dimensions (got {tuple(t.shape)})")
+    if t.dtype not in TYPES:
+        _refuse(f"{name} is fp32, fp16 or bf16 (got {t.dtype})")
+    if not (dtype is None or t.dtype == dtype):
+        _refuse(f"{name} is {t.dtype}, other arguments {dtype}")
+    if not (cols is None or t.shape[1] == cols):
+        _refuse(f"{name} has {t.shape[1]} columns, {cols} are wanted")
+    if not (rows is None or t.shape[0] == rows):
+        _refuse(f"{name} has {t.shape[0]} rows, {rows} are wanted")
+    if t.shape[1] <= 0:
+        _refuse(f"{name} has no columns")
+    if not (t.shape[1] == 1 or t.stride(1) == 1):
+        _refuse(f"the rows of {name} are not dense (strides {t.stride()})")
     if t.shape[0] <= 1:
         return t.shape[1]
-    _need(t.stride(0) >= t.shape[1], f"the rows of {name} overlap (strides {t.stride()})")
+    if t.stride(0) < t.shape[1]:
+        _refuse(f"the rows of {name} overlap (strides {t.stride()})")
     return t.stride(0)
 
 
 def _vector(name, t, n, dtype):
-    _need(t.dtype == dtype, f"{name} is {dtype} (got {t.dtype})")
-    _need(tuple(t.shape) == (n,) and t.is_contiguous(), f"{name} is a dense vector of {n} (got {tuple(t.shape)}, strides {t.stride()})")
+    if t.dtype != dtype:
+        _refuse(f"{name} is {dtype} (got {t.dtype})")
+    if not (tuple(t.shape) == (n,) and t.is_contiguous()):
+        _refuse(f"{name} is a dense vector of {n} (got {tuple(t.shape)}, strides {t.stride()})")
 
 
 def _ids(ids):
-    _need(ids.dtype == torch.int32, f"ids are int32 (got {ids.dtype})")
-    _need(ids.is_contiguous(), f"ids are dense (strides {ids.stride()})")
+    if ids.dtype != torch.int32:
+        _refuse(f"ids are int32 (got {ids.dtype})")
+    if not ids.is_contiguous():
+        _refuse(f"ids are dense (strides {ids.stride()})")
 
 
 def _scratch(nbytes, dev):
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=dev)
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
 
 
-def _stream(dev):
-    return vp(torch.cuda.current_stream(dev).cuda_stream)
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _launch(dev, call, *args):
+    """call(*args, stream) on the current stream of `dev`, with that device the current one."""
+    if dev.index == torch.cuda.current_device():
+        check(call(*args, torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            check(call(*args, torch.cuda.current_stream(dev).cuda_stream))
 
 
 # ------------------------------------------------------------------------------------------------
@@ -83,7 +106,8 @@ def embedding(table, ids, scale=1.0, out=None):
     [ids.numel(), width] matrix that receives the rows and is returned as it is."""
     dev = _device(table=table, ids=ids)
     ld = _matrix("table", table)
-    _need(table.shape[0] > 0, "table has no rows")
+    if table.shape[0] <= 0:
+        _refuse("table has no rows")
     _ids(ids)
     n, F = ids.numel(), table.shape[1]
     if out is None:
@@ -93,9 +117,8 @@ def embedding(table, ids, scale=1.0, out=None):
         _device(table=table, out=out)
         ldo = _matrix("out", out, F, n, table.dtype)
         res = out
-    with torch.cuda.device(dev):
-        check(_lib.lib().gs_embedding_fwd(ptr(table), ld, table.shape[0], F, TYPES[table.dtype], ptr(ids), n, float(scale), ptr(res), ldo,
-                                          _stream(dev)))
+    _launch(dev, _lib.lib().gs_embedding_fwd, table.data_ptr(), ld, table.shape[0], F, TYPES[table.dtype], ids.data_ptr(), n, scale,
+            res.data_ptr(), ldo)
     return res if out is not None else res.view(*ids.shape, F)
 
 
@@ -107,28 +130,33 @@ def embedding_grad(d_out, ids, n_rows, scale=1.0, out=None, accumulate=False, dt
     _ids(ids)
     n = ids.numel()
     if d_out.dim() != 2:
-        _need(d_out.dim() >= 1 and tuple(d_out.shape[:-1]) == tuple(ids.shape),
-              f"d_out is {tuple(d_out.shape)}, ids are {tuple(ids.shape)}")
-        _need(d_out.is_contiguous(), f"d_out is dense, or a matrix (strides {d_out.stride()})")
+        if not (d_out.dim() >= 1 and tuple(d_out.shape[:-1]) == tuple(ids.shape)):
+            _refuse(f"d_out is {tuple(d_out.shape)}, ids are {tuple(ids.shape)}")
+        if not d_out.is_contiguous():
+            _refuse(f"d_out is dense, or a matrix (strides {d_out.stride()})")
         d_out = d_out.view(n, d_out.shape[-1])
     ldd = _matrix("d_out", d_out, rows=n)
     n_rows, F = int(n_rows), d_out.shape[1]
-    _need(n_rows > 0, f"a table of {n_rows} rows")
+    if n_rows <= 0:
+        _refuse(f"a table of {n_rows} rows")
     if out is None:
-        _need(not accumulate, "accumulate=True adds to `out`, which is missing")
+        if not (not accumulate):
+            _refuse("accumulate=True adds to `out`, which is missing")
         dtype = d_out.dtype if dtype is None else dtype
-        _need(dtype in (d_out.dtype, torch.float32), f"the gradient is {d_out.dtype} or torch.float32 (got {dtype})")
+        if dtype not in (d_out.dtype, torch.float32):
+            _refuse(f"the gradient is {d_out.dtype} or torch.float32 (got {dtype})")
         out = torch.empty(n_rows, F, dtype=dtype, device=dev)
     else:
         _device(d_out=d_out, out=out)
-        _need(dtype in (None, out.dtype), f"out is {out.dtype}, dtype {dtype}")
-        _need(out.dtype in (d_out.dtype, torch.float32), f"the gradient is {d_out.dtype} or torch.float32 (got {out.dtype})")
+        if dtype not in (None, out.dtype):
+            _refuse(f"out is {out.dtype}, dtype {dtype}")
+        if out.dtype not in (d_out.dtype, torch.float32):
+            _refuse(f"the gradient is {d_out.dtype} or torch.float32 (got {out.dtype})")
     ldw = _matrix("out", out, F, n_rows)
     L = _lib.lib()
-    with torch.cuda.device(dev):
-        scratch = _scratch(L.gs_embedding_bwd_scratch_bytes(n, n_rows, F), dev)
-        check(L.gs_embedding_bwd(ptr(d_out), ldd, TYPES[d_out.dtype], ptr(ids), n, n_rows, F, float(scale), int(bool(accumulate)), ptr(out),
-                                 ldw, TYPES[out.dtype], ptr(scratch), _stream(dev)))
+    scratch = _scratch(L.gs_embedding_bwd_scratch_bytes(n, n_rows, F), dev)
+    _launch(dev, L.gs_embedding_bwd, d_out.data_ptr(), ldd, TYPES[d_out.dtype], ids.data_ptr(), n, n_rows, F, scale, bool(accumulate),
+            out.data_ptr(), ldw, TYPES[out.dtype], _ptr(scratch))
     return out
 
 
@@ -138,15 +166,18 @@ def embedding_grad(d_out, ids, n_rows, scale=1.0, out=None, accumulate=False, dt
 
 
 def _gated_args(x, w_gate, w_up, act):
-    _need(act in ACTIVATIONS, f"act is one of {', '.join(ACTIVATIONS)} (got {act!r})")
+    if act not in ACTIVATIONS:
+        _refuse(f"act is one of {', '.join(ACTIVATIONS)} (got {act!r})")
     dev = _device(x=x, w_gate=w_gate, w_up=w_up)
     ldx = _matrix("x", x)
     M, D = x.shape
     ldw = _matrix("w_gate", w_gate, D, dtype=x.dtype)
     F = w_gate.shape[0]
-    _need(F > 0, "w_gate has no rows")
+    if F <= 0:
+        _refuse("w_gate has no rows")
     ldu = _matrix("w_up", w_up, D, F, x.dtype)
-    _need(ldw == ldu, f"w_gate and w_up have one row stride (got {ldw} and {ldu})")
+    if ldw != ldu:
+        _refuse(f"w_gate and w_up have one row stride (got {ldw} and {ldu})")
     return dev, ldx, ldw, M, D, F
 
 
@@ -157,10 +188,9 @@ def gated_ffn(x, w_gate, w_up, act="silu", save=False):
     h = torch.empty(M, F, dtype=x.dtype, device=dev)
     saved = torch.empty(2, M, F, dtype=torch.float32, device=dev) if save else None
     L = _lib.lib()
-    with torch.cuda.device(dev):
-        scratch = _scratch(L.gs_gated_fwd_scratch_bytes(M, D, F, TYPES[x.dtype]), dev)
-        check(L.gs_gated_fwd(ptr(x), ldx, ptr(w_gate), ptr(w_up), ldw, TYPES[x.dtype], M, D, F, ACTIVATIONS[act], ptr(h), F, ptr(saved),
-                             ptr(scratch), _stream(dev)))
+    scratch = _scratch(L.gs_gated_fwd_scratch_bytes(M, D, F, TYPES[x.dtype]), dev)
+    _launch(dev, L.gs_gated_fwd, x.data_ptr(), ldx, w_gate.data_ptr(), w_up.data_ptr(), ldw, TYPES[x.dtype], M, D, F, ACTIVATIONS[act],
+            h.data_ptr(), F, _ptr(saved), _ptr(scratch))
     return (h, saved) if save else h
 
 
@@ -169,15 +199,14 @@ def gated_ffn_grad(d_h, x, w_gate, w_up, saved, act="silu"):
     dev, ldx, ldw, M, D, F = _gated_args(x, w_gate, w_up, act)
     _device(x=x, d_h=d_h, saved=saved)
     lddh = _matrix("d_h", d_h, F, M, x.dtype)
-    _need(saved.dtype == torch.float32 and tuple(saved.shape) == (2, M, F) and saved.is_contiguous(),
-          f"saved is what gated_ffn(save=True) gave: [2, {M}, {F}] in fp32 (got {saved.dtype}, {tuple(saved.shape)}, strides {saved.stride()})")
+    if not (saved.dtype == torch.float32 and tuple(saved.shape) == (2, M, F) and saved.is_contiguous()):
+        _refuse(f"saved is what gated_ffn(save=True) gave: [2, {M}, {F}] in fp32 (got {saved.dtype}, {tuple(saved.shape)}, strides {saved.stride()})")
     d_x = torch.empty(M, D, dtype=x.dtype, device=dev)
     d_wg, d_wu = (torch.empty(F, D, dtype=x.dtype, device=dev) for _ in range(2))
     L = _lib.lib()
-    with torch.cuda.device(dev):
-        scratch = _scratch(L.gs_gated_bwd_scratch_bytes(M, D, F, TYPES[x.dtype]), dev)
-        check(L.gs_gated_bwd(ptr(d_h), lddh, ptr(x), ldx, ptr(w_gate), ptr(w_up), ldw, ptr(saved), TYPES[x.dtype], M, D, F,
-                             ACTIVATIONS[act], ptr(d_x), D, ptr(d_wg), ptr(d_wu), D, ptr(scratch), _stream(dev)))
+    scratch = _scratch(L.gs_gated_bwd_scratch_bytes(M, D, F, TYPES[x.dtype]), dev)
+    _launch(dev, L.gs_gated_bwd, d_h.data_ptr(), lddh, x.data_ptr(), ldx, w_gate.data_ptr(), w_up.data_ptr(), ldw, saved.data_ptr(),
+            TYPES[x.dtype], M, D, F, ACTIVATIONS[act], d_x.data_ptr(), D, d_wg.data_ptr(), d_wu.data_ptr(), D, _ptr(scratch))
     return d_x, d_wg, d_wu
 
 
@@ -190,16 +219,20 @@ def _distill_args(logits, top_values, top_ids, tau):
     dev = _device(logits=logits, top_values=top_values, top_ids=top_ids)
     ldz = _matrix("logits", logits)
     n, V = logits.shape
-    _need(top_values.dim() == 2 and top_values.shape[0] == n and top_values.is_contiguous(),
-          f"top_values are dense, one row a row of logits (got {tuple(top_values.shape)}, strides {top_values.stride()})")
-    _need(top_values.dtype == logits.dtype, f"top_values are {top_values.dtype}, logits {logits.dtype}")
+    if not (top_values.dim() == 2 and top_values.shape[0] == n and top_values.is_contiguous()):
+        _refuse(f"top_values are dense, one row a row of logits (got {tuple(top_values.shape)}, strides {top_values.stride()})")
+    if top_values.dtype != logits.dtype:
+        _refuse(f"top_values are {top_values.dtype}, logits {logits.dtype}")
     k = top_values.shape[1]
-    _need(1 <= k <= MAX_TOP, f"1 to {MAX_TOP} teacher entries a row (got {k})")
-    _need(tuple(top_ids.shape) == (n, k), f"top_ids are {tuple(top_ids.shape)}, top_values {(n, k)}")
+    if not (1 <= k <= MAX_TOP):
+        _refuse(f"1 to {MAX_TOP} teacher entries a row (got {k})")
+    if tuple(top_ids.shape) != (n, k):
+        _refuse(f"top_ids are {tuple(top_ids.shape)}, top_values {(n, k)}")
     _ids(top_ids)
     tau = float(tau)
-    _need(0 < tau < math.inf, f"a temperature of {tau}")
-    return dev, (ptr(logits), ldz, TYPES[logits.dtype], n, V, ptr(top_values), ptr(top_ids), k, tau), n
+    if not (0 < tau < math.inf):
+        _refuse(f"a temperature of {tau}")
+    return dev, (logits.data_ptr(), ldz, TYPES[logits.dtype], n, V, top_values.data_ptr(), top_ids.data_ptr(), k, tau), n
 
 
 def _grad_out(logits, out):
@@ -215,8 +248,7 @@ def distill(logits, top_values, top_ids, tau=1.0):
     An entry whose class (top_ids) is none of the logits', or whose value is -inf, is not there; a row without any has loss 0."""
     dev, args, n = _distill_args(logits, top_values, top_ids, tau)
     loss, lse = (torch.empty(n, dtype=torch.float32, device=dev) for _ in range(2))
-    with torch.cuda.device(dev):
-        check(_lib.lib().gs_distill_fwd(*args, ptr(loss), ptr(lse), _stream(dev)))
+    _launch(dev, _lib.lib().gs_distill_fwd, *args, loss.data_ptr(), lse.data_ptr())
     return loss, lse
 
 
@@ -228,8 +260,7 @@ def distill_grad(logits, top_values, top_ids, lse, d_loss, tau=1.0, out=None):
     _vector("lse", lse, n, torch.float32)
     _vector("d_loss", d_loss, n, torch.float32)
     out, ldd = _grad_out(logits, out)
-    with torch.cuda.device(dev):
-        check(_lib.lib().gs_distill_bwd(*args, ptr(lse), ptr(d_loss), ptr(out), ldd, _stream(dev)))
+    _launch(dev, _lib.lib().gs_distill_bwd, *args, lse.data_ptr(), d_loss.data_ptr(), out.data_ptr(), ldd)
     return out
 
 
@@ -241,6 +272,5 @@ def distill_loss_grad(logits, top_values, top_ids, d_loss, tau=1.0, out=None):
     _vector("d_loss", d_loss, n, torch.float32)
     out, ldd = _grad_out(logits, out)
     loss = torch.empty(n, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        check(_lib.lib().gs_distill_loss_grad(*args, ptr(d_loss), ptr(loss), ptr(out), ldd, _stream(dev)))
+    _launch(dev, _lib.lib().gs_distill_loss_grad, *args, d_loss.data_ptr(), loss.data_ptr(), out.data_ptr(), ldd)
     return loss, out
