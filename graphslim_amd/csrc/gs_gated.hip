@@ -1,11 +1,14 @@
 // Gated feed-forward block:  g = x Wg^T, u = x Wu^T, h = act(g) u,  and its backward pass
 //   du = dh act(g), dg = dh u act'(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x.
-// Every product is brought to the form C(m, n) = sum_k A(m, k) B(n, k) with k contiguous in both operands, and runs on the 16-bit
-// matrix pipe with fp32 accumulation.  16-bit operands enter as they are; an fp32 operand is the exact sum of three bf16 parts
+// Every product C(m, n) = sum_k A(m, k) B(n, k) runs on the 16-bit matrix pipe with fp32 accumulation; an operand may have k contiguous
+// in memory (x and the weights in the forward pass) or its other index (the weights in dx, both operands of dW): tiles of the
+// latter are transposed on their way from LDS to the registers.  16-bit operands enter as they are; an fp32 operand is the exact sum of three bf16 parts
 // (x = h + m + l, 8 + 8 + 8 significant bits), and six products of parts make one product: what they leave out is below 2^-23 of it.
 // (Parts have bf16's smallest step, 2^-133: a value is represented to 2^-134 or to 24 bits, whichever is coarser.)
-// Operands whose rows are no multiple of 64 elements, or not 16-byte aligned, that have to be split or transposed, are laid out in
-// the caller's scratch first, rows padded with zeros to a multiple of 64.
+// Operands that have to be split, whose rows are not 16-byte aligned, or whose contracted rows are no multiple of 64 elements are laid
+// out in the caller's scratch first, rows padded with zeros to a multiple of 64.
+#include <type_traits>
+
 #include "gs_types.h"
 
 namespace {
@@ -76,99 +79,201 @@ struct GfPlane<GS_TYPE_F32, 3> {
 };
 
 template <int T, int PL, typename P>
-__device__ __forceinline__ void gf_put(float v, P* __restrict__ o, long plane) {
+__device__ __forceinline__ void gf_put8(const float* v, P* __restrict__ o, long plane) {
+  typedef P V __attribute__((ext_vector_type(8)));
   if constexpr (PL == 1) {
-    o[0] = (P)v;
+    V r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (P)v[j];
+    *(V*)o = r;
   } else {
-    __bf16 h, m, l;
-    gf_split(v, h, m, l);
-    o[0] = h;
-    o[plane] = m;
-    o[2 * plane] = l;
+    V h, m, l;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      __bf16 a, b, c;
+      gf_split(v[j], a, b, c);
+      h[j] = a;
+      m[j] = b;
+      l[j] = c;
+    }
+    *(V*)o = h;
+    *(V*)(o + plane) = m;
+    *(V*)(o + 2 * plane) = l;
   }
 }
 
 // ---- operand layout -------------------------------------------------------------------------------------------------------------
-// out [PL][R][ldo] = in [R][C], zeros behind column C up to `cols`
+// Up to three matrices [R][C] as [PL][Rp][Cp], zeros behind the columns and rows
+struct GatedPack {
+  const void* in[3];
+  void* out[3];
+  long ld[3], R[3], Rp[3], first[3];   // first: the matrix's first block
+  long C, Cp, n;
+};
+
 template <int T, int PL>
-__global__ __launch_bounds__(256) void gs_gated_pack_kernel(const typename GsElt<T>::type* __restrict__ in, long ldi, long R, long C,
-                                                            typename GfPlane<T, PL>::type* __restrict__ out, long ldo, long cols, long plane) {
-  const long per = cols / 8;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void gs_gated_pack_kernel(GatedPack a) {
+  typedef typename GsElt<T>::type E;
+  typedef typename GfPlane<T, PL>::type P;
+  const int w = a.n > 2 && (long)blockIdx.x >= a.first[2] ? 2 : (a.n > 1 && (long)blockIdx.x >= a.first[1] ? 1 : 0);
+  const long per = a.Cp / 8;
+  const long i = ((long)blockIdx.x - a.first[w]) * 256 + threadIdx.x;
   const long r = i / per, c = (i - r * per) * 8;
-  if (r >= R) return;
+  if (r >= a.Rp[w]) return;
   float v[8];
-  if (c < C) {
-    gs_load<typename GsElt<T>::type, 8>(in + r * ldi + c, C - c, 0.f, v);
+  if (c < a.C && r < a.R[w]) {
+    gs_load<E, 8>((const E*)a.in[w] + r * a.ld[w] + c, a.C - c, 0.f, v);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = 0.f;
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) gf_put<T, PL>(v[j], out + r * ldo + c + j, plane);
+  gf_put8<T, PL>(v, (P*)a.out[w] + r * a.Cp + c, a.Rp[w] * a.Cp);
 }
 
-// out [PL][C][ldo] = in [R][C] transposed, zeros behind column R up to the next multiple of 64
-template <int T, int PL>
-__global__ __launch_bounds__(256) void gs_gated_pack_t_kernel(const typename GsElt<T>::type* __restrict__ in, long ldi, long R, long C,
-                                                              typename GfPlane<T, PL>::type* __restrict__ out, long ldo, long plane) {
-  __shared__ float tile[64][65];
-  const long r0 = (long)blockIdx.x * 64, c0 = (long)blockIdx.y * 64;
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  for (int i = y; i < 64; i += 4) tile[i][x] = r0 + i < R && c0 + x < C ? (float)in[(r0 + i) * ldi + c0 + x] : 0.f;
-  __syncthreads();
-  for (int i = y; i < 64; i += 4)
-    if (c0 + i < C) gf_put<T, PL>(tile[x][i], out + (c0 + i) * ldo + r0 + x, plane);
-}
-
-// dg, du from dh and the saved g, u: row-major [PL][M][2 Fp] (columns [0, Fp) dg, [Fp, 2 Fp) du) and transposed [PL][2 F][Mp]
+// dg, du from dh and the saved g, u: [PL][Mp][2 Fp], columns [0, Fp) dg, [Fp, 2 Fp) du, zeros in the padding of both
 template <int T, int PL, int ACT>
 __global__ __launch_bounds__(256) void gs_gated_slopes_kernel(const typename GsElt<T>::type* __restrict__ dh, long lddh,
                                                               const float* __restrict__ saved, long M, long F,
-                                                              typename GfPlane<T, PL>::type* __restrict__ rows, long Fp, long plane_r,
-                                                              typename GfPlane<T, PL>::type* __restrict__ cols, long Mp, long plane_c) {
-  __shared__ float tg[64][65], tu[64][65];
-  const long m0 = (long)blockIdx.x * 64, f0 = (long)blockIdx.y * 64;
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  for (int i = y; i < 64; i += 4) {
-    float dg = 0.f, du = 0.f;
-    const long m = m0 + i, f = f0 + x;
-    if (m < M && f < F) {
-      const float d = (float)dh[m * lddh + f], g = saved[m * F + f], u = saved[(M + m) * F + f];
+                                                              typename GfPlane<T, PL>::type* __restrict__ out, long Mp, long Fp, long plane) {
+  typedef typename GfPlane<T, PL>::type P;
+  const long per = Fp / 8;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const long m = i / per, f = (i - m * per) * 8;
+  if (m >= Mp) return;
+  float dg[8], du[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) dg[j] = du[j] = 0.f;
+  if (m < M && f < F) {
+    float d[8], g[8], u[8];
+    gs_load<typename GsElt<T>::type, 8>(dh + m * lddh + f, F - f, 0.f, d);
+    gs_load<float, 8>(saved + m * F + f, F - f, 0.f, g);
+    gs_load<float, 8>(saved + (M + m) * F + f, F - f, 0.f, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
       float a, da;
-      gf_act<ACT>(g, a, da);
-      du = d * a;
-      dg = d * u * da;
-    }
-    tg[i][x] = dg;
-    tu[i][x] = du;
-    if (m < M) {
-      gf_put<T, PL>(dg, rows + m * 2 * Fp + f, plane_r);
-      gf_put<T, PL>(du, rows + m * 2 * Fp + Fp + f, plane_r);
+      gf_act<ACT>(g[j], a, da);
+      du[j] = d[j] * a;
+      dg[j] = d[j] * u[j] * da;
     }
   }
-  __syncthreads();
-  for (int i = y; i < 64; i += 4)
-    if (f0 + i < F) {
-      gf_put<T, PL>(tg[x][i], cols + (f0 + i) * Mp + m0 + x, plane_c);
-      gf_put<T, PL>(tu[x][i], cols + (F + f0 + i) * Mp + m0 + x, plane_c);
+  P* o = out + m * 2 * Fp + f;
+  gf_put8<T, PL>(dg, o, plane);
+  gf_put8<T, PL>(du, o + Fp, plane);
+}
+
+// ---- few rows -------------------------------------------------------------------------------------------------------------------
+// For a few rows (eight at a time) the weights are all there is to read, and the vector units keep up: a wave takes RF rows of both weights,
+// its lanes 16 bytes each of a stretch of k, and adds across the lanes at the end.  Exact fp32 products for every type.
+struct GatedRows {
+  const void *x, *wg, *wu;
+  long ldx, ldw, M, D, F, ldh;
+  void* h;
+  float* saved;
+};
+
+template <int T, int MB, int RF, int ACT>
+__global__ __launch_bounds__(256) void gs_gated_rows_kernel(GatedRows q) {
+  typedef typename GsElt<T>::type E;
+  constexpr int N = 16 / sizeof(E);
+  typedef typename GsVec<E, N>::type V;
+  const int lane = threadIdx.x & 63;
+  const long f0 = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RF, m0 = (long)blockIdx.y * MB;
+  if (f0 >= q.F) return;
+  const E* w[2 * RF];
+#pragma unroll
+  for (int r = 0; r < RF; ++r) {
+    const long f = min(f0 + r, q.F - 1);
+    w[r] = (const E*)q.wg + f * q.ldw;
+    w[RF + r] = (const E*)q.wu + f * q.ldw;
+  }
+  const E* x[MB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m) x[m] = (const E*)q.x + min(m0 + m, q.M - 1) * q.ldx;
+  float acc[MB][2 * RF];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int r = 0; r < 2 * RF; ++r) acc[m][r] = 0.f;
+  long k = (long)lane * N;
+#pragma unroll 2
+  for (; k + N <= q.D; k += 64 * N) {
+    V v[2 * RF], y[MB];
+#pragma unroll
+    for (int r = 0; r < 2 * RF; ++r) v[r] = *(const V*)(w[r] + k);
+#pragma unroll
+    for (int m = 0; m < MB; ++m) y[m] = *(const V*)(x[m] + k);
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float xe = (float)y[m][e];
+#pragma unroll
+        for (int r = 0; r < 2 * RF; ++r) acc[m][r] = fmaf((float)v[r][e], xe, acc[m][r]);
+      }
+  }
+  if (k < q.D) {             // one lane has the end of a row whose length is no multiple of N
+    for (long e = k; e < q.D; ++e)
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int r = 0; r < 2 * RF; ++r) acc[m][r] = fmaf((float)w[r][e], (float)x[m][e], acc[m][r]);
+  }
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int r = 0; r < 2 * RF; ++r) acc[m][r] = gs_wave_sum(acc[m][r]);
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int r = 0; r < RF; ++r) {
+      const long f = f0 + r;
+      if (lane == m * RF + r && m0 + m < q.M && f < q.F) {
+        float a, da;
+        gf_act<ACT>(acc[m][r], a, da);
+        ((E*)q.h)[(m0 + m) * q.ldh + f] = (E)(a * acc[m][RF + r]);
+        if (q.saved) {
+          q.saved[(m0 + m) * q.F + f] = acc[m][r];
+          q.saved[(q.M + m0 + m) * q.F + f] = acc[m][RF + r];
+        }
+      }
     }
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------------------
 struct GatedGemm {
-  const void* A;        // [PL][M][lda]
+  const void* A;        // [PL] planes; k contiguous: rows of m, else rows of k
   long lda, plane_a;
-  const void* B[2];     // [PL][N][ldb]; the gated form: gate and up projection, N rows each
+  const void* B[2];     // gated: gate and up projection; n contiguous: rows of k below `kb` in the first, the others in the second
   long ldb, plane_b;
   long M, N, K;         // K a multiple of 64
-  void* C[2];           // plain form: rows below `rows0` go to C[0], the others to C[1] (from its row 0 on)
-  long ldc, rows0;
+  long bcols;           // n contiguous: columns that rows of B have (a multiple of 8, N or more)
+  long kb, brows;       // n contiguous: rows that B[0] stands for (a multiple of 64), and rows that each of B has; behind them A is 0
+  void* C[2];           // plain form: rows [0, rows) go to C[0], rows [rows1, rows1 + rows) to C[1], others nowhere
+  long ldc, rows, rows1;
   float* saved;         // gated form: g [M][N] and u [M][N], or null
+  float* part;          // k cut into slices: slice z writes its sums to part + z * slice ([M][N]; gated: two of them), nothing to C
+  long slice;
+  int gx;               // tiles of m
+  long kslice;          // of k per slice, a multiple of BK
 };
+
+// row m of a plain product, or null if it is kept nowhere
+template <typename E>
+__device__ __forceinline__ E* gf_row(const GatedGemm& q, long m) {
+  if (m < q.rows) return (E*)q.C[0] + m * q.ldc;
+  return m >= q.rows1 && m < q.rows1 + q.rows ? (E*)q.C[1] + (m - q.rows1) * q.ldc : nullptr;
+}
 
 __device__ __forceinline__ f32x4 gf_mfma(h16x8 a, h16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 gf_mfma(b16x8 a, b16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+template <int N, typename Fn>
+__device__ __forceinline__ void gf_static_for(Fn f) {
+  if constexpr (N > 0) {
+    gf_static_for<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
 
 template <typename P>
 struct GfFrag;
@@ -181,57 +286,116 @@ struct GfFrag<__bf16> {
   typedef b16x8 type;
 };
 
-// One operand's tile in LDS: rows of BK elements as 16-byte chunks, chunk c of row r at place c ^ s(r), so that the eight lanes that a
-// 16-byte LDS read serves at once (eight rows, one chunk) fall on all banks; the permutation is made on the global side, since the
-// direct-to-LDS load writes 64 consecutive chunks.
-template <int BK>
+// An operand's tile in LDS, in 16-byte chunks; chunk c of row r lies at place c ^ s(r) of its row.  The permutation is made on the
+// global side, since the direct-to-LDS load writes 64 consecutive chunks.
+//   k contiguous: rows of BK elements; the eight lanes that a 16-byte LDS read serves at once (eight rows, one chunk) fall on all banks.
+//   else:         BK rows of W elements; ds_read_b64_tr_b16 reads four rows by 16 elements per 16 lanes and hands lane i the four
+//                 values of element i; rows that one read serves at once (r & 3, and the next group's r >> 3) fall on different banks.
+template <bool TALL, int BK>
 __device__ __forceinline__ int gf_swz(int r) {
+  if (TALL) return ((r & 3) | ((r >> 3) & 1) << 2) << 1;
   return BK == 64 ? (r & 7) : ((r >> 1) & 3);
 }
 
-// T: type of the outputs (and of 16-bit operands), PL: parts, WM x WN waves of (16 FM) x (16 FN) results, GATED: rows of B alternate
-// between gate and up every 16, so that a lane holds both sums of its outputs and the activation is applied in registers.
-template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool GATED, int ACT>
+template <typename Frag, int BK, typename P>
+__device__ __forceinline__ Frag gf_frag(const P* tile, int row0, int ks, int lane) {
+  const int r = row0 + (lane & 15), c = ks * 4 + (lane >> 4);
+  return *(const Frag*)(tile + (r * (BK / 8) + (c ^ gf_swz<false, BK>(r))) * 8);
+}
+
+// LDS byte address of a lane's first four values of fragment 0 of a tile whose rows are k; fragment i lies at that ^ (i << 5) (the
+// permutation flips the same bits), four rows of k further at + 8 W, 32 at + 64 W.
+template <int W, int BK, typename P>
+__device__ __forceinline__ unsigned gf_tr_addr(const P* tile, int row0, int lane) {
+  const int k = (lane >> 4) * 8 + ((lane >> 2) & 3), c = row0 / 8 + ((lane & 3) >> 1);
+  return (unsigned)(size_t)(lds_ptr)(tile + (k * (W / 8) + (c ^ gf_swz<true, BK>(k))) * 8 + (lane & 1) * 4);
+}
+
+// N (2 or 4) fragments from `first` on.  In assembly, with its own wait: the compiler lets no transposing read of its own pass a
+// direct-to-LDS load that is under way, though the two are on different buffers here.
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+template <int OFF, int W, typename Frag>
+__device__ __forceinline__ void gf_tr_read4(unsigned addr, int first, Frag* x) {
+  const unsigned a0 = addr ^ (first << 5), a1 = addr ^ ((first + 1) << 5), a2 = addr ^ ((first + 2) << 5), a3 = addr ^ ((first + 3) << 5);
+  i32x2 l0, h0, l1, h1, l2, h2, l3, h3;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(l0), "=&v"(h0), "=&v"(l1), "=&v"(h1), "=&v"(l2), "=&v"(h2), "=&v"(l3), "=&v"(h3)
+      : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(OFF), "n"(OFF + 8 * W)
+      : "memory");
+  x[0] = __builtin_bit_cast(Frag, __builtin_shufflevector(l0, h0, 0, 1, 2, 3));
+  x[1] = __builtin_bit_cast(Frag, __builtin_shufflevector(l1, h1, 0, 1, 2, 3));
+  x[2] = __builtin_bit_cast(Frag, __builtin_shufflevector(l2, h2, 0, 1, 2, 3));
+  x[3] = __builtin_bit_cast(Frag, __builtin_shufflevector(l3, h3, 0, 1, 2, 3));
+}
+
+// T: type of the outputs (and of 16-bit operands), PL: parts, WM x WN waves of (16 FM) x (16 FN) results.  TA, TB: the operand's other
+// index is contiguous, not k.  GATED: rows of B alternate between gate and up every 16, so that a lane holds both sums of its outputs
+// and the activation is applied in registers.
+template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool GATED, int ACT>
 __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q) {
   typedef typename GfPlane<T, PL>::type P;
   typedef typename GfFrag<P>::type Frag;
   typedef typename GsElt<T>::type E;
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16, NT = WM * WN * 64;
-  constexpr int CH = BK / 8;                                  // 16-byte chunks of a row
+  constexpr int CA = (TA ? BM : BK) / 8, CB = (TB ? BN : BK) / 8;   // 16-byte chunks of a row
   constexpr int TILE_A = BM * BK, TILE_B = BN * BK, STAGE = PL * (TILE_A + TILE_B);
-  constexpr int ITA = BM * CH / NT, ITB = BN * CH / NT;
-  static_assert(BM * CH % NT == 0 && BN * CH % NT == 0, "whole waves load a tile");
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int ITA = TILE_A / 8 / NT, ITB = TILE_B / 8 / NT;
+  static_assert(TILE_A / 8 % NT == 0 && TILE_B / 8 % NT == 0, "whole waves load a tile");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
   P* lds = (P*)smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave / WN, wn = wave % WN;
-  const long m0 = (long)blockIdx.x * BM;
-  const long n0 = (long)blockIdx.y * (GATED ? BN / 2 : BN);
+  // Tiles of m first: what runs at a time on an XCD (every eighth workgroup) shares four rows of tiles and their columns in its L2.
+  // (8192 x 2048 x 8192: giving each XCD a run of consecutive tiles instead changes nothing without `saved`, and with it costs 100 us
+  // of 560, since neighbouring pieces of its rows are then written far apart in time.)
+  const long m0 = (long)(blockIdx.x % q.gx) * BM;
+  const long n0 = (long)(blockIdx.x / q.gx) * (GATED ? BN / 2 : BN);
+  const long k_begin = blockIdx.y * q.kslice, k_end = min(k_begin + q.kslice, q.K);
   const P* A = (const P*)q.A;
 
   const P* srcA[ITA];
-  const P* srcB[ITB];
+  long srcB[ITB], endB[ITB];   // offsets from B's base; from that of the step with B's last rows, where they are fewer than BK
 #pragma unroll
   for (int i = 0; i < ITA; ++i) {
-    const int s = i * NT + tid, r = s / CH, c = (s % CH) ^ gf_swz<BK>(r);
-    srcA[i] = A + min(m0 + r, q.M - 1) * q.lda + c * 8;
+    const int s = i * NT + tid, r = s / CA, c = (s % CA) ^ gf_swz<TA, BK>(r);
+    srcA[i] = TA ? A + r * q.lda + min(m0 + c * 8, q.M - 8) : A + min(m0 + r, q.M - 1) * q.lda + c * 8;
   }
 #pragma unroll
   for (int i = 0; i < ITB; ++i) {
-    const int s = i * NT + tid, r = s / CH, c = (s % CH) ^ gf_swz<BK>(r);
+    const int s = i * NT + tid, r = s / CB, c = (s % CB) ^ gf_swz<TB, BK>(r);
     const long n = GATED ? n0 + (r >> 5) * 16 + (r & 15) : n0 + r;
-    srcB[i] = (const P*)q.B[GATED ? (r >> 4) & 1 : 0] + min(n, q.N - 1) * q.ldb + c * 8;
+    const P* base = (const P*)q.B[GATED ? (r >> 4) & 1 : 0];
+    const long col = min(n0 + c * 8, q.bcols - 8);
+    srcB[i] = TB ? r * q.ldb + col : (long)(base + min(n, q.N - 1) * q.ldb + c * 8 - (const P*)q.B[0]);
+    endB[i] = TB ? min((long)r, (q.brows - 1) % BK) * q.ldb + col : 0;
   }
   auto stage = [&](int buf, long k0) {
     P* base = lds + buf * STAGE;
+    const P* b0 = (const P*)q.B[0] + k0;
+    bool end = false;
+    if constexpr (TB) {
+      // A is zero behind B's rows: a step that lies there altogether takes B's last ones
+      const long kk = min(k0 < q.kb ? k0 : k0 - q.kb, (q.brows - 1) / BK * BK);
+      b0 = (const P*)q.B[k0 < q.kb ? 0 : 1] + kk * q.ldb;
+      end = kk + BK > q.brows;
+    }
 #pragma unroll
     for (int p = 0; p < PL; ++p) {
 #pragma unroll
       for (int i = 0; i < ITA; ++i)
-        __builtin_amdgcn_global_load_lds((gbl_ptr)(srcA[i] + p * q.plane_a + k0), (lds_ptr)(base + p * TILE_A + (i * NT + wave * 64) * 8), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gbl_ptr)(srcA[i] + p * q.plane_a + (TA ? k0 * q.lda : k0)),
+                                         (lds_ptr)(base + p * TILE_A + (i * NT + wave * 64) * 8), 16, 0, 0);
 #pragma unroll
-      for (int i = 0; i < ITB; ++i)
-        __builtin_amdgcn_global_load_lds((gbl_ptr)(srcB[i] + p * q.plane_b + k0), (lds_ptr)(base + PL * TILE_A + p * TILE_B + (i * NT + wave * 64) * 8), 16, 0, 0);
+      for (int i = 0; i < ITB; ++i) {
+        const long off = TB && end ? endB[i] : srcB[i];
+        __builtin_amdgcn_global_load_lds((gbl_ptr)(b0 + p * q.plane_b + off), (lds_ptr)(base + PL * TILE_A + p * TILE_B + (i * NT + wave * 64) * 8), 16, 0, 0);
+      }
     }
   };
 
@@ -241,46 +405,60 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-  const int lr = lane & 15, lc = lane >> 4;
-  stage(0, 0);
+  const unsigned tra = TA ? gf_tr_addr<BM, BK>(lds, wm * FM * 16, lane) : 0u;
+  const unsigned trb = TB ? gf_tr_addr<BN, BK>(lds + PL * TILE_A, wn * FN * 16, lane) : 0u;
+  stage(0, k_begin);
   int buf = 0;
-  for (long k0 = 0; k0 < q.K; k0 += BK, buf ^= 1) {
+  for (long k0 = k_begin; k0 < k_end; k0 += BK, buf ^= 1) {
     __syncthreads();   // this step's tile has landed; the other buffer has been read by all
-    if (k0 + BK < q.K) stage(buf ^ 1, k0 + BK);
-    const P* base = lds + buf * STAGE;
-#pragma unroll
-    for (int ks = 0; ks < BK / 32; ++ks) {
+    const P* ta = lds + buf * STAGE;
+    const P* tb = ta + PL * TILE_A;
+    if (k0 + BK < k_end) stage(buf ^ 1, k0 + BK);
+    gf_static_for<BK / 32>([&](auto ks_) {
+      constexpr int ks = decltype(ks_)::value;
       Frag a[PL][FM], b[PL][FN];
+      gf_static_for<PL>([&](auto p_) {
+        constexpr int p = decltype(p_)::value;
+        if constexpr (TB) {
+          gf_static_for<FN / 4>([&](auto j_) {
+            constexpr int j = decltype(j_)::value * 4;
+            gf_tr_read4<p * TILE_B * 2 + ks * 64 * BN, BN>(trb + buf * STAGE * 2, j, &b[p][j]);
+          });
+        } else {
 #pragma unroll
-      for (int p = 0; p < PL; ++p) {
-#pragma unroll
-        for (int i = 0; i < FM; ++i) {
-          const int r = (wm * FM + i) * 16 + lr;
-          a[p][i] = *(const Frag*)(base + p * TILE_A + (r * CH + ((ks * 4 + lc) ^ gf_swz<BK>(r))) * 8);
+          for (int j = 0; j < FN; ++j) b[p][j] = gf_frag<Frag, BK>(tb + p * TILE_B, (wn * FN + j) * 16, ks, lane);
         }
+        if constexpr (!TA) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          const int r = (wn * FN + j) * 16 + lr;
-          b[p][j] = *(const Frag*)(base + PL * TILE_A + p * TILE_B + (r * CH + ((ks * 4 + lc) ^ gf_swz<BK>(r))) * 8);
+          for (int i = 0; i < FM; ++i) a[p][i] = gf_frag<Frag, BK>(ta + p * TILE_A, (wm * FM + i) * 16, ks, lane);
         }
-      }
+      });
+      gf_static_for<FM / 4>([&](auto i_) {
+        constexpr int i0 = decltype(i_)::value * 4;
+        if constexpr (TA)
+          gf_static_for<PL>([&](auto p_) {
+            constexpr int p = decltype(p_)::value;
+            gf_tr_read4<p * TILE_A * 2 + ks * 64 * BM, BM>(tra + buf * STAGE * 2, i0, &a[p][i0]);
+          });
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+        for (int i = i0; i < i0 + 4; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          if constexpr (PL == 3) {   // small terms first
-            acc[i][j] = gf_mfma(b[2][j], a[0][i], acc[i][j]);
-            acc[i][j] = gf_mfma(b[0][j], a[2][i], acc[i][j]);
-            acc[i][j] = gf_mfma(b[1][j], a[1][i], acc[i][j]);
-            acc[i][j] = gf_mfma(b[1][j], a[0][i], acc[i][j]);
-            acc[i][j] = gf_mfma(b[0][j], a[1][i], acc[i][j]);
+          for (int j = 0; j < FN; ++j) {
+            if constexpr (PL == 3) {   // small terms first
+              acc[i][j] = gf_mfma(b[2][j], a[0][i], acc[i][j]);
+              acc[i][j] = gf_mfma(b[0][j], a[2][i], acc[i][j]);
+              acc[i][j] = gf_mfma(b[1][j], a[1][i], acc[i][j]);
+              acc[i][j] = gf_mfma(b[1][j], a[0][i], acc[i][j]);
+              acc[i][j] = gf_mfma(b[0][j], a[1][i], acc[i][j]);
+            }
+            acc[i][j] = gf_mfma(b[0][j], a[0][i], acc[i][j]);
           }
-          acc[i][j] = gf_mfma(b[0][j], a[0][i], acc[i][j]);
-        }
-    }
+      });
+    });
   }
 
   // B is the first operand, so a lane holds four consecutive n of one m
+  const int lr = lane & 15, lc = lane >> 4;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const long m = m0 + (wm * FM + i) * 16 + lr;
@@ -295,6 +473,15 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
         for (int e = 0; e < 4; ++e) {
           g[e] = acc[i][j][e];
           u[e] = acc[i][j + 1][e];
+        }
+        if (q.part) {
+          float* o = q.part + blockIdx.y * q.slice + m * q.N + n;
+          gs_store<float, 4>(o, q.N - n, g);
+          gs_store<float, 4>(o + q.M * q.N, q.N - n, u);
+          continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
           gf_act<ACT>(g[e], h[e], da);
           h[e] *= u[e];
         }
@@ -305,7 +492,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
         }
       }
     } else {
-      E* row = m < q.rows0 ? (E*)q.C[0] + m * q.ldc : (E*)q.C[1] + (m - q.rows0) * q.ldc;
+      E* row = gf_row<E>(q, m);
+      if (!row) continue;
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         const long n = n0 + (wn * FN + j) * 16 + lc * 4;
@@ -313,19 +501,91 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
-        gs_store<E, 4>(row + n, q.N - n, v);
+        if (q.part) gs_store<float, 4>(q.part + blockIdx.y * q.slice + m * q.N + n, q.N - n, v);
+        else gs_store<E, 4>(row + n, q.N - n, v);
       }
     }
   }
 }
 
+// Sums the slices of k in their order and finishes what the product's epilogue does.  A thread takes four columns of a row.
+template <int T, bool GATED, int ACT>
+__global__ __launch_bounds__(256) void gs_gated_join_kernel(GatedGemm q, int slices) {
+  typedef typename GsElt<T>::type E;
+  const long per = (q.N + 3) / 4, i = (long)blockIdx.x * 256 + threadIdx.x;
+  const long m = i / per, n = (i - m * per) * 4;
+  if (m >= q.M) return;
+  E* row = GATED ? (E*)q.C[0] + m * q.ldc : gf_row<E>(q, m);
+  if (!row) return;
+  float g[4] = {}, u[4] = {};
+  const float* at = q.part + m * q.N + n;
+  for (int z = 0; z < slices; ++z) {
+    float v[4];
+    gs_load<float, 4>(at + z * q.slice, q.N - n, 0.f, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) g[e] += v[e];
+    if constexpr (GATED) {
+      gs_load<float, 4>(at + z * q.slice + q.M * q.N, q.N - n, 0.f, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] += v[e];
+    }
+  }
+  if constexpr (GATED) {
+    if (q.saved) {
+      gs_store<float, 4>(q.saved + m * q.N + n, q.N - n, g);
+      gs_store<float, 4>(q.saved + (q.M + m) * q.N + n, q.N - n, u);
+    }
+    float da;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      gf_act<ACT>(g[e], g[e], da);
+      g[e] *= u[e];
+    }
+  }
+  gs_store<E, 4>(row + n, q.N - n, g);
+}
+
 // ---- host -----------------------------------------------------------------------------------------------------------------------
+// What a product costs, in units of one workgroup's 64 of k in the small tile, and the scratch that its slices take.
+struct GatedSplit {
+  bool big;
+  int slices;
+  long kslice;        // in elements
+  size_t part;        // floats
+};
+
+// Two tiles, 128 x 128 (two workgroups on a compute unit) and 256 x 256 (one): per 64 of k the large one takes 1.75 times as long for
+// four times the products of one of the two small ones side by side.  A product that does not fill the 256 compute units is cut along k; its slices
+// are summed by a second launch, which costs about 4 steps and the traffic of the partial sums.
+GatedSplit gf_split_of(long M, long N, long K, bool gated, int pl) {
+  GatedSplit best = {};
+  double least = 1e300;
+  const long cols = gated ? 2 * N : N;
+  for (int big = 0; big < 2; ++big) {
+    const long bm = big ? 256 : 128, bn = big && pl == 1 ? 256 : 128, bk = pl == 3 ? 32 : 64;
+    const long tiles = ((M + bm - 1) / bm) * ((cols + bn - 1) / bn), slots = big || pl == 3 ? 256 : 512, steps = K / bk;
+    const double step = big ? 1.75 : 1.0;
+    for (long want = 1; want <= 64 && want <= steps; ++want) {
+      const long per = (steps + want - 1) / want, slices = (steps + per - 1) / per;
+      if (want > 1 && tiles * slices > 2 * slots) break;
+      double cost = (double)((tiles * slices + slots - 1) / slots) * step * (per + 2);
+      if (slices > 1) cost += 4 + (double)slices * M * cols * 8 / 4e6;
+      if (cost < least) {
+        least = cost;
+        best = {big != 0, (int)slices, per * bk, slices > 1 ? (size_t)slices * M * cols : 0};
+      }
+    }
+  }
+  return best;
+}
+
 // Where the laid-out operands lie in the scratch (elements of 2 bytes).  The sizes go by the shapes and the type alone.
 struct GatedPlan {
   int pl;
   long Dp, Fp, Mp;
-  size_t x, wg, wu, fwd;                       // forward: x, Wg, Wu with padded rows
-  size_t rows, cols, wt, xt, bwd;              // backward: [dg | du], its transpose, [Wg; Wu]^T, x^T
+  size_t x, wg, wu, fwd;              // x, Wg, Wu with padded rows (both passes)
+  size_t dgu, bwd;                    // backward: [dg | du]
+  size_t part_fwd, part_bwd;          // partial sums of products that are cut along k, behind the operands
 };
 
 GatedPlan gf_plan(long M, long D, long F, int type) {
@@ -336,56 +596,55 @@ GatedPlan gf_plan(long M, long D, long F, int type) {
   p.Mp = gf_up(M);
   size_t o = 0;
   auto take = [&](size_t n) { size_t at = o; o += n * p.pl; return at; };
-  p.x = take((size_t)M * p.Dp);
-  p.wg = take((size_t)F * p.Dp);
-  p.wu = take((size_t)F * p.Dp);
-  p.fwd = o;
-  o = 0;
-  p.rows = take((size_t)M * 2 * p.Fp);
-  p.cols = take((size_t)2 * F * p.Mp);
-  p.wt = take((size_t)D * 2 * p.Fp);
-  p.xt = take((size_t)D * p.Mp);
-  p.bwd = o;
+  p.x = take((size_t)p.Mp * p.Dp);
+  p.wg = take((size_t)p.Fp * p.Dp);
+  p.wu = take((size_t)p.Fp * p.Dp);
+  p.part_fwd = o;
+  p.fwd = o + 2 * gf_split_of(M, F, p.Dp, true, p.pl).part;
+  p.dgu = take((size_t)p.Mp * 2 * p.Fp);
+  p.part_bwd = o;
+  const size_t dx = gf_split_of(M, D, 2 * p.Fp, false, p.pl).part, dw = gf_split_of(2 * p.Fp, D, p.Mp, false, p.pl).part;
+  p.bwd = o + 2 * (dx > dw ? dx : dw);
   return p;
 }
 
-template <int T, int PL, bool GATED, int ACT>
-int gf_gemm(const GatedGemm& q, hipStream_t s) {
-  constexpr int BK = PL == 3 ? 32 : 64;
-  constexpr int LDS = 2 * PL * (128 + 128) * BK * 2;
-  auto kern = gs_gated_gemm_kernel<T, PL, 2, 2, 4, 4, BK, GATED, ACT>;
-  GS_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-  const long gx = (q.M + 127) / 128, gy = (q.N + (GATED ? 63 : 127)) / (GATED ? 64 : 128);
-  if (gx > 0x7fffffffL || gy > 65535) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", q.M, q.N);
-  kern<<<dim3((unsigned)gx, (unsigned)gy), dim3(256), LDS, s>>>(q);
+template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool GATED, int ACT>
+int gf_tile(GatedGemm q, const GatedSplit& sp, float* part, hipStream_t s) {
+  constexpr int BM = WM * FM * 16, BN = WN * FN * 16 / (GATED ? 2 : 1), LDS = 2 * PL * (WM * FM + WN * FN) * 16 * BK * 2;
+  auto kern = gs_gated_gemm_kernel<T, PL, WM, WN, FM, FN, BK, TA, TB, GATED, ACT>;
+  if (LDS > 65536) GS_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+  const long gx = (q.M + BM - 1) / BM, gy = (q.N + BN - 1) / BN;
+  if (gx * gy > 0x1fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", q.M, q.N);
+  q.gx = (int)gx;
+  q.kslice = sp.kslice;
+  if (sp.slices > 1) {
+    q.part = part;
+    q.slice = q.M * q.N * (GATED ? 2 : 1);
+  }
+  kern<<<dim3((unsigned)(gx * gy), (unsigned)sp.slices), dim3(WM * WN * 64), LDS, s>>>(q);
   GS_LAUNCH_CHECK();
+  if (sp.slices > 1) {
+    const long blocks = (q.M * ((q.N + 3) / 4) + 255) / 256;
+    gs_gated_join_kernel<T, GATED, ACT><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(q, sp.slices);
+    GS_LAUNCH_CHECK();
+  }
   return GS_OK;
 }
 
-template <int T, int PL>
-int gf_pack(const void* in, long ldi, long R, long C, void* out, long ldo, long plane, hipStream_t s) {
-  typedef typename GsElt<T>::type E;
-  typedef typename GfPlane<T, PL>::type P;
-  const long cols = gf_up(C), blocks = (R * (cols / 8) + 255) / 256;
-  if (blocks > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", R, C);
-  gs_gated_pack_kernel<T, PL><<<dim3((unsigned)blocks), dim3(256), 0, s>>>((const E*)in, ldi, R, C, (P*)out, ldo, cols, plane);
-  GS_LAUNCH_CHECK();
-  return GS_OK;
+template <int T, int PL, bool TA, bool TB, bool GATED, int ACT>
+int gf_gemm(const GatedGemm& q, float* part, hipStream_t s) {
+  const GatedSplit sp = gf_split_of(q.M, q.N, q.K, GATED, PL);
+  if constexpr (PL == 3) {
+    if (sp.big) return gf_tile<T, PL, 4, 2, 4, 4, 32, TA, TB, GATED, ACT>(q, sp, part, s);
+    return gf_tile<T, PL, 2, 2, 4, 4, 32, TA, TB, GATED, ACT>(q, sp, part, s);
+  } else {
+    if (sp.big) return gf_tile<T, PL, 2, 4, 8, 4, 64, TA, TB, GATED, ACT>(q, sp, part, s);
+    return gf_tile<T, PL, 2, 2, 4, 4, 64, TA, TB, GATED, ACT>(q, sp, part, s);
+  }
 }
 
-template <int T, int PL>
-int gf_pack_t(const void* in, long ldi, long R, long C, void* out, long ldo, long plane, hipStream_t s) {
-  typedef typename GsElt<T>::type E;
-  typedef typename GfPlane<T, PL>::type P;
-  const long gx = (R + 63) / 64, gy = (C + 63) / 64;
-  if (gx > 0x7fffffffL || gy > 65535) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", R, C);
-  gs_gated_pack_t_kernel<T, PL><<<dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, s>>>((const E*)in, ldi, R, C, (P*)out, ldo, plane);
-  GS_LAUNCH_CHECK();
-  return GS_OK;
-}
-
-// whether rows of `n` elements with stride ld can be read as they are
-inline bool gf_plain(const void* p, long ld, long n) { return n % GF_PAD == 0 && ld % 8 == 0 && ((size_t)p & 15) == 0; }
+// whether rows of `n` elements with stride ld can be read as they are: in chunks of 16 bytes, whole steps of 64 where k is contiguous
+inline bool gf_plain(const void* p, long ld, long n, int step) { return n % step == 0 && ld % 8 == 0 && ((size_t)p & 15) == 0; }
 
 struct GatedCall {
   const void *x, *wg, *wu, *dh;
@@ -398,29 +657,74 @@ struct GatedCall {
   char* scratch;
 };
 
+// x, Wg and Wu as operands: as they are, or laid out in the scratch
+struct GatedOperands {
+  const void *x, *w[2];
+  long ldx, ldw, plane_x, plane_w;
+};
+
+template <int T, int PL>
+int gf_operands(const GatedCall& c, const GatedPlan& p, int step, GatedOperands* o, hipStream_t s) {
+  typedef typename GfPlane<T, PL>::type P;
+  P* sc = (P*)c.scratch;
+  *o = {c.x, {c.wg, c.wu}, c.ldx, c.ldw, 0, 0};
+  GatedPack a = {};
+  a.C = c.D;
+  a.Cp = p.Dp;
+  long blocks = 0;
+  auto add = [&](const void* in, long ld, long R, long Rp, P* out) {
+    a.in[a.n] = in; a.out[a.n] = out; a.ld[a.n] = ld; a.R[a.n] = R; a.Rp[a.n] = Rp; a.first[a.n] = blocks;
+    ++a.n;
+    blocks += (Rp * (p.Dp / 8) + 255) / 256;
+  };
+  if (PL > 1 || !gf_plain(c.x, c.ldx, c.D, step)) {
+    o->x = sc + p.x; o->ldx = p.Dp; o->plane_x = p.Mp * p.Dp;
+    add(c.x, c.ldx, c.M, p.Mp, sc + p.x);
+  }
+  if (PL > 1 || !gf_plain(c.wg, c.ldw, c.D, step) || !gf_plain(c.wu, c.ldw, c.D, step)) {
+    o->w[0] = sc + p.wg; o->w[1] = sc + p.wu; o->ldw = p.Dp; o->plane_w = p.Fp * p.Dp;
+    add(c.wg, c.ldw, c.F, p.Fp, sc + p.wg);
+    add(c.wu, c.ldw, c.F, p.Fp, sc + p.wu);
+  }
+  if (blocks > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: operands of width %ld are beyond one launch", c.D);
+  if (blocks) {
+    gs_gated_pack_kernel<T, PL><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(a);
+    GS_LAUNCH_CHECK();
+  }
+  return GS_OK;
+}
+
+// Rows up to which the weights are read by gs_gated_rows_kernel.  2048 x 8192: bf16, 4 rows 16 us and 8 rows 25 us against 22 for the
+// matrix pipe; fp32, 24 rows 96 us against 115, of which laying out the split weights is most.
+inline bool gf_few(long M, int type) { return M <= (type == GS_TYPE_F32 ? 24 : 4); }
+
+template <int T, int MB, int ACT>
+int gf_rows(const GatedCall& c, hipStream_t s) {
+  constexpr int RF = 2;
+  GatedRows q = {c.x, c.wg, c.wu, c.ldx, c.ldw, c.M, c.D, c.F, c.ldh, c.h, c.saved};
+  gs_gated_rows_kernel<T, MB, RF, ACT><<<dim3((unsigned)((c.F + 4 * RF - 1) / (4 * RF)), (unsigned)((c.M + MB - 1) / MB)), dim3(256), 0, s>>>(q);
+  GS_LAUNCH_CHECK();
+  return GS_OK;
+}
+
 template <int T, int PL, int ACT>
 int gf_fwd(const GatedCall& c, hipStream_t s) {
   typedef typename GfPlane<T, PL>::type P;
+  if (gf_few(c.M, T)) {
+    if (c.M == 1) return gf_rows<T, 1, ACT>(c, s);
+    if (c.M == 2) return gf_rows<T, 2, ACT>(c, s);
+    return c.M <= 4 ? gf_rows<T, 4, ACT>(c, s) : gf_rows<T, 8, ACT>(c, s);
+  }
   const GatedPlan p = gf_plan(c.M, c.D, c.F, T);
-  P* sc = (P*)c.scratch;
+  GatedOperands o;
+  GS_TRY((gf_operands<T, PL>(c, p, GF_PAD, &o, s)));
   GatedGemm q = {};
+  q.A = o.x; q.lda = o.ldx; q.plane_a = o.plane_x;
+  q.B[0] = o.w[0]; q.B[1] = o.w[1]; q.ldb = o.ldw; q.plane_b = o.plane_w;
   q.M = c.M; q.N = c.F; q.K = p.Dp;
-  q.C[0] = c.h; q.ldc = c.ldh; q.rows0 = c.M;
+  q.C[0] = c.h; q.ldc = c.ldh;
   q.saved = c.saved;
-  if (PL == 1 && gf_plain(c.x, c.ldx, c.D)) {
-    q.A = c.x; q.lda = c.ldx;
-  } else {
-    q.A = sc + p.x; q.lda = p.Dp; q.plane_a = c.M * p.Dp;
-    GS_TRY((gf_pack<T, PL>(c.x, c.ldx, c.M, c.D, sc + p.x, p.Dp, q.plane_a, s)));
-  }
-  if (PL == 1 && gf_plain(c.wg, c.ldw, c.D) && gf_plain(c.wu, c.ldw, c.D)) {
-    q.B[0] = c.wg; q.B[1] = c.wu; q.ldb = c.ldw;
-  } else {
-    q.B[0] = sc + p.wg; q.B[1] = sc + p.wu; q.ldb = p.Dp; q.plane_b = c.F * p.Dp;
-    GS_TRY((gf_pack<T, PL>(c.wg, c.ldw, c.F, c.D, sc + p.wg, p.Dp, q.plane_b, s)));
-    GS_TRY((gf_pack<T, PL>(c.wu, c.ldw, c.F, c.D, sc + p.wu, p.Dp, q.plane_b, s)));
-  }
-  return gf_gemm<T, PL, true, ACT>(q, s);
+  return gf_gemm<T, PL, false, false, true, ACT>(q, (float*)((P*)c.scratch + p.part_fwd), s);
 }
 
 template <int T, int PL, int ACT>
@@ -428,27 +732,28 @@ int gf_bwd(const GatedCall& c, hipStream_t s) {
   typedef typename GsElt<T>::type E;
   typedef typename GfPlane<T, PL>::type P;
   const GatedPlan p = gf_plan(c.M, c.D, c.F, T);
-  P* sc = (P*)c.scratch;
-  const long plane_r = c.M * 2 * p.Fp, plane_c = 2 * c.F * p.Mp, plane_w = c.D * 2 * p.Fp, plane_x = c.D * p.Mp;
-  const long gx = p.Mp / 64, gy = p.Fp / 64;
-  if (gx > 0x7fffffffL || gy > 65535) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated_bwd: %ld x %ld is beyond one launch", c.M, c.F);
-  gs_gated_slopes_kernel<T, PL, ACT><<<dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, s>>>(
-      (const E*)c.dh, c.lddh, c.saved, c.M, c.F, sc + p.rows, p.Fp, plane_r, sc + p.cols, p.Mp, plane_c);
+  P* dgu = (P*)c.scratch + p.dgu;
+  const long plane = p.Mp * 2 * p.Fp, blocks = (p.Mp * (p.Fp / 8) + 255) / 256;
+  if (blocks > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated_bwd: %ld x %ld is beyond one launch", c.M, c.F);
+  GatedOperands o;
+  GS_TRY((gf_operands<T, PL>(c, p, 8, &o, s)));
+  gs_gated_slopes_kernel<T, PL, ACT><<<dim3((unsigned)blocks), dim3(256), 0, s>>>((const E*)c.dh, c.lddh, c.saved, c.M, c.F, dgu, p.Mp, p.Fp, plane);
   GS_LAUNCH_CHECK();
-  GS_TRY((gf_pack_t<T, PL>(c.wg, c.ldw, c.F, c.D, sc + p.wt, 2 * p.Fp, plane_w, s)));
-  GS_TRY((gf_pack_t<T, PL>(c.wu, c.ldw, c.F, c.D, sc + p.wt + p.Fp, 2 * p.Fp, plane_w, s)));
-  GS_TRY((gf_pack_t<T, PL>(c.x, c.ldx, c.M, c.D, sc + p.xt, p.Mp, plane_x, s)));
+  // dx: k runs over the columns of dg, then of du, and over the rows of Wg, then of Wu
   GatedGemm q = {};
-  q.A = sc + p.rows; q.lda = 2 * p.Fp; q.plane_a = plane_r;
-  q.B[0] = sc + p.wt; q.ldb = 2 * p.Fp; q.plane_b = plane_w;
-  q.M = c.M; q.N = c.D; q.K = 2 * p.Fp;
-  q.C[0] = c.dx; q.ldc = c.lddx; q.rows0 = c.M;
-  GS_TRY((gf_gemm<T, PL, false, GS_ACT_SILU>(q, s)));
-  q.A = sc + p.cols; q.lda = p.Mp; q.plane_a = plane_c;
-  q.B[0] = sc + p.xt; q.ldb = p.Mp; q.plane_b = plane_x;
-  q.M = 2 * c.F; q.N = c.D; q.K = p.Mp;
-  q.C[0] = c.dwg; q.C[1] = c.dwu; q.ldc = c.lddw; q.rows0 = c.F;
-  return gf_gemm<T, PL, false, GS_ACT_SILU>(q, s);
+  q.A = dgu; q.lda = 2 * p.Fp; q.plane_a = plane;
+  q.B[0] = o.w[0]; q.B[1] = o.w[1]; q.ldb = o.ldw; q.plane_b = o.plane_w;
+  q.M = c.M; q.K = 2 * p.Fp; q.kb = p.Fp; q.brows = o.plane_w ? p.Fp : c.F;
+  q.N = c.D; q.bcols = o.plane_w ? p.Dp : c.D;
+  q.C[0] = c.dx; q.ldc = c.lddx; q.rows = q.rows1 = c.M;
+  float* part = (float*)((P*)c.scratch + p.part_bwd);
+  GS_TRY((gf_gemm<T, PL, false, true, false, GS_ACT_SILU>(q, part, s)));
+  // dWg, dWu: k runs over the tokens
+  q.B[0] = o.x; q.ldb = o.ldx; q.plane_b = o.plane_x;
+  q.M = 2 * p.Fp; q.K = p.Mp; q.kb = p.Mp; q.brows = o.plane_x ? p.Mp : c.M;
+  q.bcols = o.plane_x ? p.Dp : c.D;
+  q.C[0] = c.dwg; q.C[1] = c.dwu; q.ldc = c.lddw; q.rows = c.F; q.rows1 = p.Fp;
+  return gf_gemm<T, PL, true, true, false, GS_ACT_SILU>(q, part, s);
 }
 
 // dW = 0 where there are no tokens
@@ -498,7 +803,7 @@ int gf_run(const GatedCall& c, int type, bool bwd, hipStream_t s) {
 
 extern "C" size_t gs_gated_fwd_scratch_bytes(long M, long D, long F, int type) {
   if (M < 0 || D < 1 || F < 1 || !gs_type_bytes(type)) return 0;
-  return gf_plan(M, D, F, type).fwd * 2;
+  return gf_few(M, type) ? 0 : gf_plan(M, D, F, type).fwd * 2;
 }
 
 extern "C" size_t gs_gated_bwd_scratch_bytes(long M, long D, long F, int type) {
@@ -514,7 +819,7 @@ extern "C" int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const v
   GS_TRY(gf_check("gs_gated_fwd", c, type));
   if (ldh < F) GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: a row stride is below the width %ld", F);
   if (M == 0) return GS_OK;
-  if (!x || !w_gate || !w_up || !h || !scratch) GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: null pointer");
+  if (!x || !w_gate || !w_up || !h || (!scratch && !gf_few(M, type))) GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: null pointer");
   if ((size_t)scratch & 15) GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: the scratch is not 16-byte aligned");
   return gf_run(c, type, false, (hipStream_t)stream);
 }

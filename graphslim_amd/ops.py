@@ -19,6 +19,8 @@ import torch
 from . import _lib
 from ._lib import check
 
+_raw_stream = torch._C._cuda_getCurrentRawStream      # the handle of torch.cuda.current_stream(device), without an object around it
+
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 MAX_TOP = 1024
@@ -34,11 +36,12 @@ def _device(**tensors):
     for name, t in tensors.items():
         if not isinstance(t, torch.Tensor):
             _refuse(f"{name} is a tensor (got {type(t).__name__})")
-        if t.device.type != "cuda":
-            _refuse(f"{name} is on {t.device}: there is no CPU path")
-        if not (dev is None or t.device == dev):
+        if dev is None:
+            dev = t.device
+            if dev.type != "cuda":
+                _refuse(f"{name} is on {dev}: there is no CPU path")
+        elif t.device != dev:
             _refuse(f"{name} is on {t.device}, other arguments on {dev}")
-        dev = t.device
     return dev
 
 
@@ -46,23 +49,25 @@ def _matrix(name, t, cols=None, rows=None, dtype=None):
     """Row stride of a 2-D tensor with dense rows."""
     if t.dim() != 2:
         _refuse(f"{name} has two dimensions (got {tuple(t.shape)})")
+    n, c = t.shape
+    ld, step = t.stride()
+    if dtype is not None and t.dtype != dtype:
+        _refuse(f"{name} is {t.dtype}, other arguments {dtype}")
     if t.dtype not in TYPES:
         _refuse(f"{name} is fp32, fp16 or bf16 (got {t.dtype})")
-    if not (dtype is None or t.dtype == dtype):
-        _refuse(f"{name} is {t.dtype}, other arguments {dtype}")
-    if not (cols is None or t.shape[1] == cols):
-        _refuse(f"{name} has {t.shape[1]} columns, {cols} are wanted")
-    if not (rows is None or t.shape[0] == rows):
-        _refuse(f"{name} has {t.shape[0]} rows, {rows} are wanted")
-    if t.shape[1] <= 0:
+    if cols is not None and c != cols:
+        _refuse(f"{name} has {c} columns, {cols} are wanted")
+    if rows is not None and n != rows:
+        _refuse(f"{name} has {n} rows, {rows} are wanted")
+    if c == 0:
         _refuse(f"{name} has no columns")
-    if not (t.shape[1] == 1 or t.stride(1) == 1):
-        _refuse(f"the rows of {name} are not dense (strides {t.stride()})")
-    if t.shape[0] <= 1:
-        return t.shape[1]
-    if t.stride(0) < t.shape[1]:
-        _refuse(f"the rows of {name} overlap (strides {t.stride()})")
-    return t.stride(0)
+    if step != 1 and c > 1:
+        _refuse(f"the rows of {name} are not dense (strides {(ld, step)})")
+    if n <= 1:
+        return c
+    if ld < c:
+        _refuse(f"the rows of {name} overlap (strides {(ld, step)})")
+    return ld
 
 
 def _vector(name, t, n, dtype):
@@ -90,10 +95,12 @@ def _ptr(t):
 def _launch(dev, call, *args):
     """call(*args, stream) on the current stream of `dev`, with that device the current one."""
     if dev.index == torch.cuda.current_device():
-        check(call(*args, torch.cuda.current_stream(dev).cuda_stream))
+        rc = call(*args, _raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            check(call(*args, torch.cuda.current_stream(dev).cuda_stream))
+            rc = call(*args, _raw_stream(dev.index))
+    if rc:
+        check(rc)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -111,15 +118,14 @@ def embedding(table, ids, scale=1.0, out=None):
     _ids(ids)
     n, F = ids.numel(), table.shape[1]
     if out is None:
-        res = torch.empty(n, F, dtype=table.dtype, device=dev)
+        out = torch.empty(*ids.shape, F, dtype=table.dtype, device=dev)
         ldo = F
     else:
         _device(table=table, out=out)
         ldo = _matrix("out", out, F, n, table.dtype)
-        res = out
     _launch(dev, _lib.lib().gs_embedding_fwd, table.data_ptr(), ld, table.shape[0], F, TYPES[table.dtype], ids.data_ptr(), n, scale,
-            res.data_ptr(), ldo)
-    return res if out is not None else res.view(*ids.shape, F)
+            out.data_ptr(), ldo)
+    return out
 
 
 def embedding_grad(d_out, ids, n_rows, scale=1.0, out=None, accumulate=False, dtype=None):
