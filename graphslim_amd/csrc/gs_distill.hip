@@ -12,7 +12,7 @@ constexpr float DS_LOG2E = 1.4426950408889634f;
 
 struct DistillArgs {
   const void* Z;
-  long ldz;
+  long ldz, n;
   int V, k;
   const void* tv;
   const int* ti;
@@ -25,145 +25,358 @@ struct DistillArgs {
   long ldd;
 };
 
-template <int OP>   // 0 sum, 1 max
-__device__ __forceinline__ float ds_reduce(float v, float* sh) {
-  v = OP ? gs_wave_max(v) : gs_wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = sh[0];
-  for (int i = 1; i < (int)(blockDim.x >> 6); ++i) v = OP ? fmaxf(v, sh[i]) : v + sh[i];
-  return v;
-}
+__device__ __forceinline__ float ds_exp(float x) { return __builtin_amdgcn_exp2f(x * DS_LOG2E); }
 
 // log q = z / tau - lse; a masked class (-inf) stays at -inf whatever the log-sum is
 __device__ __forceinline__ float ds_logq(const DistillArgs& a, float z, float lse) {
   return z == -INFINITY ? z : fmaf(z, a.inv_lo, fmaf(z, a.inv_hi, -lse));
 }
 
-__device__ __forceinline__ float ds_exp(float x) { return __builtin_amdgcn_exp2f(x * DS_LOG2E); }
+// A barrier for what lies in LDS: loads of the row stay under way across it.
+__device__ __forceinline__ void ds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 
-// One workgroup per row.  STATS: the log-sum is taken from z (a running maximum and sum per thread, one pass), else it is given.
-template <int T, bool STATS, bool LOSS, bool GRAD>
-__global__ __launch_bounds__(256) void gs_distill_row_kernel(DistillArgs a) {
-  typedef typename GsElt<T>::type E;
-  constexpr int N = 16 / sizeof(E);
-  extern __shared__ float sh_top[];   // p [k], class [k]
-  __shared__ float red[4];
-  float* sp = sh_top;
-  int* si = (int*)(sh_top + a.k);
-  const long row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const E* z = (const E*)a.Z + row * a.ldz;
-  // the teacher's softmax
-  float tm = -INFINITY, any = 0.f;
-  for (int j = tid; j < a.k; j += 256) {
-    const int c = a.ti[row * a.k + j];
-    const float v = (float)((const E*)a.tv)[row * a.k + j] / a.tau;
-    const bool there = c >= 0 && c < a.V && v != -INFINITY;
-    si[j] = there ? c : -1;
-    sp[j] = there ? v : -INFINITY;
-    if (there) { any = 1.f; tm = fmaxf(tm, v); }
+// A row is worked on by G threads (a wave, or a workgroup).  Reductions over them: the wave's, then one value a wave through LDS, with
+// a slot for each reduction, so that one barrier does.
+template <int G, bool MAX>
+__device__ __forceinline__ float ds_reduce(float v, float* slot) {
+  v = MAX ? gs_wave_max(v) : gs_wave_sum(v);
+  if constexpr (G > 64) {
+    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+    ds_barrier();
+    v = slot[0];
+#pragma unroll
+    for (int i = 1; i < G / 64; ++i) v = MAX ? fmaxf(v, slot[i]) : v + slot[i];
   }
-  tm = ds_reduce<1>(tm, red);
-  any = ds_reduce<1>(any, red);
-  float ts = 0.f;
-  for (int j = tid; j < a.k; j += 256)
-    if (si[j] >= 0) ts += ds_exp(sp[j] - tm);
-  ts = ds_reduce<0>(ts, red);
-  const float lts = logf(ts);
+  return v;
+}
+
+// One row's teacher.  Every wave of the row finds out by itself whether there are any entries; the first one also keeps them in LDS
+// and works out the loss and the gradient at their classes, while the others are at the row.
+template <typename E>
+struct DistillTeacher {
+  static constexpr int WORDS = 4;   // of LDS per entry
+  int* c;       // [k rounded up to 4] class or -1
+  float* v;     // [k] t / tau, then log p
+  float* r;     // [k] gradient at the entry's class, if the entry is the first of that class
+  int* at;      // [k] that class, else -1
+  int c0;       // the first 64 entries: their loads come before the row's, so that they need not wait for it
+  float v0;
+  bool any;
+
+  __device__ __forceinline__ DistillTeacher(void* lds, int k) {
+    const int k4 = (k + 3) & ~3;
+    c = (int*)lds;
+    v = (float*)(c + k4);
+    r = v + k4;
+    at = (int*)(r + k4);
+  }
+
+  __device__ __forceinline__ void entry(const DistillArgs& a, long row, int j, int& cj, float& vj) {
+    cj = -1;
+    vj = -INFINITY;
+    if (j < a.k) {
+      cj = a.ti[row * a.k + j];
+      vj = (float)((const E*)a.tv)[row * a.k + j];
+    }
+  }
+
+  __device__ __forceinline__ void look(const DistillArgs& a, long row, int lane, bool first) {
+    const int k4 = (a.k + 3) & ~3;
+    bool have = false;
+    float top = -INFINITY;
+    for (int base = 0; base < k4; base += 64) {
+      const int j = base + lane;
+      int cj = c0;
+      float vj = v0;
+      if (base) entry(a, row, j, cj, vj);
+      const bool ok = cj >= 0 && cj < a.V && vj != -INFINITY;
+      have |= ok;
+      if (first && j < k4) {
+        vj /= a.tau;
+        c[j] = ok ? cj : -1;
+        v[j] = vj;
+        if (ok) top = fmaxf(top, vj);
+      }
+    }
+    any = __ballot(have) != 0;
+    if (!first) return;
+    top = gs_wave_max(top);
+    float s = 0.f;
+    for (int j = lane; j < a.k; j += 64)
+      if (c[j] >= 0) s += ds_exp(v[j] - top);
+    const float log_sum = logf(gs_wave_sum(s));
+    for (int j = lane; j < a.k; j += 64) v[j] = v[j] - top - log_sum;
+  }
+
+  // sum of p (log p - log q) over the entries
+  __device__ __forceinline__ float loss(const DistillArgs& a, const E* z, int lane, float lse) {
+    float s = 0.f;
+    for (int j = lane; j < a.k; j += 64)
+      if (c[j] >= 0) {
+        const float p = ds_exp(v[j]);
+        if (p != 0.f) s += p * (v[j] - ds_logq(a, (float)z[c[j]], lse));
+      }
+    return gs_wave_sum(s);
+  }
+
+  // The gradient at the entries' classes, w (q - sum of p over the entries of that class); before any of the row is written, since dz
+  // may lie on z.
+  template <typename QOf>
+  __device__ __forceinline__ void slopes(const DistillArgs& a, const E* z, int lane, float w, QOf q_of) {
+    for (int j = lane; j < a.k; j += 64) {
+      const int cj = c[j];
+      bool first = cj >= 0;
+      if (first) {
+        const float zc = (float)z[cj];
+        float p = 0.f;
+        for (int o = 0; o < a.k; o += 4) {
+          const int4 four = *(const int4*)(c + o);
+          const int cs[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (cs[e] == cj) {
+              p += ds_exp(v[o + e]);
+              first &= o + e >= j;
+            }
+        }
+        r[j] = w * (q_of(zc) - p);
+      }
+      at[j] = first ? cj : -1;
+    }
+  }
+
+  __device__ __forceinline__ void store(const DistillArgs& a, E* d, int lane) const {
+    for (int j = lane; j < a.k; j += 64)
+      if (at[j] >= 0) d[at[j]] = (E)r[j];
+  }
+};
+
+// The row in registers, EP logits a thread: read once, written once.
+template <int T, int G, int EP, bool LOSS, bool GRAD>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void gs_distill_regs_kernel(DistillArgs a) {
+  typedef typename GsElt<T>::type E;
+  constexpr int N = 16 / sizeof(E), NV = EP / N, ROWS = G < 256 ? 256 / G : 1, W = G / 64;
+  typedef typename GsVec<E, N>::type V;
+  extern __shared__ __attribute__((aligned(16))) char sh[];
+  __shared__ float red[2][W];
+  const int g = threadIdx.x % G, sub = threadIdx.x / G, lane = threadIdx.x & 63, full = a.V / N;
+  const bool first = g < 64;
+  const long mine = (long)blockIdx.x * ROWS + sub;
+  const bool live = mine < a.n;
+  const long row = live ? mine : a.n - 1;
+  const E* z = (const E*)a.Z + row * a.ldz;
+  DistillTeacher<E> t(sh + (size_t)sub * ((a.k + 3) & ~3) * 4 * DistillTeacher<E>::WORDS, a.k);
+  t.entry(a, row, lane, t.c0, t.v0);
   float w = 0.f;
   if (GRAD) w = a.w[row] * a.tau;
-  // the student's log-sum
-  float m = -INFINITY, s = 0.f, lse = 0.f;
-  if (STATS) {
-    for (long f = (long)tid * N; f < a.V; f += 256 * N) {
-      float v[N];
-      gs_load<E, N>(z + f, a.V - f, -INFINITY, v);
-      float mx = v[0];
+  V raw[NV];
 #pragma unroll
-      for (int i = 1; i < N; ++i) mx = fmaxf(mx, v[i]);
-      mx = fmaxf(mx, m);
-      const float ref = mx == -INFINITY ? 0.f : mx;
-      s *= ds_exp((m - ref) * a.inv_hi);
+  for (int i = 0; i < NV; ++i) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += ds_exp((v[i] - ref) * a.inv_hi);
-      m = mx;
-    }
-    const float all = ds_reduce<1>(m, red);
-    const float ref = all == -INFINITY ? 0.f : all;
-    s = ds_reduce<0>(s * ds_exp((m - ref) * a.inv_hi), red);
-    lse = ref / a.tau + logf(s);
-    m = ref;
-  } else {
-    lse = a.lse_in[row];
+    for (int e = 0; e < N; ++e) raw[i][e] = (E)-INFINITY;
+    if (i * G + g < full) raw[i] = *(const V*)(z + (long)(i * G + g) * N);
   }
-  if (LOSS) {
-    float sum = 0.f;
-    for (int j = tid; j < a.k; j += 256)
-      if (si[j] >= 0) {
-        const float lp = sp[j] - tm - lts, p = ds_exp(sp[j] - tm) / ts;
-        if (p != 0.f) sum += p * (lp - ds_logq(a, (float)z[si[j]], lse));
-      }
-    sum = ds_reduce<0>(sum, red);
-    if (tid == 0) {
-      a.loss[row] = any ? a.tau * a.tau * sum : 0.f;
+  float end = -INFINITY;                                  // what is left behind whole vectors: one element of the first lanes
+  const bool has_end = g < a.V - full * N;
+  if (has_end) end = (float)z[full * N + g];
+  t.look(a, row, lane, first);
+  float m = end;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < N; ++e) m = fmaxf(m, (float)raw[i][e]);
+  m = ds_reduce<G, true>(m, red[0]);
+  if (m == -INFINITY) m = 0.f;
+  const float c = a.inv_hi * DS_LOG2E;                     // (x - m first: x c - m c would be off by an ulp of m c)
+  auto e_of = [&](float v) { return __builtin_amdgcn_exp2f((v - m) * c); };
+  // fp32 rows keep the exponentials in place; 16-bit rows stay packed, half the registers, and are converted and raised again in each
+  // pass (opaque in between, or the compiler keeps what it has seen, in 32 bits)
+  constexpr bool KEEP = sizeof(E) == 4;
+  auto hide = [&] {
+    if constexpr (!KEEP) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(raw[i]));
+    }
+  };
+  hide();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float v = e_of((float)raw[i][e]);
+      if constexpr (KEEP) raw[i][e] = v;
+      s += v;
+    }
+  end = e_of(end);
+  s += end;
+  s = ds_reduce<G, false>(s, red[1]);
+  if (first) {
+    const float lse = m / a.tau + logf(s);
+    const float sum = t.loss(a, z, lane, lse);
+    if (lane == 0 && live) {
+      a.loss[row] = t.any ? a.tau * a.tau * sum : 0.f;
       if (a.lse) a.lse[row] = lse;
     }
+    if (GRAD) t.slopes(a, z, lane, w, [&](float zc) { return s == 0.f ? 0.f : e_of(zc) / s; });
   }
   if (!GRAD) return;
   E* d = (E*)a.dZ + row * a.ldd;
-  const bool zero = any == 0.f || w == 0.f;
-  // the entries' gradients, before any of the row is written (dz may lie on z); of equal classes the first one holds the sum
-  float mine[DS_MAX_TOP / 256];
-  int at[DS_MAX_TOP / 256];
+  const bool zero = !t.any || w == 0.f;
+  const float ws = s == 0.f ? 0.f : w / s;                // (all logits -inf: q = 0)
+  if (a.dZ == a.Z) __syncthreads();                       // in place: z has been read at the entries' classes
+  if (live) {
+    hide();
 #pragma unroll
-  for (int q = 0; q < DS_MAX_TOP / 256; ++q) {
-    const int j = tid + q * 256;
-    at[q] = -1;
-    if (j < a.k && !zero && si[j] >= 0) {
-      const int c = si[j];
-      float p = 0.f;
-      bool first = true;
-      for (int o = 0; o < a.k; ++o)
-        if (si[o] == c) {
-          p += ds_exp(sp[o] - tm) / ts;
-          first &= o >= j;
-        }
-      const float zc = (float)z[c];
-      const float qc = lse == -INFINITY ? 0.f
-                       : STATS          ? ds_exp((zc - m) * a.inv_hi) / s
-                                        : ds_exp(ds_logq(a, zc, lse));
-      mine[q] = w * (qc - p);
-      if (first) at[q] = c;
-    }
+    for (int i = 0; i < NV; ++i)
+      if (i * G + g < full) {
+        V r;
+#pragma unroll
+        for (int e = 0; e < N; ++e) r[e] = (E)(zero ? 0.f : (KEEP ? (float)raw[i][e] : e_of((float)raw[i][e])) * ws);
+        *(V*)(d + (long)(i * G + g) * N) = r;
+      }
+    if (has_end) d[full * N + g] = (E)(zero ? 0.f : end * ws);
   }
   __syncthreads();
-  const float ws = STATS ? (s == 0.f ? 0.f : w / s) : w;
-  for (long f = (long)tid * N; f < a.V; f += 256 * N) {
-    float v[N];
-    gs_load<E, N>(z + f, a.V - f, 0.f, v);
+  if (first && live && !zero) t.store(a, d, lane);
+}
+
+// Rows of any length, a workgroup each.  STATS: the log-sum is taken from z (a running maximum and sum per thread, one pass), else it is
+// given.
+template <int T, int G, bool STATS, bool LOSS, bool GRAD>
+__global__ __launch_bounds__(G) void gs_distill_row_kernel(DistillArgs a) {
+  typedef typename GsElt<T>::type E;
+  constexpr int N = 16 / sizeof(E), U = 4;
+  typedef typename GsVec<E, N>::type V;
+  extern __shared__ __attribute__((aligned(16))) char sh[];
+  __shared__ float red[2][G / 64];
+  const long row = blockIdx.x;
+  const int g = threadIdx.x, lane = g & 63, full = a.V / N;
+  const bool first = g < 64, has_end = g < a.V - full * N;
+  const E* z = (const E*)a.Z + row * a.ldz;
+  DistillTeacher<E> t(sh, a.k);
+  t.entry(a, row, lane, t.c0, t.v0);
+  float w = 0.f, lse = 0.f;
+  if (GRAD) w = a.w[row] * a.tau;
+  if (!STATS) lse = a.lse_in[row];
+  t.look(a, row, lane, first);
+  const bool zero = GRAD && (!t.any || w == 0.f);
+  const float c = a.inv_hi * DS_LOG2E;
+  float m = 0.f, s = 0.f;
+  if (STATS) {
+    m = -INFINITY;
+    auto add = [&](float mx, auto each) {                 // values whose maximum is mx
+      mx = fmaxf(mx, m);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      s *= __builtin_amdgcn_exp2f((m - ref) * c);
+      each(ref);
+      m = mx;
+    };
+    for (int base = 0; base < full; base += U * G) {
+      V r[U];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (zero || lse == -INFINITY) v[i] = 0.f;
-      else if (STATS) v[i] = ws * ds_exp((v[i] - m) * a.inv_hi);
-      else v[i] = ws * ds_exp(ds_logq(a, v[i], lse));
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) r[u][e] = (E)-INFINITY;
+        if (base + u * G + g < full) r[u] = *(const V*)(z + (long)(base + u * G + g) * N);
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e) mx = fmaxf(mx, (float)r[u][e]);
+      add(mx, [&](float ref) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < N; ++e) s += __builtin_amdgcn_exp2f(((float)r[u][e] - ref) * c);
+      });
     }
-    gs_store<E, N>(d + f, a.V - f, v);
+    if (has_end) {
+      const float v = (float)z[full * N + g];
+      add(v, [&](float ref) { s += __builtin_amdgcn_exp2f((v - ref) * c); });
+    }
+    float all = ds_reduce<G, true>(m, red[0]);
+    if (all == -INFINITY) all = 0.f;
+    s = ds_reduce<G, false>(s * __builtin_amdgcn_exp2f((m - all) * c), red[1]);
+    m = all;
+    lse = m / a.tau + logf(s);
   }
-  __syncthreads();
+  auto q_of = [&](float v) {
+    if (STATS) return __builtin_amdgcn_exp2f((v - m) * c);
+    return ds_exp(fminf(ds_logq(a, v, lse), 0.f));        // (a log-sum of 1e38 in fp32 is off by more than any exponent)
+  };
+  const float over = STATS ? (s == 0.f ? 0.f : 1.f / s) : (lse == -INFINITY ? 0.f : (lse == lse ? 1.f : lse)), ws = w * over;
+  if (first) {
+    if (LOSS) {
+      const float sum = t.loss(a, z, lane, lse);
+      if (lane == 0) {
+        a.loss[row] = t.any ? a.tau * a.tau * sum : 0.f;
+        if (a.lse) a.lse[row] = lse;
+      }
+    }
+    if (GRAD) t.slopes(a, z, lane, w, [&](float zc) { return q_of(zc) * over; });
+  }
+  if (!GRAD) return;
+  E* d = (E*)a.dZ + row * a.ldd;
+  if (a.dZ == a.Z) __syncthreads();                       // in place: z has been read at the entries' classes
+  for (int base = 0; base < full; base += U * G) {
+    V r[U];
 #pragma unroll
-  for (int q = 0; q < DS_MAX_TOP / 256; ++q)
-    if (at[q] >= 0) d[at[q]] = (E)mine[q];
+    for (int u = 0; u < U; ++u)
+      if (!zero && base + u * G + g < full) r[u] = *(const V*)(z + (long)(base + u * G + g) * N);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (base + u * G + g < full) {
+        V o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = (E)(zero ? 0.f : q_of((float)r[u][e]) * ws);
+        *(V*)(d + (long)(base + u * G + g) * N) = o;
+      }
+  }
+  if (has_end) d[full * N + g] = (E)(zero ? 0.f : q_of((float)z[full * N + g]) * ws);
+  __syncthreads();
+  if (first && !zero) t.store(a, d, lane);
+}
+
+inline size_t ds_lds(int k) { return (size_t)((k + 3) & ~3) * 4 * DistillTeacher<float>::WORDS; }
+
+template <int T, int G, int EP, bool LOSS, bool GRAD>
+void ds_regs(const DistillArgs& a, hipStream_t s) {
+  constexpr int ROWS = G < 256 ? 256 / G : 1;
+  gs_distill_regs_kernel<T, G, EP, LOSS, GRAD><<<dim3((unsigned)((a.n + ROWS - 1) / ROWS)), dim3(G < 256 ? 256 : G), ROWS * ds_lds(a.k), s>>>(a);
+}
+
+// Rows that fit the registers are read once; a wave works on the shortest.  Where a choice is left, the fewest threads: several rows
+// on a compute unit overlap one's loads with another's arithmetic and barriers (8192 x 32000 bf16: 512 threads of 64 logits 222 us =
+// 4.7 TB/s, 1024 of 32 248 us; 2048 x 60000: 512 of 128 120 us, 1024 of 64 143 us).  Longer rows, and losses alone, which gain nothing
+// from holding a long row, are walked (1024 x 131072 bf16, loss and gradient: 128 us held, 159 us walked twice).
+template <int T, bool LOSS, bool GRAD>
+void ds_stats(const DistillArgs& a, hipStream_t s) {
+  const bool few = a.k <= 256;                            // (four rows' entries in a workgroup's LDS)
+  if (few && a.V <= 64 * 8) return ds_regs<T, 64, 8, LOSS, GRAD>(a, s);
+  if (few && a.V <= 64 * 32) return ds_regs<T, 64, 32, LOSS, GRAD>(a, s);
+  if (a.V <= 256 * 32) return ds_regs<T, 256, 32, LOSS, GRAD>(a, s);
+  if (a.V <= 512 * 32) return ds_regs<T, 512, 32, LOSS, GRAD>(a, s);
+  if (a.V <= 512 * 64) return ds_regs<T, 512, 64, LOSS, GRAD>(a, s);
+  if constexpr (T == GS_TYPE_F32) {
+    if (GRAD && a.V <= 1024 * 64) return ds_regs<T, 1024, 64, LOSS, GRAD>(a, s);
+  } else {
+    if (GRAD && a.V <= 512 * 128) return ds_regs<T, 512, 128, LOSS, GRAD>(a, s);
+    if (GRAD && a.V <= 1024 * 128) return ds_regs<T, 1024, 128, LOSS, GRAD>(a, s);
+  }
+  gs_distill_row_kernel<T, 1024, true, LOSS, GRAD><<<dim3((unsigned)a.n), dim3(1024), ds_lds(a.k), s>>>(a);
 }
 
 template <int T>
-int ds_launch(const DistillArgs& a, long n, hipStream_t s) {
-  const dim3 grid((unsigned)n), block(256);
-  const size_t lds = (size_t)a.k * 8;
-  if (!a.dZ) gs_distill_row_kernel<T, true, true, false><<<grid, block, lds, s>>>(a);
-  else if (a.loss) gs_distill_row_kernel<T, true, true, true><<<grid, block, lds, s>>>(a);
-  else gs_distill_row_kernel<T, false, false, true><<<grid, block, lds, s>>>(a);
+int ds_launch(const DistillArgs& a, hipStream_t s) {
+  if (!a.dZ) ds_stats<T, true, false>(a, s);
+  else if (a.loss) ds_stats<T, true, true>(a, s);
+  else gs_distill_row_kernel<T, 512, false, false, true><<<dim3((unsigned)a.n), dim3(512), ds_lds(a.k), s>>>(a);
   GS_LAUNCH_CHECK();
   return GS_OK;
 }
@@ -179,9 +392,9 @@ int ds_run(const char* who, DistillArgs a, int type, long n, hipStream_t s) {
   if (!a.Z || !a.tv || !a.ti) GS_FAIL(GS_ERR_ARG, "%s: null pointer", who);
   a.inv_hi = 1.f / a.tau;
   a.inv_lo = (float)(1.0 / (double)a.tau - (double)a.inv_hi);
-  if (type == GS_TYPE_F32) return ds_launch<GS_TYPE_F32>(a, n, s);
-  if (type == GS_TYPE_F16) return ds_launch<GS_TYPE_F16>(a, n, s);
-  return ds_launch<GS_TYPE_BF16>(a, n, s);
+  if (type == GS_TYPE_F32) return ds_launch<GS_TYPE_F32>(a, s);
+  if (type == GS_TYPE_F16) return ds_launch<GS_TYPE_F16>(a, s);
+  return ds_launch<GS_TYPE_BF16>(a, s);
 }
 
 }  // namespace
@@ -189,20 +402,20 @@ int ds_run(const char* who, DistillArgs a, int type, long n, hipStream_t s) {
 extern "C" int gs_distill_fwd(const void* Z, long ldz, int type, long n, int V, const void* top_val, const int* top_cls, int k, float tau,
                               float* loss, float* lse, gs_stream_t stream) {
   if (n > 0 && (!loss || !lse)) GS_FAIL(GS_ERR_ARG, "gs_distill_fwd: null pointer");
-  DistillArgs a = {Z, ldz, V, k, top_val, top_cls, tau, 0.f, 0.f, nullptr, nullptr, loss, lse, nullptr, 0};
+  DistillArgs a = {Z, ldz, n, V, k, top_val, top_cls, tau, 0.f, 0.f, nullptr, nullptr, loss, lse, nullptr, 0};
   return ds_run("gs_distill_fwd", a, type, n, (hipStream_t)stream);
 }
 
 extern "C" int gs_distill_bwd(const void* Z, long ldz, int type, long n, int V, const void* top_val, const int* top_cls, int k, float tau,
                               const float* lse, const float* d_loss, void* dZ, long ldd, gs_stream_t stream) {
   if (n > 0 && (!lse || !d_loss || !dZ)) GS_FAIL(GS_ERR_ARG, "gs_distill_bwd: null pointer");
-  DistillArgs a = {Z, ldz, V, k, top_val, top_cls, tau, 0.f, 0.f, lse, d_loss, nullptr, nullptr, dZ, ldd};
+  DistillArgs a = {Z, ldz, n, V, k, top_val, top_cls, tau, 0.f, 0.f, lse, d_loss, nullptr, nullptr, dZ, ldd};
   return ds_run("gs_distill_bwd", a, type, n, (hipStream_t)stream);
 }
 
 extern "C" int gs_distill_loss_grad(const void* Z, long ldz, int type, long n, int V, const void* top_val, const int* top_cls, int k,
                                     float tau, const float* d_loss, float* loss, void* dZ, long ldd, gs_stream_t stream) {
   if (n > 0 && (!d_loss || !loss || !dZ)) GS_FAIL(GS_ERR_ARG, "gs_distill_loss_grad: null pointer");
-  DistillArgs a = {Z, ldz, V, k, top_val, top_cls, tau, 0.f, 0.f, nullptr, d_loss, loss, nullptr, dZ, ldd};
+  DistillArgs a = {Z, ldz, n, V, k, top_val, top_cls, tau, 0.f, 0.f, nullptr, d_loss, loss, nullptr, dZ, ldd};
   return ds_run("gs_distill_loss_grad", a, type, n, (hipStream_t)stream);
 }

@@ -117,7 +117,8 @@ def distill(z, tv, ti, tau, d_loss=None, lse_in=None):
     zt = z / tau
     lse = torch.logsumexp(zt, 1)
     zc = zt.gather(1, at)
-    logq = torch.where(lse[:, None] == -math.inf, -math.inf, zc - lse[:, None])
+    # (shifted by the maximum, not by lse: at 1e38 even 64 bits hold no log-sum beside it)
+    logq = torch.where(lse[:, None] == -math.inf, -math.inf, torch.log_softmax(zt, 1).gather(1, at))
     terms = torch.where(there & (p != 0), p * (logp - logq), 0.0)
     loss = tau * tau * terms.sum(1)
     # exp of a difference d: its argument carries 4 roundings of |d|, exp2 itself 2; underflow to 0 is below 2^-126
@@ -147,7 +148,8 @@ def distill(z, tv, ti, tau, d_loss=None, lse_in=None):
     else:
         lse_used = lse
         eq = 4 * spread * U + esum[:, None] + 10 * U
-    q = torch.where(lse_used[:, None] == -math.inf, 0.0, torch.exp(zt - lse_used[:, None]))
+    q = torch.exp(zt - lse_used[:, None]) if lse_in is not None else torch.softmax(zt, 1)
+    q = torch.where(lse_used[:, None] == -math.inf, 0.0, q)
     w = torch.where(any_there, d_loss.double() * tau, 0.0)[:, None]
     on = w[:, 0] != 0
     g, mag = torch.zeros_like(q), torch.zeros_like(q)

@@ -325,6 +325,28 @@ def test_distill_masks(ops, dtype, V):
         assert not grad[r].any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [33, 3000, 40000, 70001])
+def test_distill_extreme_values(ops, dtype, V):
+    """Rows of nothing but the type's lowest value (all classes masked that way: q is even), of its highest, and of both."""
+    g = gen("extreme", V)
+    big = torch.finfo(dtype).max
+    z = torch.full((4, V), -big, dtype=dtype)
+    z[1], z[2, ::2], z[3, 5] = big, big, 0.0
+    tv, ti = teacher(g, 4, V, 4, dtype, ragged=False)
+    ti[2], ti[3] = torch.tensor([0, 2, 4, 6], dtype=torch.int32), torch.tensor([5, 5, 5, 5], dtype=torch.int32)
+    want = R.distill(z, tv, ti, 2.0, torch.ones(4))
+    zd, td, id_, wd = z.to(DEV), tv.to(DEV), ti.to(DEV), torch.ones(4, device=DEV)
+    loss, lse = ops.distill(zd, td, id_, 2.0)
+    R.within(loss, want["loss"], "loss")
+    R.within(lse, want["lse"], "lse")
+    both, grad = ops.distill_loss_grad(zd, td, id_, wd, 2.0)
+    R.within(both, want["loss"], "loss of the call for both")
+    R.within(grad, want["d_logits"], "gradient of the call for both")
+    # a log-sum in fp32 resolves no class beside 1e38: q is some number of [0, 1] there, and no more can be said
+    assert (ops.distill_grad(zd, td, id_, lse, wd, 2.0).abs() <= 2.0 * 2).all()
+
+
 def test_distill_nan_stays_in_its_row(ops):
     g = gen("nan")
     z = normal(g, 5, 300)
@@ -334,6 +356,8 @@ def test_distill_nan_stays_in_its_row(ops):
     z[2, 250] = float("nan")
     loss, grad = [t.cpu() for t in ops.distill_loss_grad(z.to(DEV), tv.to(DEV), ti.to(DEV), w.to(DEV))]
     assert math.isnan(loss[2]) and torch.isnan(grad[2]).all()
+    lse = ops.distill(z.to(DEV), tv.to(DEV), ti.to(DEV))[1]
+    assert torch.isnan(ops.distill_grad(z.to(DEV), tv.to(DEV), ti.to(DEV), lse, w.to(DEV))[2]).all()
     keep = [0, 1, 3, 4]
     assert torch.equal(loss[keep], clean[0][keep]) and torch.equal(grad[keep], clean[1][keep])
 
