@@ -1,6 +1,8 @@
 // Embedding lookup with scaling, and the gradient of its table:
 //   out[t] = s W[id_t]              (0 where id_t is no row of the table: padding)
 //   dW[v]  = s sum_{t : id_t = v} dOut[t], the tokens in ascending order, in fp32, rounded once.
+#include <algorithm>
+
 #include "gs_types.h"
 
 namespace {
@@ -36,28 +38,33 @@ __global__ __launch_bounds__(256) void gs_embedding_fwd_kernel(const typename Gs
 //   few tokens:  one launch, every workgroup picks its bucket's tokens out of all ids itself.
 //   many:        gs_embedding_count / _place sort the tokens by bucket first; a bucket of more than EM_SPAN tokens (a frequent id) is
 //                cut into spans with a workgroup each, whose sums gs_embedding_join adds in the spans' order.
-constexpr int EM_TILE = 1024;      // ids per workgroup of the sort: four a thread, all loaded at once
-constexpr int EM_WAVES = 8;        // waves of a workgroup that sums
+constexpr int EM_TILE = 4096;      // ids per workgroup of the sort: four a thread, all loaded at once
+constexpr int EM_WAVES = 8;        // waves of a workgroup that sums a span
+constexpr int EM_WAVES_DIRECT = 16;
 constexpr int EM_SPAN = 256;       // tokens of a bucket per workgroup
 constexpr int EM_MAX_BUCKETS = 2048;
 constexpr int EM_MAX_R = 1024;     // rows of a bucket at most
 constexpr long EM_MAX_V = (long)EM_MAX_R * EM_MAX_BUCKETS;
-constexpr long EM_DIRECT = 6144;   // tokens up to which one launch does it all
+constexpr long EM_DIRECT = 8192;   // tokens up to which one launch does it all
 
 struct EmbPlan {
-  int R, nb, nbp;      // rows per bucket (a power of two), buckets, rounded up to 8
+  int R, nb, nbp;      // rows per bucket (sorted: a power of two), buckets, rounded up to 8
   int tiles, extra;    // sort tiles; workgroups for the second and further spans
   bool direct;
-  size_t cnt, start, xs, list, ptrs, part, bytes;
+  size_t cnt, start, xs, owner, list, ptrs, part, bytes;
 };
 
 EmbPlan emb_plan(long n, long V, int F) {
   EmbPlan p;
-  p.R = 4;
-  while ((V + p.R - 1) / p.R > 1024 && p.R < 64) p.R *= 2;
-  while ((V + p.R - 1) / p.R > EM_MAX_BUCKETS) p.R *= 2;
+  p.direct = n <= EM_DIRECT;
+  if (p.direct) {        // one bucket for each compute unit, of up to 64 rows
+    p.R = (int)std::min(std::max(gs_cdiv(V, 256), 4), 64);
+  } else {
+    p.R = 4;
+    while ((V + p.R - 1) / p.R > 1024 && p.R < 64) p.R *= 2;
+    while ((V + p.R - 1) / p.R > EM_MAX_BUCKETS) p.R *= 2;
+  }
   p.nb = gs_cdiv(V, p.R);
-  p.direct = n <= EM_DIRECT && p.R <= 64;
   p.tiles = gs_cdiv(n, EM_TILE);
   p.extra = (int)(n / EM_SPAN);
   size_t o = 0;
@@ -66,6 +73,7 @@ EmbPlan emb_plan(long n, long V, int F) {
   p.cnt = take((size_t)p.tiles * p.nbp * 4);
   p.start = take((size_t)(p.nb + 1) * 4);
   p.xs = take((size_t)(p.nb + 1) * 4);
+  p.owner = take((size_t)p.extra * 4);
   p.list = take((size_t)n * 8);
   p.ptrs = take((size_t)2 * p.extra * p.R * 4);
   p.part = take((size_t)2 * p.extra * (p.R < EM_SPAN ? p.R : EM_SPAN) * F * 4);
@@ -85,67 +93,62 @@ __device__ __forceinline__ unsigned long long emb_match(int key, bool on, int bi
 }
 
 // cnt[tile][bucket]: tokens of the tile in the bucket (rows of nbp = nb rounded up to 8 counts)
-__global__ __launch_bounds__(256) void gs_embedding_count_kernel(const int* __restrict__ ids, long n, long V, int rshift, int nbp,
-                                                                 int* __restrict__ cnt) {
+__global__ __launch_bounds__(1024) void gs_embedding_count_kernel(const int* __restrict__ ids, long n, long V, int rshift, int nbp,
+                                                                  int* __restrict__ cnt) {
   __shared__ int h[EM_MAX_BUCKETS];
+  constexpr int Q = EM_TILE / 1024;
   const long t0 = (long)blockIdx.x * EM_TILE;
-  int id[EM_TILE / 256];
+  int id[Q];
 #pragma unroll
-  for (int i = 0; i < EM_TILE / 256; ++i) {
-    const long t = t0 + i * 256 + threadIdx.x;
+  for (int i = 0; i < Q; ++i) {
+    const long t = t0 + i * 1024 + threadIdx.x;
     id[i] = t < n ? ids[t] : -1;
   }
-  for (int b = threadIdx.x; b < nbp; b += 256) h[b] = 0;
+  for (int b = threadIdx.x; b < nbp; b += 1024) h[b] = 0;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < EM_TILE / 256; ++i)
+  for (int i = 0; i < Q; ++i)
     if (id[i] >= 0 && id[i] < V) atomicAdd(&h[id[i] >> rshift], 1);
   __syncthreads();
-  for (int b = threadIdx.x; b < nbp; b += 256) cnt[(long)blockIdx.x * nbp + b] = h[b];
+  for (int b = threadIdx.x; b < nbp; b += 1024) cnt[(long)blockIdx.x * nbp + b] = h[b];
 }
 
 // Stable: a tile's place in a bucket follows from the counts of the tiles before it, a wave's from those of the waves before it, a
-// lane's from the lanes before it.  start[b]: where bucket b begins in the list; xs[b]: further spans of the buckets before b.
-__global__ __launch_bounds__(256) void gs_embedding_place_kernel(const int* __restrict__ ids, long n, long V, int rshift, int nb, int nbp,
-                                                                 int bits, const int* __restrict__ cnt, int tiles,
-                                                                 int* __restrict__ start, int* __restrict__ xs, int2* __restrict__ list) {
-  __shared__ int pos[4][EM_MAX_BUCKETS];     // per wave: the next place of each bucket
-  __shared__ int wsum[4], wext[4];
+// lane's from the lanes before it.  start[b]: where bucket b begins in the list; xs[b]: further spans of the buckets before b; owner[e]:
+// the bucket of further span e, or -1.
+__global__ __launch_bounds__(1024) void gs_embedding_place_kernel(const int* __restrict__ ids, long n, long V, int rshift, int nb, int nbp,
+                                                                  int bits, const int* __restrict__ cnt, int tiles,
+                                                                  int* __restrict__ start, int* __restrict__ xs, int* __restrict__ owner,
+                                                                  int extra, int2* __restrict__ list) {
+  constexpr int W = 16, Q = EM_TILE / 1024, PER = EM_MAX_BUCKETS / 1024;
+  static_assert(PER == 2 && EM_TILE < 65536, "two buckets a thread; places within a tile in 16 bits");
+  __shared__ unsigned short pos[W][EM_MAX_BUCKETS];   // per wave: the next place of each bucket, from the tile's first one
+  __shared__ int first[EM_MAX_BUCKETS];
+  __shared__ int wsum[W], wext[W];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  constexpr int Q = EM_TILE / 256;
-  const long t0 = (long)blockIdx.x * EM_TILE + wave * (EM_TILE / 4) + lane;
+  const long t0 = (long)blockIdx.x * EM_TILE + wave * (EM_TILE / W) + lane;
   int id[Q];
 #pragma unroll
   for (int i = 0; i < Q; ++i) {
     id[i] = t0 + i * 64 < n ? ids[t0 + i * 64] : -1;
     if (id[i] >= V) id[i] = -1;
   }
-  for (int b = tid; b < nb; b += 256) pos[0][b] = pos[1][b] = pos[2][b] = pos[3][b] = 0;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < Q; ++i)
-    if (id[i] >= 0) atomicAdd(&pos[wave][id[i] >> rshift], 1);
-  constexpr int PER = EM_MAX_BUCKETS / 256;  // consecutive buckets of a thread, so that its prefix is a running one
-  static_assert(PER == 8, "two 16-byte loads");
-  int before[PER] = {}, all[PER] = {}, mine = 0, ext = 0;
+  int before[PER] = {}, all[PER] = {};
   if (tid * PER < nbp) {
-    const int4* c = (const int4*)(cnt + tid * PER);
-#pragma unroll 4
+    const int2* c = (const int2*)cnt + tid;
+#pragma unroll 8
     for (int t = 0; t < tiles; ++t) {
-      const int4 u = c[(long)t * (nbp / 4)], v = c[(long)t * (nbp / 4) + 1];
-      const int x[PER] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        all[j] += x[j];
-        before[j] += t < (int)blockIdx.x ? x[j] : 0;
-      }
+      const int2 u = c[(long)t * (nbp / 2)];
+      const bool low = t < (int)blockIdx.x;
+      all[0] += u.x;
+      all[1] += u.y;
+      before[0] += low ? u.x : 0;
+      before[1] += low ? u.y : 0;
     }
   }
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    mine += all[j];
-    ext += all[j] > 0 ? (all[j] - 1) / EM_SPAN : 0;
-  }
+  for (int i = tid; i < W * EM_MAX_BUCKETS / 2; i += 1024) ((int*)pos)[i] = 0;
+  const int spans[PER] = {all[0] > 0 ? (all[0] - 1) / EM_SPAN : 0, all[1] > 0 ? (all[1] - 1) / EM_SPAN : 0};
+  const int mine = all[0] + all[1], ext = spans[0] + spans[1];
   int inc = mine, einc = ext;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -154,43 +157,68 @@ __global__ __launch_bounds__(256) void gs_embedding_place_kernel(const int* __re
   }
   if (lane == 63) { wsum[wave] = inc; wext[wave] = einc; }
   __syncthreads();
-  int base = inc - mine, ebase = einc - ext;
-  for (int w = 0; w < wave; ++w) { base += wsum[w]; ebase += wext[w]; }
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int b = tid * PER + j;
-    if (b >= nb) break;
-    if (blockIdx.x == 0) { start[b] = base; xs[b] = ebase; }
-    int at = base + before[j];
-    for (int w = 0; w < 4; ++w) {
-      const int c = pos[w][b];
-      pos[w][b] = at;
-      at += c;
-    }
-    base += all[j];
-    ebase += all[j] > 0 ? (all[j] - 1) / EM_SPAN : 0;
-    if (blockIdx.x == 0 && b == nb - 1) { start[nb] = base; xs[nb] = ebase; }
-  }
-  __syncthreads();
+  // counts of the wave's quarter thousand, stably numbered at once: a lane's number among its like, and the wave's total
+  unsigned rank[Q];
 #pragma unroll
   for (int i = 0; i < Q; ++i) {
     const bool on = id[i] >= 0;
     const int b = on ? id[i] >> rshift : 0;
     const unsigned long long same = emb_match(b, on, bits);
+    rank[i] = 0;
     if (on) {
-      volatile int* p = &pos[wave][b];
-      const int at = *p;
-      list[at + __popcll(same & ((1ull << lane) - 1))] = make_int2((int)(t0 + i * 64), id[i]);
-      if ((same >> lane) == 1) *p = at + __popcll(same);     // the last lane of its kind, after all have read (one wave, in order)
+      volatile unsigned short* p = &pos[wave][b];
+      const unsigned at = *p;
+      rank[i] = at + __popcll(same & ((1ull << lane) - 1));
+      if ((same >> lane) == 1) *p = (unsigned short)(at + __popcll(same));     // the last lane of its kind, after all have read
     }
     __builtin_amdgcn_wave_barrier();
   }
+  int base = inc - mine, ebase = einc - ext;
+  for (int w = 0; w < wave; ++w) { base += wsum[w]; ebase += wext[w]; }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int b = tid * PER + j;
+    if (b >= nb) break;
+    first[b] = base + before[j];
+    unsigned at = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const unsigned c = pos[w][b];
+      pos[w][b] = (unsigned short)at;
+      at += c;
+    }
+    if (blockIdx.x == 0) {
+      start[b] = base;
+      xs[b] = ebase;
+      for (int e = 0; e < spans[j]; ++e) owner[ebase + e] = b;
+    }
+    base += all[j];
+    ebase += spans[j];
+    if (blockIdx.x == 0 && b == nb - 1) {
+      start[nb] = base;
+      xs[nb] = ebase;
+    }
+  }
+  if (blockIdx.x == 0) {                              // further spans that there are not
+    int total = 0;
+    for (int w = 0; w < W; ++w) total += wext[w];
+    for (int e = total + tid; e < extra; e += 1024) owner[e] = -1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < Q; ++i)
+    if (id[i] >= 0) {
+      const int b = id[i] >> rshift;
+      list[first[b] + pos[wave][b] + rank[i]] = make_int2((int)(t0 + i * 64), id[i]);
+    }
 }
 
 struct EmbSum {
   const int* ids;        // direct: all ids
   const int* start;      // sorted: as gs_embedding_place_kernel left them
   const int* xs;
+  const int* owner;
   const int2* list;
   int* ptrs;             // [2 extra][R]: place of a row's sum in its span's slot or -1, where a bucket has several spans
   float* part;           // [2 extra][slot rows][F]: their sums
@@ -199,7 +227,7 @@ struct EmbSum {
   void* dW;
   long ldw;
   long n, V;
-  int F, R, rshift, nb, extra, slot_rows, cap, cw;
+  int F, R, rshift, nb, extra, slot_rows, cap, cw, cws, rbits;
   float scale;
   int accumulate;
 };
@@ -217,13 +245,12 @@ __device__ __forceinline__ void emb_store(E* __restrict__ row, int f, int f0, co
   }
 }
 
-template <int TO, int N>
-__device__ __forceinline__ void emb_write(const EmbSum& a, long row, int f, int f0, float* acc) {
-  typedef typename GsElt<TO>::type EO;
-  EO* o = (EO*)a.dW + row * a.ldw;
+// A finished sum into its row of the table's gradient
+template <typename EO, int N>
+__device__ __forceinline__ void emb_write(EO* __restrict__ o, bool accumulate, float scale, int f, int f0, float* acc) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] *= a.scale;
-  if (a.accumulate) {
+  for (int i = 0; i < N; ++i) acc[i] *= scale;
+  if (accumulate) {
     float old[N];
     gs_load<EO, N>(o + f, N, 0.f, old);
 #pragma unroll
@@ -237,11 +264,13 @@ __device__ __forceinline__ void emb_write(const EmbSum& a, long row, int f, int 
 // from one part into the next is summed by the wave that it begins in, from what the others leave in LDS, in order.
 // Blocks [0, extra) are the further spans, the longest work, and begin first.
 template <int T, int TO, int N, bool DIRECT>
-__global__ __launch_bounds__(EM_WAVES * 64) void gs_embedding_sum_kernel(EmbSum a) {
+__global__ __launch_bounds__((DIRECT ? EM_WAVES_DIRECT : EM_WAVES) * 64) void gs_embedding_sum_kernel(EmbSum a) {
   typedef typename GsElt<T>::type E;
   typedef typename GsElt<TO>::type EO;
   typedef typename GsVec<E, N>::type V;
-  constexpr int U = 8, W = EM_WAVES;                   // rows of dout in flight per lane
+  constexpr int U = DIRECT ? 16 : 8;                   // rows of dout in flight per lane
+  constexpr int W = DIRECT ? EM_WAVES_DIRECT : EM_WAVES, WS = DIRECT ? 4 : 3;
+  static_assert(1 << WS == W, "a power of two");
   extern __shared__ int dyn[];
   int* ptr = dyn;                                      // [R + 1] where a row's tokens begin
   int* cnt = ptr + a.R + 1;                            // [W][R] per wave: tokens of a row, then the next one's place
@@ -249,23 +278,16 @@ __global__ __launch_bounds__(EM_WAVES * 64) void gs_embedding_sum_kernel(EmbSum 
   unsigned short* sr = (unsigned short*)(st + a.cap);  // [cap] their rows in the bucket
   unsigned short* place = sr + a.cap;                  // [R] rows with tokens before this one
   __shared__ float slot_sum[W][64][N];                 // a wave's part of a run that began before its part
-  __shared__ int found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int b, span = 0, spans = 1, i0 = 0, i1 = (int)a.n, slot = 0;
   if (DIRECT) {
     b = blockIdx.x;
   } else {
-    if ((int)blockIdx.x < a.extra) {                   // which bucket this further span is of
-      if (tid == 0) found[0] = -1;
-      __syncthreads();
-      const int e = blockIdx.x;
-      for (int q = tid; q < a.nb; q += W * 64)
-        if (a.xs[q] <= e && e < a.xs[q + 1]) { found[0] = q; found[1] = e - a.xs[q] + 1; }
-      __syncthreads();
-      if (found[0] < 0) return;
-      b = found[0];
-      span = found[1];
-      slot = e;
+    if ((int)blockIdx.x < a.extra) {
+      slot = blockIdx.x;
+      b = a.owner[slot];
+      if (b < 0) return;
+      span = slot - a.xs[b] + 1;
     } else {
       b = blockIdx.x - a.extra;
       slot = a.extra + a.xs[b];
@@ -274,32 +296,45 @@ __global__ __launch_bounds__(EM_WAVES * 64) void gs_embedding_sum_kernel(EmbSum 
     i0 = a.start[b] + span * EM_SPAN;
     i1 = min(i0 + EM_SPAN, a.start[b + 1]);
   }
-  const long row0 = (long)b << a.rshift;
+  const long row0 = (long)b * a.R;
   const int rows = (int)min((long)a.R, a.V - row0);
-  // stable counting sort of items [i0, i1) by row: each wave takes a share, in order
-  const int len = i1 - i0, q = ((len + W - 1) / W + 63) / 64 * 64;
-  const int w0 = min(i0 + wave * q, i1), w1 = min(w0 + q, i1);
-  auto item = [&](int i, int& t) -> int {              // its row in the bucket, or -1
-    if (i >= w1) return -1;
-    if (DIRECT) {
-      t = i;
-      const long r = (long)a.ids[i] - row0;
-      return r >= 0 && r < rows ? (int)r : -1;
+  // stable counting sort of items [i0, i1) by row: each wave takes 64 P of them, in order
+  constexpr int P = DIRECT ? (int)(EM_DIRECT / (W * 64)) : 1;
+  static_assert(W * 64 * P >= (DIRECT ? EM_DIRECT : EM_SPAN), "one go");
+  int t[P], r[P];                                      // tokens, their rows in the bucket or -1
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const int i = i0 + (wave * P + j) * 64 + lane;
+    r[j] = -1;
+    t[j] = i;
+    if (i < i1) {
+      long row;
+      if (DIRECT) {
+        row = a.ids[i];
+      } else {
+        const int2 v = a.list[i];
+        t[j] = v.x;
+        row = v.y;
+      }
+      row -= row0;
+      if (row >= 0 && row < rows) r[j] = (int)row;
     }
-    const int2 v = a.list[i];
-    t = v.x;
-    return (int)(v.y - row0);
-  };
+  }
   for (int i = tid; i < W * a.R; i += W * 64) cnt[i] = 0;
   __syncthreads();
-  constexpr int P = DIRECT ? 8 : 1;                    // items in flight per lane
-  for (int i = w0; i < w1; i += 64 * P) {
-    int t, r[P];
+  unsigned short rank[P];                              // among the wave's items of the row
 #pragma unroll
-    for (int j = 0; j < P; ++j) r[j] = item(i + j * 64 + lane, t);
-#pragma unroll
-    for (int j = 0; j < P; ++j)
-      if (r[j] >= 0) atomicAdd(&cnt[wave * a.R + r[j]], 1);
+  for (int j = 0; j < P; ++j) {
+    rank[j] = 0;
+    if (!__ballot(r[j] >= 0)) continue;
+    const unsigned long long same = emb_match(r[j], r[j] >= 0, a.rbits);
+    if (r[j] >= 0) {
+      volatile int* p = &cnt[wave * a.R + r[j]];
+      const int at = *p;
+      rank[j] = (unsigned short)(at + __popcll(same & ((1ull << lane) - 1)));
+      if ((same >> lane) == 1) *p = at + __popcll(same);   // the last lane of its kind, after all have read (one wave, in order)
+    }
+    __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
   if (wave == 0) {                                     // exclusive prefix, row by row and within a row wave by wave
@@ -326,81 +361,71 @@ __global__ __launch_bounds__(EM_WAVES * 64) void gs_embedding_sum_kernel(EmbSum 
     if (lane == 0) ptr[a.R] = run;
   }
   __syncthreads();
-  for (int i = w0; i < w1; i += 64 * P) {
-    int t[P], r[P];
 #pragma unroll
-    for (int j = 0; j < P; ++j) r[j] = item(i + j * 64 + lane, t[j]);
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-      if (!__ballot(r[j] >= 0)) continue;
-      const unsigned long long same = emb_match(r[j], r[j] >= 0, a.rshift);
-      if (r[j] >= 0) {
-        volatile int* p = &cnt[wave * a.R + r[j]];
-        const int at = *p;
-        const int to = at + __popcll(same & ((1ull << lane) - 1));
-        st[to] = t[j];
-        sr[to] = (unsigned short)r[j];
-        if ((same >> lane) == 1) *p = at + __popcll(same);
-      }
-      __builtin_amdgcn_wave_barrier();
+  for (int j = 0; j < P; ++j)
+    if (r[j] >= 0) {
+      const int to = cnt[wave * a.R + r[j]] + rank[j];
+      st[to] = t[j];
+      sr[to] = (unsigned short)r[j];
     }
-  }
   __syncthreads();
   const int total = ptr[a.R];
   const bool whole = spans == 1;
   if (!whole && blockIdx.y == 0)
     for (int r = tid; r < a.R; r += W * 64) a.ptrs[(long)slot * a.R + r] = ptr[r] < ptr[r + 1] ? place[r] : -1;
 
-  const int tw = wave / a.cw, groups = W / a.cw;
-  const int f0 = ((int)blockIdx.y * a.cw + wave % a.cw) * 64 * N + lane * N, f = min(f0, a.F - N);
+  const int tw = wave >> a.cws, gsh = WS - a.cws, groups = 1 << gsh;   // (powers of two: no division)
+  const int f0 = (((int)blockIdx.y << a.cws) + (wave & (a.cw - 1))) * 64 * N + lane * N, f = min(f0, a.F - N);
   const bool on = f0 < a.F;
-  const int p0 = (int)((long)total * tw / groups), p1 = (int)((long)total * (tw + 1) / groups);
+  auto part_at = [&](int g) { return (int)((unsigned)(total * g) >> gsh); };   // (total is at most EM_DIRECT)
+  const int p0 = part_at(tw), p1 = part_at(tw + 1);
   const E* src = (const E*)a.dout + f;
   float* part = a.part + (long)slot * a.slot_rows * a.F;
+  EO* table = (EO*)a.dW + row0 * a.ldw;
+  const long ldd = a.ldd, ldw = a.ldw;
+  const bool accumulate = a.accumulate != 0;
+  const float scale = a.scale;
+  if (whole && !accumulate && on) {                    // rows without tokens; their stores go out before the walk's loads return
+    const float z[N] = {};
+    for (int row = tw; row < rows; row += groups)
+      if (ptr[row] == ptr[row + 1]) emb_store<EO, N>(table + row * ldw, f, f0, z);
+  }
   float acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
   const int before = p0 > 0 ? __builtin_amdgcn_readfirstlane(sr[p0 - 1]) : -1;
-  int cur = -1, next = before + 1;                     // row being summed, first row not written yet
-  bool foreign = false;                                // cur's run began before this part
-  auto fill = [&](int upto) {                          // zeros for the rows without tokens below `upto`
-    if (whole && !a.accumulate && on) {
-      const float z[N] = {};
-      for (; next < upto; ++next) emb_store<EO, N>((EO*)a.dW + (row0 + next) * a.ldw, f, f0, z);
-    }
-  };
+  int cur = -1;                                        // row being summed
+  bool foreign = false;                                // its run began before this part
   auto finish = [&]() {                                // the sum of row cur
     if (cur >= 0) {
       if (foreign) {
 #pragma unroll
         for (int i = 0; i < N; ++i) slot_sum[wave][lane][i] = acc[i];
       } else if (on) {
-        if (whole) emb_write<TO, N>(a, row0 + cur, f, f0, acc);
+        if (whole) emb_write<EO, N>(table + cur * ldw, accumulate, scale, f, f0, acc);
         else emb_store<float, N>(part + (long)place[cur] * a.F, f, f0, acc);
       }
-      next = cur + 1;
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] = 0.f;
     }
   };
   for (int base = p0; base < p1; base += U) {
     V v[U];
-    int r[U];
+    int of[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int at = min(base + j, p1 - 1);
-      const int t = __builtin_amdgcn_readfirstlane(st[at]);
-      r[j] = __builtin_amdgcn_readfirstlane(sr[at]);
-      v[j] = *(const V*)(src + (long)t * a.ldd);
+      const int token = __builtin_amdgcn_readfirstlane(st[at]);
+      of[j] = __builtin_amdgcn_readfirstlane(sr[at]);
+      v[j] = *(const V*)(src + token * ldd);
     }
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       if (base + j < p1) {
-        if (r[j] != cur) {
+        if (of[j] != cur) {
           finish();
-          foreign = cur < 0 && r[j] == before;
-          cur = r[j];
-          fill(cur);
+          foreign = cur < 0 && of[j] == before;
+          cur = of[j];
         }
         if constexpr (N == 1) {
           acc[0] += (float)v[j];
@@ -416,33 +441,26 @@ __global__ __launch_bounds__(EM_WAVES * 64) void gs_embedding_sum_kernel(EmbSum 
   __syncthreads();
   if (open && !foreign) {
     for (int g = tw + 1; g < groups; ++g) {
-      const int q0 = (int)((long)total * g / groups), q1 = (int)((long)total * (g + 1) / groups);
+      const int q0 = part_at(g), q1 = part_at(g + 1);
       if (q0 == q1) continue;
       if (sr[q0] != cur) break;
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += slot_sum[g * a.cw + wave % a.cw][lane][i];
+      for (int i = 0; i < N; ++i) acc[i] += slot_sum[(g << a.cws) + (wave & (a.cw - 1))][lane][i];
       if (sr[q1 - 1] != cur) break;
     }
     finish();
   }
-  if (p1 == total && (p0 < p1 || (total == 0 && tw == 0))) fill(rows);
 }
 
 // Buckets of several spans: the sums of each row in the spans' order, a wave per row.  Blocks (e, ., .) work if e is a bucket's first
 // further span.
 template <int TO, int N>
 __global__ __launch_bounds__(256) void gs_embedding_join_kernel(EmbSum a) {
-  __shared__ int found;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int e = blockIdx.x;
-  if (tid == 0) found = -1;
-  __syncthreads();
-  for (int q = tid; q < a.nb; q += 256)
-    if (a.xs[q] == e && a.xs[q + 1] > e) found = q;
-  __syncthreads();
-  if (found < 0) return;
-  const int b = found, spans = a.xs[b + 1] - e + 1;
-  const long row0 = (long)b << a.rshift;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int e = blockIdx.x, b = a.owner[e];
+  if (b < 0 || a.xs[b] != e) return;
+  const int spans = a.xs[b + 1] - e + 1;
+  const long row0 = (long)b * a.R;
   const int r = blockIdx.z * 4 + wave;
   if (r >= (int)min((long)a.R, a.V - row0)) return;
   const int f0 = blockIdx.y * 64 * N + lane * N, f = min(f0, a.F - N);
@@ -476,7 +494,10 @@ __global__ __launch_bounds__(256) void gs_embedding_join_kernel(EmbSum a) {
       }
     }
   }
-  if (f0 < a.F && (any || !a.accumulate)) emb_write<TO, N>(a, row0 + r, f, f0, acc);
+  if (f0 < a.F && (any || !a.accumulate)) {
+    typedef typename GsElt<TO>::type EO;
+    emb_write<EO, N>((EO*)a.dW + (row0 + r) * a.ldw, a.accumulate != 0, a.scale, f, f0, acc);
+  }
 }
 
 template <int T>
@@ -492,12 +513,13 @@ int emb_fwd(const void* W, long ldw, long V, int F, const int* ids, long n, floa
 
 template <int T, int TO, int N>
 int emb_sum(const EmbPlan& p, EmbSum a, hipStream_t s) {
+  const int waves = p.direct ? EM_WAVES_DIRECT : EM_WAVES;
   a.cw = 1;
-  while (a.cw < EM_WAVES && a.cw * 64 * N < a.F) a.cw *= 2;
+  while (a.cw < waves && a.cw * 64 * N < a.F) { a.cw *= 2; ++a.cws; }
   const unsigned gy = (unsigned)gs_cdiv(a.F, a.cw * 64 * N);
   a.cap = p.direct ? (int)(a.n > 0 ? a.n : 1) : EM_SPAN;
-  const size_t lds = (size_t)a.cap * 6 + (size_t)((EM_WAVES + 1) * p.R + 1) * 4 + (size_t)p.R * 2 + 2;
-  const dim3 block(EM_WAVES * 64);
+  const size_t lds = (size_t)a.cap * 6 + (size_t)((waves + 1) * p.R + 1) * 4 + (size_t)p.R * 2 + 2;
+  const dim3 block(waves * 64);
   if (p.direct) {
     gs_embedding_sum_kernel<T, TO, N, true><<<dim3((unsigned)p.nb, gy), block, lds, s>>>(a);
   } else {
@@ -517,19 +539,21 @@ int emb_bwd(const void* dout, long ldd, const int* ids, long n, long V, int F, f
   EmbSum a = {};
   a.ids = ids; a.dout = dout; a.ldd = ldd; a.dW = dW; a.ldw = ldw; a.n = n; a.V = V; a.F = F; a.scale = scale; a.accumulate = accumulate;
   a.R = p.R; a.nb = p.nb; a.extra = p.extra; a.slot_rows = p.R < EM_SPAN ? p.R : EM_SPAN;
-  while ((1 << a.rshift) < p.R) ++a.rshift;
+  while ((1 << a.rbits) < p.R) ++a.rbits;
+  a.rshift = a.rbits;
   if (!p.direct) {
     int* start = (int*)(scratch + p.start);
     int* xs = (int*)(scratch + p.xs);
+    int* owner = (int*)(scratch + p.owner);
     int2* list = (int2*)(scratch + p.list);
     int* cnt = (int*)(scratch + p.cnt);
     int bits = 0;
     while ((1 << bits) < p.nb) ++bits;
-    gs_embedding_count_kernel<<<dim3((unsigned)p.tiles), dim3(256), 0, s>>>(ids, n, V, a.rshift, p.nbp, cnt);
+    gs_embedding_count_kernel<<<dim3((unsigned)p.tiles), dim3(1024), 0, s>>>(ids, n, V, a.rshift, p.nbp, cnt);
     GS_LAUNCH_CHECK();
-    gs_embedding_place_kernel<<<dim3((unsigned)p.tiles), dim3(256), 0, s>>>(ids, n, V, a.rshift, p.nb, p.nbp, bits, cnt, p.tiles, start, xs, list);
+    gs_embedding_place_kernel<<<dim3((unsigned)p.tiles), dim3(1024), 0, s>>>(ids, n, V, a.rshift, p.nb, p.nbp, bits, cnt, p.tiles, start, xs, owner, p.extra, list);
     GS_LAUNCH_CHECK();
-    a.start = start; a.xs = xs; a.list = list; a.ptrs = (int*)(scratch + p.ptrs); a.part = (float*)(scratch + p.part);
+    a.start = start; a.xs = xs; a.owner = owner; a.list = list; a.ptrs = (int*)(scratch + p.ptrs); a.part = (float*)(scratch + p.part);
   }
   // columns per lane: 16 bytes of dout where the width has them, so that more waves share a frequent row
   constexpr int N = T == GS_TYPE_F32 ? 4 : 8;

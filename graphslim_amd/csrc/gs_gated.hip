@@ -7,6 +7,7 @@
 // (Parts have bf16's smallest step, 2^-133: a value is represented to 2^-134 or to 24 bits, whichever is coarser.)
 // Operands that have to be split, whose rows are not 16-byte aligned, or whose contracted rows are no multiple of 64 elements are laid
 // out in the caller's scratch first, rows padded with zeros to a multiple of 64.
+#include <atomic>
 #include <type_traits>
 
 #include "gs_types.h"
@@ -554,9 +555,10 @@ struct GatedSplit {
   size_t part;        // floats
 };
 
-// Two tiles, 128 x 128 (two workgroups on a compute unit) and 256 x 256 (one): per 64 of k the large one takes 1.75 times as long for
-// four times the products of one of the two small ones side by side.  A product that does not fill the 256 compute units is cut along k; its slices
-// are summed by a second launch, which costs about 4 steps and the traffic of the partial sums.
+// 16-bit operands: 128 x 128 (two workgroups on a compute unit) or 256 x 256 (one), which takes 1.75 times as long a step of 64 for twice
+// the products of the two.  fp32: 128 x 128 or 256 x 128, one workgroup each, 1.4 times as long a step of 32 for twice the products.  A
+// product that does not fill the 256 compute units is cut along k; its slices are summed by a second launch, which costs about 4 steps
+// and the traffic of the partial sums.
 GatedSplit gf_split_of(long M, long N, long K, bool gated, int pl) {
   GatedSplit best = {};
   double least = 1e300;
@@ -564,7 +566,7 @@ GatedSplit gf_split_of(long M, long N, long K, bool gated, int pl) {
   for (int big = 0; big < 2; ++big) {
     const long bm = big ? 256 : 128, bn = big && pl == 1 ? 256 : 128, bk = pl == 3 ? 32 : 64;
     const long tiles = ((M + bm - 1) / bm) * ((cols + bn - 1) / bn), slots = big || pl == 3 ? 256 : 512, steps = K / bk;
-    const double step = big ? 1.75 : 1.0;
+    const double step = big ? (pl == 3 ? 1.4 : 1.75) : 1.0;
     for (long want = 1; want <= 64 && want <= steps; ++want) {
       const long per = (steps + want - 1) / want, slices = (steps + per - 1) / per;
       if (want > 1 && tiles * slices > 2 * slots) break;
@@ -612,7 +614,15 @@ template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool T
 int gf_tile(GatedGemm q, const GatedSplit& sp, float* part, hipStream_t s) {
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16 / (GATED ? 2 : 1), LDS = 2 * PL * (WM * FM + WN * FN) * 16 * BK * 2;
   auto kern = gs_gated_gemm_kernel<T, PL, WM, WN, FM, FN, BK, TA, TB, GATED, ACT>;
-  if (LDS > 65536) GS_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+  if (LDS > 65536) {   // once for each device
+    static std::atomic<unsigned long long> known{0};
+    int dev = 0;
+    GS_HIP(hipGetDevice(&dev));
+    if (dev > 63 || !(known.load(std::memory_order_relaxed) >> dev & 1)) {
+      GS_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+      if (dev <= 63) known.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+  }
   const long gx = (q.M + BM - 1) / BM, gy = (q.N + BN - 1) / BN;
   if (gx * gy > 0x1fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", q.M, q.N);
   q.gx = (int)gx;

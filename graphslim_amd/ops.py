@@ -243,7 +243,7 @@ def _distill_args(logits, top_values, top_ids, tau):
 
 def _grad_out(logits, out):
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[1]
     _device(logits=logits, out=out)
     return out, _matrix("out", out, logits.shape[1], logits.shape[0], logits.dtype)
 
