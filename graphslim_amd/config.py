@@ -129,7 +129,8 @@ _INITS = ["variation_neighborhoods", "variation_edges", "variation_cliques", "he
 @click.option("--seed", "-S", default=1, show_default=True)
 @click.option("--nlayers", default=2, show_default=True)
 @click.option("--verbose", "-V", is_flag=True, show_default=True)
-@click.option("--soft_label", default=0, show_default=True)
+@click.option("--soft_label", default=0, show_default=True, help="with --eval_loss KLD: teacher logits kept a condensed node")
+@click.option("--soft_tau", default=1.0, show_default=True, help="temperature of --soft_label")
 @click.option("--wandb", is_flag=True, show_default=True)
 @click.option("--wandb_project", default="graphslim", show_default=True)
 @click.option("--wandb_run_name", default=None)

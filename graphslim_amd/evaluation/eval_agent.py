@@ -20,8 +20,20 @@ class Evaluator:
     def reset_parameters(self):
         pass
 
-    def test(self, data, model_type, verbose=True, reduced=True, mode="eval", MIA=False):
-        """eval_agent.py:159-232 (no attack / MIA branches: outside the GCond path)."""
+    def teacher(self, data, model_type, verbose=False):
+        """`--eval_loss KLD --soft_label k`: the evaluation model trained on the original graph, and its k top logits of the condensed
+        nodes; None for any other setting (`--soft_label 0`, the default)."""
+        args = self.args
+        k = int(getattr(args, "soft_label", 0) or 0)
+        if getattr(args, "eval_loss", "CE") != "KLD" or k <= 0:
+            return None
+        seed_everything(args.seed)              # the same teacher on every rank
+        model = _MODELS[model_type](data.feat_full.shape[1], args.hidden, data.nclass, evaluation_args(args), mode="eval")
+        model.fit_with_val(data, train_iters=args.eval_epochs, normadj=True, verbose=verbose, setting=args.setting, reduced=False)
+        return model.top_logits(data.feat_syn, data.adj_syn, k, float(getattr(args, "soft_tau", 1.0)))
+
+    def test(self, data, model_type, verbose=True, reduced=True, mode="eval", MIA=False, teacher=None):
+        """eval_agent.py:159-232 (no attack / MIA branches: outside the GCond path).  teacher: see `teacher`."""
         args = self.args
         if model_type not in _MODELS:
             raise NotImplementedError(f"graphslim_amd evaluates with GCN only (got {model_type})")
@@ -29,7 +41,7 @@ class Evaluator:
             print(f"======= testing {model_type}")
         model = _MODELS[model_type](data.feat_full.shape[1], args.hidden, data.nclass, evaluation_args(args), mode=mode)
         best_acc_val = model.fit_with_val(data, train_iters=args.eval_epochs, normadj=True, verbose=verbose,
-                                          setting=args.setting, reduced=reduced)
+                                          setting=args.setting, reduced=reduced, teacher=teacher)
         acc_test = model.test(data, setting=args.setting, verbose=False)
         if verbose:
             print("Test full set results:", f"accuracy= {acc_test:.4f}")
@@ -43,6 +55,7 @@ class Evaluator:
         # multi-GPU (one process per GPU under torch.distributed): the seeded runs are sharded over the ranks
         # (args.eval_parallel = "runs", default) or every run row-shards its full-graph passes (= "rows")
         dist = active_dist()
+        teacher = self.teacher(data, model_type, verbose=args.verbose) if reduced and model_type in _MODELS else None
         by_rows = dist is not None and getattr(args, "eval_parallel", "runs") == "rows"
         if by_rows:
             args.eval_row_shard = RowShard(dist)
@@ -57,7 +70,7 @@ class Evaluator:
         for k in runs:
             i = mine[k]
             seed_everything(args.seed + i)
-            _, acc = self.test(data, model_type=model_type, verbose=args.verbose, reduced=reduced, mode=mode)
+            _, acc = self.test(data, model_type=model_type, verbose=args.verbose, reduced=reduced, mode=mode, teacher=teacher)
             res[i] = acc
             if verbose:
                 runs.set_postfix(test_acc=acc)

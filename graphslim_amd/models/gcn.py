@@ -11,7 +11,7 @@ import numpy as np
 import scipy.sparse as sp
 import torch
 
-from .. import _lib, host
+from .. import _lib, host, ops
 from .._lib import check, ptr, stream
 from ..engine import adam_step, dense_gcn_norm_fwd, gemm, gemm_tn_splitk, spmm_csr
 
@@ -134,6 +134,7 @@ class GCN:
         # row-block sharding of the full-graph passes (parallel.RowShard); a single-GPU run owns every row
         from ..parallel import RowShard
         self.shard = getattr(args, "eval_row_shard", None) or RowShard()
+        self._teacher = None                    # (values, ids, row weights, tau) while training on a teacher's top logits
         self.initialize()
 
     # -- parameters -----------------------------------------------------------------------------------
@@ -207,8 +208,7 @@ class GCN:
             Hin, win = H, wout
         Z = Hs[-1]
         G = torch.empty(n, Cn, device=dev)
-        lossr = torch.empty(n, device=dev)
-        check(L.gs_softmax_nll_grad_f32(ptr(Z), Cn, ptr(labels_i32), n, Cn, ptr(G), ptr(lossr), stream()))
+        lossr = self._loss_grad(Z, labels_i32, G)
         g = torch.empty_like(self.P)
         gs = self._views(g)
         dZ = G                                                           # d loss / d pre-activation of layer l (masked below l = K)
@@ -243,8 +243,7 @@ class GCN:
         spmm_csr(*csr, T2, F=ldc, out=Z)
         check(L.gs_bias_act_f32(ptr(Z), ldc, ptr(ps[-1]), nt, Cn, 0, stream()))
         Gz = torch.empty(nt, Cn, device=dev)
-        lossr = torch.empty(nt, device=dev)
-        check(L.gs_softmax_nll_grad_f32(ptr(Z), ldc, ptr(labels_i32), nt, Cn, ptr(Gz), ptr(lossr), stream()))
+        lossr = self._loss_grad(Z, labels_i32, Gz)
         g = torch.empty_like(self.P)
         gs = self._views(g)
         ones = self._ones(max(N, nt))
@@ -313,8 +312,7 @@ class GCN:
         Z = torch.empty(n, Cn, device=dev)
         gemm(A, T2, Z, n, Cn, n, (n, 1), (Cn, 1), Cn, bias=b2)
         G = torch.empty(n, Cn, device=dev)
-        lossr = torch.empty(n, device=dev)
-        check(L.gs_softmax_nll_grad_f32(ptr(Z), Cn, ptr(labels_i32), n, Cn, ptr(G), ptr(lossr), stream()))
+        lossr = self._loss_grad(Z, labels_i32, G)
         g = torch.empty_like(self.P)
         gW1, gb1, gW2, gb2 = self._views(g)
         check(L.gs_colsum_f32(ptr(G), Cn, n, Cn, ptr(gb2), stream()))
@@ -348,8 +346,7 @@ class GCN:
         spmm_csr(*csr, T2, F=ldc, out=Z)
         check(L.gs_bias_act_f32(ptr(Z), ldc, ptr(b2), nt, Cn, 0, stream()))
         Gz = torch.empty(nt, Cn, device=dev)
-        lossr = torch.empty(nt, device=dev)
-        check(L.gs_softmax_nll_grad_f32(ptr(Z), ldc, ptr(labels_i32), nt, Cn, ptr(Gz), ptr(lossr), stream()))
+        lossr = self._loss_grad(Z, labels_i32, Gz)
         g = torch.empty_like(self.P)
         gW1, gb1, gW2, gb2 = self._views(g)
         ones = self._ones(max(N, nt))
@@ -362,6 +359,17 @@ class GCN:
         gemm_tn_splitk(G.S, G.S.stride(0), dH, h, gW1, d, h, N)              # S^T dH
         opt["step"] += 1
         adam_step(self.P, g, opt["m"], opt["v"], opt["lr"], opt["step"], weight_decay=self.weight_decay)
+        return lossr
+
+    def _loss_grad(self, Z, labels_i32, G):
+        """Gradient of the mean loss over the rows of Z [n, >= C] into G [n, C], and the loss of each row: negative log-likelihood of
+        the labels (models/base.py:156-161), or, while training on a teacher, tau^2 KL of its top logits (`teacher` of fit_with_val)."""
+        n, Cn = G.shape
+        if self._teacher is not None:
+            values, ids, weight, tau = self._teacher
+            return ops.distill_loss_grad(Z[:, :Cn], values, ids, weight, tau, out=G)[0]
+        lossr = torch.empty(n, device=self.device)
+        check(_lib.lib().gs_softmax_nll_grad_f32(ptr(Z), Z.stride(0), ptr(labels_i32), n, Cn, ptr(G), ptr(lossr), stream()))
         return lossr
 
     def _ones(self, n):
@@ -404,9 +412,11 @@ class GCN:
         return idx, labels.to(self.device).to(torch.int32), n_total
 
     def fit_with_val(self, data, train_iters=600, verbose=False, normadj=True, setting="trans", reduced=False,
-                     final_output=False, best_val=None, **kwargs):
+                     final_output=False, best_val=None, teacher=None, **kwargs):
         """models/base.py:80-187 for the reduced-graph case: train on (adj_syn, feat_syn, labels_syn), validate on the
-        full graph (trans) / validation graph (ind) every epoch, keep the best-validation weights."""
+        full graph (trans) / validation graph (ind) every epoch, keep the best-validation weights.  teacher: (top logits [n, k],
+        their classes [n, k] int32, temperature) of the n rows the loss is taken on, as `top_logits` gives them — the loss is then
+        tau^2 KL(teacher || student) instead of the labels' likelihood."""
         dev = self.device
         self.initialize()
         if reduced:
@@ -434,6 +444,16 @@ class GCN:
         else:
             G = self._graph_for(data, "full")
             idx_val, labels_val, n_val = self._targets(G, data.idx_val, data.labels_val)
+        if teacher is not None:
+            values, ids, tau = teacher
+            values = torch.as_tensor(values).to(dev, torch.float32).contiguous()
+            ids = torch.as_tensor(ids).to(dev, torch.int32).contiguous()
+            if values.shape != ids.shape or values.dim() != 2 or values.shape[0] != labels.numel():
+                raise ValueError(f"graphslim_amd.GCN.fit_with_val: the teacher's top logits are {tuple(values.shape)}, their classes "
+                                 f"{tuple(ids.shape)}, for {labels.numel()} training rows")
+            self._teacher = (values, ids, torch.full((labels.numel(),), 1.0 / labels.numel(), device=dev), float(tau))
+        else:
+            self._teacher = None
         best_acc = 0 if best_val is None else best_val
         weights = None
         opt = self._new_opt(self.lr)
@@ -451,6 +471,7 @@ class GCN:
             if acc_val > best_acc:
                 best_acc = acc_val
                 weights = self.state_dict()
+        self._teacher = None
         if final_output:
             return
         if weights is not None:
@@ -470,6 +491,19 @@ class GCN:
         if verbose:
             print("Test set results:", "accuracy= {:.4f}".format(acc))
         return acc
+
+    @torch.no_grad()
+    def top_logits(self, feat, adj, k, tau=1.0):
+        """What `fit_with_val(teacher=...)` takes, of this model as the teacher: its k largest log-probabilities a node of a graph
+        (dense [n, n], or a batch of structures over the same nodes [B, n, n] as one block-diagonal graph; or scipy sparse), their
+        classes, the temperature.  The selection is host-side index arithmetic on [n, C], like the coreset rules'."""
+        if not sp.issparse(adj):
+            adj = torch.as_tensor(adj).detach().cpu()
+            feat = torch.as_tensor(feat).repeat(adj.shape[0] if adj.dim() == 3 else 1, 1)
+            adj = sp.csr_matrix(np.asarray(torch.block_diag(*adj) if adj.dim() == 3 else adj))
+        out = self.predict(torch.as_tensor(feat).detach(), adj).cpu()
+        values, ids = torch.topk(out, min(int(k), self.nclass), dim=1)
+        return values, ids.to(torch.int32), tau
 
     @torch.no_grad()
     def predict(self, features=None, adj=None, normadj=True, output_layer_features=False):
