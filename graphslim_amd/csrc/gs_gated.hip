@@ -5,8 +5,8 @@
 // latter are transposed on their way from LDS to the registers.  16-bit operands enter as they are; an fp32 operand is the exact sum of three bf16 parts
 // (x = h + m + l, 8 + 8 + 8 significant bits), and six products of parts make one product: what they leave out is below 2^-23 of it.
 // (Parts have bf16's smallest step, 2^-133: a value is represented to 2^-134 or to 24 bits, whichever is coarser.)
-// Operands that have to be split, whose rows are not 16-byte aligned, or whose contracted rows are no multiple of 64 elements are laid
-// out in the caller's scratch first, rows padded with zeros to a multiple of 64.
+// The parts of fp32 operands, and [dg | du], are laid out in the caller's scratch first, rows padded with zeros to a multiple of 64;
+// 16-bit operands are read where they are, whatever their alignment and width.
 #include <atomic>
 #include <type_traits>
 
@@ -104,19 +104,19 @@ __device__ __forceinline__ void gf_put8(const float* v, P* __restrict__ o, long 
 }
 
 // ---- operand layout -------------------------------------------------------------------------------------------------------------
-// Up to three matrices [R][C] as [PL][Rp][Cp], zeros behind the columns and rows
+// Three matrices [R][C] as [PL][Rp][Cp], zeros behind the columns and rows
 struct GatedPack {
   const void* in[3];
   void* out[3];
   long ld[3], R[3], Rp[3], first[3];   // first: the matrix's first block
-  long C, Cp, n;
+  long C, Cp;
 };
 
 template <int T, int PL>
 __global__ __launch_bounds__(256) void gs_gated_pack_kernel(GatedPack a) {
   typedef typename GsElt<T>::type E;
   typedef typename GfPlane<T, PL>::type P;
-  const int w = a.n > 2 && (long)blockIdx.x >= a.first[2] ? 2 : (a.n > 1 && (long)blockIdx.x >= a.first[1] ? 1 : 0);
+  const int w = (long)blockIdx.x >= a.first[2] ? 2 : ((long)blockIdx.x >= a.first[1] ? 1 : 0);
   const long per = a.Cp / 8;
   const long i = ((long)blockIdx.x - a.first[w]) * 256 + threadIdx.x;
   const long r = i / per, c = (i - r * per) * 8;
@@ -247,6 +247,7 @@ struct GatedGemm {
   const void* B[2];     // gated: gate and up projection; n contiguous: rows of k below `kb` in the first, the others in the second
   long ldb, plane_b;
   long M, N, K;         // K a multiple of 64
+  long k_end;           // RAW: elements that a row of k has (A's and B's)
   long bcols;           // n contiguous: columns that rows of B have (a multiple of 8, N or more)
   long kb, brows;       // n contiguous: rows that B[0] stands for (a multiple of 64), and rows that each of B has; behind them A is 0
   void* C[2];           // plain form: rows [0, rows) go to C[0], rows [rows1, rows1 + rows) to C[1], others nowhere
@@ -336,9 +337,10 @@ __device__ __forceinline__ void gf_tr_read4(unsigned addr, int first, Frag* x) {
 }
 
 // T: type of the outputs (and of 16-bit operands), PL: parts, WM x WN waves of (16 FM) x (16 FN) results.  TA, TB: the operand's other
-// index is contiguous, not k.  GATED: rows of B alternate between gate and up every 16, so that a lane holds both sums of its outputs
+// index is contiguous, not k.  RAW: x and the weights are read where they are though their rows begin at any element or end inside a
+// step of k: through registers, with zeros behind a row's end.  GATED: rows of B alternate between gate and up every 16, so that a lane holds both sums of its outputs
 // and the activation is applied in registers.
-template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool GATED, int ACT>
+template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED, int ACT>
 __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q) {
   typedef typename GfPlane<T, PL>::type P;
   typedef typename GfFrag<P>::type Frag;
@@ -361,21 +363,48 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
   const P* A = (const P*)q.A;
 
   const P* srcA[ITA];
+  int colA[ITA];
+  long colB[ITB];       // of a chunk in its row: of k, or of n
   long srcB[ITB], endB[ITB];   // offsets from B's base; from that of the step with B's last rows, where they are fewer than BK
 #pragma unroll
   for (int i = 0; i < ITA; ++i) {
     const int s = i * NT + tid, r = s / CA, c = (s % CA) ^ gf_swz<TA, BK>(r);
-    srcA[i] = TA ? A + r * q.lda + min(m0 + c * 8, q.M - 8) : A + min(m0 + r, q.M - 1) * q.lda + c * 8;
+    colA[i] = c * 8;
+    srcA[i] = TA ? A + r * q.lda + min(m0 + c * 8, q.M - 8) : A + min(m0 + r, q.M - 1) * q.lda + (RAW && !TB ? 0 : c * 8);
   }
 #pragma unroll
   for (int i = 0; i < ITB; ++i) {
     const int s = i * NT + tid, r = s / CB, c = (s % CB) ^ gf_swz<TB, BK>(r);
     const long n = GATED ? n0 + (r >> 5) * 16 + (r & 15) : n0 + r;
     const P* base = (const P*)q.B[GATED ? (r >> 4) & 1 : 0];
-    const long col = min(n0 + c * 8, q.bcols - 8);
-    srcB[i] = TB ? r * q.ldb + col : (long)(base + min(n, q.N - 1) * q.ldb + c * 8 - (const P*)q.B[0]);
-    endB[i] = TB ? min((long)r, (q.brows - 1) % BK) * q.ldb + col : 0;
+    // (RAW: offsets of rows, the column comes when they are read)
+    const long col = RAW ? n0 + c * 8 : min(n0 + c * 8, q.bcols - 8), in_row = RAW ? 0 : (TB ? col : c * 8);
+    colB[i] = TB ? col : c * 8;
+    srcB[i] = (TB ? r * q.ldb : (long)(base + min(n, q.N - 1) * q.ldb - (const P*)q.B[0])) + in_row;
+    endB[i] = TB ? min((long)r, (q.brows - 1) % BK) * q.ldb + in_row : 0;
   }
+  // RAW: the chunks of the next tile on their way through registers.  A chunk that reaches behind its row's end is loaded from the
+  // row's last 8 elements and shifted down when it goes to LDS, zeros behind (rows of fewer than 8 elements are taken one by one).
+  typedef typename GsVec<P, 8>::type Chunk;
+  constexpr bool RAW_A = RAW && !TA && !TB;                        // (behind TB, A is the laid-out [dg | du])
+  Chunk ra[RAW_A ? ITA : 1], rb[RAW ? ITB : 1];
+  const long row_end = TB ? q.bcols : q.k_end;                     // of a row that is read raw
+  const bool narrow = row_end < 8;
+  long k_raw = 0;                                                  // the step that is on its way
+  auto raw_load = [&](const P* row, long at) {
+    if (!narrow) return *(const Chunk*)(row + min(at, row_end - 8));
+    Chunk v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = at + e < row_end ? row[at + e] : (P)0.f;
+    return v;
+  };
+  auto raw_shift = [&](Chunk v, long at) {
+    if (narrow || at <= row_end - 8) return v;
+    const int by = (int)(at - (row_end - 8));
+    unsigned __int128 x = __builtin_bit_cast(unsigned __int128, v);
+    x = by >= 8 ? (unsigned __int128)0 : x >> (16 * by);
+    return __builtin_bit_cast(Chunk, x);
+  };
   auto stage = [&](int buf, long k0) {
     P* base = lds + buf * STAGE;
     const P* b0 = (const P*)q.B[0] + k0;
@@ -386,6 +415,14 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
       b0 = (const P*)q.B[k0 < q.kb ? 0 : 1] + kk * q.ldb;
       end = kk + BK > q.brows;
     }
+    k_raw = k0;
+    if constexpr (RAW_A) {
+#pragma unroll
+      for (int i = 0; i < ITA; ++i) ra[i] = raw_load(srcA[i], k0 + colA[i]);
+#pragma unroll
+      for (int i = 0; i < ITB; ++i) rb[i] = raw_load((const P*)q.B[0] + srcB[i], k0 + colB[i]);
+      return;
+    }
 #pragma unroll
     for (int p = 0; p < PL; ++p) {
 #pragma unroll
@@ -395,8 +432,24 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
 #pragma unroll
       for (int i = 0; i < ITB; ++i) {
         const long off = TB && end ? endB[i] : srcB[i];
-        __builtin_amdgcn_global_load_lds((gbl_ptr)(b0 + p * q.plane_b + off), (lds_ptr)(base + PL * TILE_A + p * TILE_B + (i * NT + wave * 64) * 8), 16, 0, 0);
+        if constexpr (RAW) rb[i] = raw_load(b0 + off, colB[i]);
+        else
+          __builtin_amdgcn_global_load_lds((gbl_ptr)(b0 + p * q.plane_b + off), (lds_ptr)(base + PL * TILE_A + p * TILE_B + (i * NT + wave * 64) * 8), 16, 0, 0);
       }
+    }
+  };
+  auto land = [&](int buf) {
+    typedef P Whole __attribute__((ext_vector_type(8)));
+    P* base = lds + buf * STAGE;
+    if constexpr (RAW) {
+      const bool ends = TB ? n0 + BN > row_end : k_raw + BK > row_end;   // (the whole workgroup's)
+      if constexpr (RAW_A) {
+#pragma unroll
+        for (int i = 0; i < ITA; ++i) *(Whole*)(base + (i * NT + tid) * 8) = ends ? raw_shift(ra[i], k_raw + colA[i]) : ra[i];
+      }
+#pragma unroll
+      for (int i = 0; i < ITB; ++i)
+        *(Whole*)(base + TILE_A + (i * NT + tid) * 8) = ends ? raw_shift(rb[i], TB ? colB[i] : k_raw + colB[i]) : rb[i];
     }
   };
 
@@ -409,6 +462,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
   const unsigned tra = TA ? gf_tr_addr<BM, BK>(lds, wm * FM * 16, lane) : 0u;
   const unsigned trb = TB ? gf_tr_addr<BN, BK>(lds + PL * TILE_A, wn * FN * 16, lane) : 0u;
   stage(0, k_begin);
+  land(0);
   int buf = 0;
   for (long k0 = k_begin; k0 < k_end; k0 += BK, buf ^= 1) {
     __syncthreads();   // this step's tile has landed; the other buffer has been read by all
@@ -456,6 +510,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
           }
       });
     });
+    if (k0 + BK < k_end) land(buf ^ 1);
   }
 
   // B is the first operand, so a lane holds four consecutive n of one m
@@ -585,7 +640,7 @@ GatedSplit gf_split_of(long M, long N, long K, bool gated, int pl) {
 struct GatedPlan {
   int pl;
   long Dp, Fp, Mp;
-  size_t x, wg, wu, fwd;              // x, Wg, Wu with padded rows (both passes)
+  size_t x, wg, wu, fwd;              // fp32: the parts of x, Wg, Wu with padded rows (both passes)
   size_t dgu, bwd;                    // backward: [dg | du]
   size_t part_fwd, part_bwd;          // partial sums of products that are cut along k, behind the operands
 };
@@ -598,9 +653,11 @@ GatedPlan gf_plan(long M, long D, long F, int type) {
   p.Mp = gf_up(M);
   size_t o = 0;
   auto take = [&](size_t n) { size_t at = o; o += n * p.pl; return at; };
-  p.x = take((size_t)p.Mp * p.Dp);
-  p.wg = take((size_t)p.Fp * p.Dp);
-  p.wu = take((size_t)p.Fp * p.Dp);
+  if (p.pl > 1) {
+    p.x = take((size_t)p.Mp * p.Dp);
+    p.wg = take((size_t)p.Fp * p.Dp);
+    p.wu = take((size_t)p.Fp * p.Dp);
+  }
   p.part_fwd = o;
   p.fwd = o + 2 * gf_split_of(M, F, p.Dp, true, p.pl).part;
   p.dgu = take((size_t)p.Mp * 2 * p.Fp);
@@ -610,10 +667,10 @@ GatedPlan gf_plan(long M, long D, long F, int type) {
   return p;
 }
 
-template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool GATED, int ACT>
+template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED, int ACT>
 int gf_tile(GatedGemm q, const GatedSplit& sp, float* part, hipStream_t s) {
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16 / (GATED ? 2 : 1), LDS = 2 * PL * (WM * FM + WN * FN) * 16 * BK * 2;
-  auto kern = gs_gated_gemm_kernel<T, PL, WM, WN, FM, FN, BK, TA, TB, GATED, ACT>;
+  auto kern = gs_gated_gemm_kernel<T, PL, WM, WN, FM, FN, BK, TA, TB, RAW, GATED, ACT>;
   if (LDS > 65536) {   // once for each device
     static std::atomic<unsigned long long> known{0};
     int dev = 0;
@@ -642,14 +699,17 @@ int gf_tile(GatedGemm q, const GatedSplit& sp, float* part, hipStream_t s) {
 }
 
 template <int T, int PL, bool TA, bool TB, bool GATED, int ACT>
-int gf_gemm(const GatedGemm& q, float* part, hipStream_t s) {
+int gf_gemm(const GatedGemm& q, bool raw, float* part, hipStream_t s) {
   const GatedSplit sp = gf_split_of(q.M, q.N, q.K, GATED, PL);
   if constexpr (PL == 3) {
-    if (sp.big) return gf_tile<T, PL, 4, 2, 4, 4, 32, TA, TB, GATED, ACT>(q, sp, part, s);
-    return gf_tile<T, PL, 2, 2, 4, 4, 32, TA, TB, GATED, ACT>(q, sp, part, s);
+    if (sp.big) return gf_tile<T, PL, 4, 2, 4, 4, 32, TA, TB, false, GATED, ACT>(q, sp, part, s);
+    return gf_tile<T, PL, 2, 2, 4, 4, 32, TA, TB, false, GATED, ACT>(q, sp, part, s);
+  } else if (raw) {
+    if (sp.big) return gf_tile<T, PL, 2, 4, 8, 4, 64, TA, TB, true, GATED, ACT>(q, sp, part, s);
+    return gf_tile<T, PL, 2, 2, 4, 4, 64, TA, TB, true, GATED, ACT>(q, sp, part, s);
   } else {
-    if (sp.big) return gf_tile<T, PL, 2, 4, 8, 4, 64, TA, TB, GATED, ACT>(q, sp, part, s);
-    return gf_tile<T, PL, 2, 2, 4, 4, 64, TA, TB, GATED, ACT>(q, sp, part, s);
+    if (sp.big) return gf_tile<T, PL, 2, 4, 8, 4, 64, TA, TB, false, GATED, ACT>(q, sp, part, s);
+    return gf_tile<T, PL, 2, 2, 4, 4, 64, TA, TB, false, GATED, ACT>(q, sp, part, s);
   }
 }
 
@@ -667,38 +727,24 @@ struct GatedCall {
   char* scratch;
 };
 
-// x, Wg and Wu as operands: as they are, or laid out in the scratch
+// x, Wg and Wu as operands: as they are, or split and laid out in the scratch
 struct GatedOperands {
   const void *x, *w[2];
   long ldx, ldw, plane_x, plane_w;
 };
 
 template <int T, int PL>
-int gf_operands(const GatedCall& c, const GatedPlan& p, int step, GatedOperands* o, hipStream_t s) {
+int gf_operands(const GatedCall& c, const GatedPlan& p, GatedOperands* o, hipStream_t s) {
   typedef typename GfPlane<T, PL>::type P;
-  P* sc = (P*)c.scratch;
   *o = {c.x, {c.wg, c.wu}, c.ldx, c.ldw, 0, 0};
-  GatedPack a = {};
-  a.C = c.D;
-  a.Cp = p.Dp;
-  long blocks = 0;
-  auto add = [&](const void* in, long ld, long R, long Rp, P* out) {
-    a.in[a.n] = in; a.out[a.n] = out; a.ld[a.n] = ld; a.R[a.n] = R; a.Rp[a.n] = Rp; a.first[a.n] = blocks;
-    ++a.n;
-    blocks += (Rp * (p.Dp / 8) + 255) / 256;
-  };
-  if (PL > 1 || !gf_plain(c.x, c.ldx, c.D, step)) {
-    o->x = sc + p.x; o->ldx = p.Dp; o->plane_x = p.Mp * p.Dp;
-    add(c.x, c.ldx, c.M, p.Mp, sc + p.x);
-  }
-  if (PL > 1 || !gf_plain(c.wg, c.ldw, c.D, step) || !gf_plain(c.wu, c.ldw, c.D, step)) {
-    o->w[0] = sc + p.wg; o->w[1] = sc + p.wu; o->ldw = p.Dp; o->plane_w = p.Fp * p.Dp;
-    add(c.wg, c.ldw, c.F, p.Fp, sc + p.wg);
-    add(c.wu, c.ldw, c.F, p.Fp, sc + p.wu);
-  }
-  if (blocks > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: operands of width %ld are beyond one launch", c.D);
-  if (blocks) {
-    gs_gated_pack_kernel<T, PL><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(a);
+  if constexpr (PL > 1) {
+    P* sc = (P*)c.scratch;
+    *o = {sc + p.x, {sc + p.wg, sc + p.wu}, p.Dp, p.Dp, p.Mp * p.Dp, p.Fp * p.Dp};
+    const long bx = (p.Mp * (p.Dp / 8) + 255) / 256, bw = (p.Fp * (p.Dp / 8) + 255) / 256;
+    if (bx + 2 * bw > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: operands of width %ld are beyond one launch", c.D);
+    const GatedPack a = {{c.x, c.wg, c.wu}, {sc + p.x, sc + p.wg, sc + p.wu}, {c.ldx, c.ldw, c.ldw}, {c.M, c.F, c.F}, {p.Mp, p.Fp, p.Fp},
+                         {0, bx, bx + bw}, c.D, p.Dp};
+    gs_gated_pack_kernel<T, PL><<<dim3((unsigned)(bx + 2 * bw)), dim3(256), 0, s>>>(a);
     GS_LAUNCH_CHECK();
   }
   return GS_OK;
@@ -727,14 +773,16 @@ int gf_fwd(const GatedCall& c, hipStream_t s) {
   }
   const GatedPlan p = gf_plan(c.M, c.D, c.F, T);
   GatedOperands o;
-  GS_TRY((gf_operands<T, PL>(c, p, GF_PAD, &o, s)));
+  GS_TRY((gf_operands<T, PL>(c, p, &o, s)));
+  const bool raw = PL == 1 && !(gf_plain(c.x, c.ldx, c.D, GF_PAD) && gf_plain(c.wg, c.ldw, c.D, GF_PAD) && gf_plain(c.wu, c.ldw, c.D, GF_PAD));
   GatedGemm q = {};
   q.A = o.x; q.lda = o.ldx; q.plane_a = o.plane_x;
   q.B[0] = o.w[0]; q.B[1] = o.w[1]; q.ldb = o.ldw; q.plane_b = o.plane_w;
   q.M = c.M; q.N = c.F; q.K = p.Dp;
   q.C[0] = c.h; q.ldc = c.ldh;
   q.saved = c.saved;
-  return gf_gemm<T, PL, false, false, true, ACT>(q, (float*)((P*)c.scratch + p.part_fwd), s);
+  q.k_end = c.D;
+  return gf_gemm<T, PL, false, false, true, ACT>(q, raw, (float*)((P*)c.scratch + p.part_fwd), s);
 }
 
 template <int T, int PL, int ACT>
@@ -746,7 +794,7 @@ int gf_bwd(const GatedCall& c, hipStream_t s) {
   const long plane = p.Mp * 2 * p.Fp, blocks = (p.Mp * (p.Fp / 8) + 255) / 256;
   if (blocks > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated_bwd: %ld x %ld is beyond one launch", c.M, c.F);
   GatedOperands o;
-  GS_TRY((gf_operands<T, PL>(c, p, 8, &o, s)));
+  GS_TRY((gf_operands<T, PL>(c, p, &o, s)));
   gs_gated_slopes_kernel<T, PL, ACT><<<dim3((unsigned)blocks), dim3(256), 0, s>>>((const E*)c.dh, c.lddh, c.saved, c.M, c.F, dgu, p.Mp, p.Fp, plane);
   GS_LAUNCH_CHECK();
   // dx: k runs over the columns of dg, then of du, and over the rows of Wg, then of Wu
@@ -757,13 +805,14 @@ int gf_bwd(const GatedCall& c, hipStream_t s) {
   q.N = c.D; q.bcols = o.plane_w ? p.Dp : c.D;
   q.C[0] = c.dx; q.ldc = c.lddx; q.rows = q.rows1 = c.M;
   float* part = (float*)((P*)c.scratch + p.part_bwd);
-  GS_TRY((gf_gemm<T, PL, false, true, false, GS_ACT_SILU>(q, part, s)));
+  const bool raw_w = PL == 1 && !(gf_plain(c.wg, c.ldw, c.D, 8) && gf_plain(c.wu, c.ldw, c.D, 8)), raw_x = PL == 1 && !gf_plain(c.x, c.ldx, c.D, 8);
+  GS_TRY((gf_gemm<T, PL, false, true, false, GS_ACT_SILU>(q, raw_w, part, s)));
   // dWg, dWu: k runs over the tokens
   q.B[0] = o.x; q.ldb = o.ldx; q.plane_b = o.plane_x;
   q.M = 2 * p.Fp; q.K = p.Mp; q.kb = p.Mp; q.brows = o.plane_x ? p.Mp : c.M;
   q.bcols = o.plane_x ? p.Dp : c.D;
   q.C[0] = c.dwg; q.C[1] = c.dwu; q.ldc = c.lddw; q.rows = c.F; q.rows1 = p.Fp;
-  return gf_gemm<T, PL, true, true, false, GS_ACT_SILU>(q, part, s);
+  return gf_gemm<T, PL, true, true, false, GS_ACT_SILU>(q, raw_x, part, s);
 }
 
 // dW = 0 where there are no tokens
@@ -829,7 +878,8 @@ extern "C" int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const v
   GS_TRY(gf_check("gs_gated_fwd", c, type));
   if (ldh < F) GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: a row stride is below the width %ld", F);
   if (M == 0) return GS_OK;
-  if (!x || !w_gate || !w_up || !h || (!scratch && !gf_few(M, type))) GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: null pointer");
+  if (!x || !w_gate || !w_up || !h || (!scratch && gs_gated_fwd_scratch_bytes(M, D, F, type) > 0))
+    GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: null pointer");
   if ((size_t)scratch & 15) GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: the scratch is not 16-byte aligned");
   return gf_run(c, type, false, (hipStream_t)stream);
 }
