@@ -39,12 +39,11 @@ __global__ __launch_bounds__(256) void gs_embedding_fwd_kernel(const typename Gs
 //   many:        gs_embedding_count / _place sort the tokens by bucket first; a bucket of more than EM_SPAN tokens (a frequent id) is
 //                cut into spans with a workgroup each, whose sums gs_embedding_join adds in the spans' order.
 constexpr int EM_TILE = 4096;      // ids per workgroup of the sort: four a thread, all loaded at once
-constexpr int EM_WAVES = 8;        // waves of a workgroup that sums a span
-constexpr int EM_WAVES_DIRECT = 16;
 constexpr int EM_SPAN = 256;       // tokens of a bucket per workgroup
 constexpr int EM_MAX_BUCKETS = 2048;
 constexpr int EM_MAX_R = 1024;     // rows of a bucket at most
 constexpr long EM_MAX_V = (long)EM_MAX_R * EM_MAX_BUCKETS;
+constexpr long EM_FEW = 512;       // ids up to which many small workgroups do it: writing the empty rows is all the work
 constexpr long EM_DIRECT = 8192;   // tokens up to which one launch does it all
 
 struct EmbPlan {
@@ -57,8 +56,8 @@ struct EmbPlan {
 EmbPlan emb_plan(long n, long V, int F) {
   EmbPlan p;
   p.direct = n <= EM_DIRECT;
-  if (p.direct) {        // one bucket for each compute unit, of up to 64 rows
-    p.R = (int)std::min(std::max(gs_cdiv(V, 256), 4), 64);
+  if (p.direct) {        // a bucket for each compute unit (few ids: four), of up to 64 rows
+    p.R = (int)std::min(std::max(gs_cdiv(V, n <= EM_FEW ? 1024 : 256), 4), 64);
   } else {
     p.R = 4;
     while ((V + p.R - 1) / p.R > 1024 && p.R < 64) p.R *= 2;
@@ -259,17 +258,16 @@ __device__ __forceinline__ void emb_write(EO* __restrict__ o, bool accumulate, f
   emb_store<EO, N>(o, f, f0, acc);
 }
 
-// One workgroup of EM_WAVES waves per span of a bucket's tokens and 64 N cw columns: cw waves side by side on the columns, EM_WAVES / cw
+// One workgroup of W waves per span of a bucket's tokens (at most 64 W P) and 64 N cw columns: cw waves side by side on the columns, W / cw
 // groups of them on consecutive parts of the sorted tokens, so that a frequent row is walked by several waves.  A run that crosses
 // from one part into the next is summed by the wave that it begins in, from what the others leave in LDS, in order.
-// Blocks [0, extra) are the further spans, the longest work, and begin first.
-template <int T, int TO, int N, bool DIRECT>
-__global__ __launch_bounds__((DIRECT ? EM_WAVES_DIRECT : EM_WAVES) * 64) void gs_embedding_sum_kernel(EmbSum a) {
+// U rows of dout are in flight per lane.  Blocks [0, extra) are the further spans, the longest work, and begin first.
+template <int T, int TO, int N, bool DIRECT, int W, int P, int U>
+__global__ __launch_bounds__(W * 64) void gs_embedding_sum_kernel(EmbSum a) {
   typedef typename GsElt<T>::type E;
   typedef typename GsElt<TO>::type EO;
   typedef typename GsVec<E, N>::type V;
-  constexpr int U = DIRECT ? 16 : 8;                   // rows of dout in flight per lane
-  constexpr int W = DIRECT ? EM_WAVES_DIRECT : EM_WAVES, WS = DIRECT ? 4 : 3;
+  constexpr int WS = W == 16 ? 4 : 3;
   static_assert(1 << WS == W, "a power of two");
   extern __shared__ int dyn[];
   int* ptr = dyn;                                      // [R + 1] where a row's tokens begin
@@ -299,8 +297,6 @@ __global__ __launch_bounds__((DIRECT ? EM_WAVES_DIRECT : EM_WAVES) * 64) void gs
   const long row0 = (long)b * a.R;
   const int rows = (int)min((long)a.R, a.V - row0);
   // stable counting sort of items [i0, i1) by row: each wave takes 64 P of them, in order
-  constexpr int P = DIRECT ? (int)(EM_DIRECT / (W * 64)) : 1;
-  static_assert(W * 64 * P >= (DIRECT ? EM_DIRECT : EM_SPAN), "one go");
   int t[P], r[P];                                      // tokens, their rows in the bucket or -1
 #pragma unroll
   for (int j = 0; j < P; ++j) {
@@ -511,24 +507,27 @@ int emb_fwd(const void* W, long ldw, long V, int F, const int* ids, long n, floa
   return GS_OK;
 }
 
+template <int T, int TO, int N, bool DIRECT, int W, int P, int U>
+int emb_sum_launch(const EmbPlan& p, EmbSum a, hipStream_t s) {
+  a.cw = 1;
+  while (a.cw < W && a.cw * 64 * N < a.F) { a.cw *= 2; ++a.cws; }
+  const unsigned gy = (unsigned)gs_cdiv(a.F, a.cw * 64 * N);
+  a.cap = (int)std::min<long>(DIRECT ? std::max<long>(a.n, 1) : EM_SPAN, W * 64 * P);
+  const size_t lds = (size_t)a.cap * 6 + (size_t)((W + 1) * p.R + 1) * 4 + (size_t)p.R * 2 + 2;
+  gs_embedding_sum_kernel<T, TO, N, DIRECT, W, P, U><<<dim3((unsigned)((DIRECT ? 0 : p.extra) + p.nb), gy), dim3(W * 64), lds, s>>>(a);
+  GS_LAUNCH_CHECK();
+  return GS_OK;
+}
+
 template <int T, int TO, int N>
 int emb_sum(const EmbPlan& p, EmbSum a, hipStream_t s) {
-  const int waves = p.direct ? EM_WAVES_DIRECT : EM_WAVES;
-  a.cw = 1;
-  while (a.cw < waves && a.cw * 64 * N < a.F) { a.cw *= 2; ++a.cws; }
-  const unsigned gy = (unsigned)gs_cdiv(a.F, a.cw * 64 * N);
-  a.cap = p.direct ? (int)(a.n > 0 ? a.n : 1) : EM_SPAN;
-  const size_t lds = (size_t)a.cap * 6 + (size_t)((waves + 1) * p.R + 1) * 4 + (size_t)p.R * 2 + 2;
-  const dim3 block(waves * 64);
-  if (p.direct) {
-    gs_embedding_sum_kernel<T, TO, N, true><<<dim3((unsigned)p.nb, gy), block, lds, s>>>(a);
-  } else {
-    gs_embedding_sum_kernel<T, TO, N, false><<<dim3((unsigned)(p.extra + p.nb), gy), block, lds, s>>>(a);
+  static_assert(8 * 64 >= EM_FEW && 16 * 64 * 8 >= EM_DIRECT && 8 * 64 >= EM_SPAN, "a workgroup takes its items in one go");
+  if (p.direct) return a.n <= EM_FEW ? emb_sum_launch<T, TO, N, true, 8, 1, 8>(p, a, s) : emb_sum_launch<T, TO, N, true, 16, 8, 16>(p, a, s);
+  GS_TRY((emb_sum_launch<T, TO, N, false, 8, 1, 8>(p, a, s)));
+  if (p.extra > 0) {
+    gs_embedding_join_kernel<TO, N><<<dim3((unsigned)p.extra, (unsigned)gs_cdiv(a.F, 64 * N), (unsigned)gs_cdiv(p.R, 4)), dim3(256), 0, s>>>(a);
     GS_LAUNCH_CHECK();
-    if (p.extra > 0)
-      gs_embedding_join_kernel<TO, N><<<dim3((unsigned)p.extra, (unsigned)gs_cdiv(a.F, 64 * N), (unsigned)gs_cdiv(p.R, 4)), dim3(256), 0, s>>>(a);
   }
-  GS_LAUNCH_CHECK();
   return GS_OK;
 }
 
