@@ -7,28 +7,41 @@
 
 namespace {
 
-// One thread takes 16 bytes of one output row.
+// One thread takes two 16-byte pieces of output rows, half of all pieces apart, so that two dependent loads (id, row) are under way.
+// 32-bit arithmetic: a 64-bit division costs more than the piece's traffic.
 template <int T>
 __global__ __launch_bounds__(256) void gs_embedding_fwd_kernel(const typename GsElt<T>::type* __restrict__ W, long ldw, long V, int F,
-                                                               const int* __restrict__ ids, long n, float scale,
-                                                               typename GsElt<T>::type* __restrict__ out, long ldo, int pieces) {
+                                                               const int* __restrict__ ids, unsigned total, float scale,
+                                                               typename GsElt<T>::type* __restrict__ out, long ldo, unsigned pieces) {
   typedef typename GsElt<T>::type E;
   constexpr int N = 16 / sizeof(E);
-  const long c = (long)blockIdx.x * 256 + threadIdx.x;
-  const long t = c / pieces;
-  if (t >= n) return;
-  const int f = (int)(c - t * pieces) * N;
-  const long id = ids[t];
-  float v[N];
-  if (id >= 0 && id < V) {
-    gs_load<E, N>(W + id * ldw + f, F - f, 0.f, v);
+  const unsigned half = (total + 1) / 2, c0 = blockIdx.x * 256u + threadIdx.x;
+  if (c0 >= half) return;
+  float v[2][N];
+  unsigned t[2];
+  int f[2];
+  long id[2];
+  bool on[2];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] *= scale;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.f;
+  for (int i = 0; i < 2; ++i) {
+    const unsigned c = c0 + i * half;
+    on[i] = c < total;
+    t[i] = on[i] ? c / pieces : 0;
+    f[i] = on[i] ? (int)(c - t[i] * pieces) * N : 0;
+    id[i] = ids[t[i]];
   }
-  gs_store<E, N>(out + t * ldo + f, F - f, v);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[i][e] = 0.f;
+    if (id[i] >= 0 && id[i] < V) gs_load<E, N>(W + id[i] * ldw + f[i], F - f[i], 0.f, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[i][e] *= scale;
+    if (on[i]) gs_store<E, N>(out + t[i] * ldo + f[i], F - f[i], v[i]);
+  }
 }
 
 // ---- the gradient ---------------------------------------------------------------------------------------------------------------
@@ -499,11 +512,14 @@ __global__ __launch_bounds__(256) void gs_embedding_join_kernel(EmbSum a) {
 template <int T>
 int emb_fwd(const void* W, long ldw, long V, int F, const int* ids, long n, float scale, void* out, long ldo, hipStream_t s) {
   typedef typename GsElt<T>::type E;
-  const int pieces = gs_cdiv(F, 16 / sizeof(E));
-  const long blocks = (n * pieces + 255) / 256;
-  if (blocks > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_embedding_fwd: %ld x %d is beyond one launch", n, F);
-  gs_embedding_fwd_kernel<T><<<dim3((unsigned)blocks), dim3(256), 0, s>>>((const E*)W, ldw, V, F, ids, n, scale, (E*)out, ldo, pieces);
-  GS_LAUNCH_CHECK();
+  const unsigned pieces = (unsigned)gs_cdiv(F, 16 / sizeof(E));
+  const long band = std::max(1L, (1L << 31) / (long)pieces);          // rows of a launch: their pieces are counted in 32 bits
+  for (long t0 = 0; t0 < n; t0 += band) {
+    const unsigned total = (unsigned)(std::min(band, n - t0) * pieces);
+    gs_embedding_fwd_kernel<T><<<dim3((total / 2 + 256) / 256), dim3(256), 0, s>>>((const E*)W, ldw, V, F, ids + t0, total, scale,
+                                                                                  (E*)out + t0 * ldo, ldo, pieces);
+    GS_LAUNCH_CHECK();
+  }
   return GS_OK;
 }
 

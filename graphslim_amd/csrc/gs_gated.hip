@@ -22,6 +22,8 @@ typedef const __attribute__((address_space(1))) void* gbl_ptr;
 
 constexpr int GF_PAD = 64;   // rows of laid-out operands are multiples of this many elements
 
+constexpr long GF_MAX_BLOCKS = 0xffffffL;   // of 256 threads that count their work in 32 bits
+
 inline long gf_up(long n) { return (n + GF_PAD - 1) / GF_PAD * GF_PAD; }
 
 // ---- activations: the value and its derivative ---------------------------------------------------------------------------------
@@ -117,9 +119,8 @@ __global__ __launch_bounds__(256) void gs_gated_pack_kernel(GatedPack a) {
   typedef typename GsElt<T>::type E;
   typedef typename GfPlane<T, PL>::type P;
   const int w = (long)blockIdx.x >= a.first[2] ? 2 : ((long)blockIdx.x >= a.first[1] ? 1 : 0);
-  const long per = a.Cp / 8;
-  const long i = ((long)blockIdx.x - a.first[w]) * 256 + threadIdx.x;
-  const long r = i / per, c = (i - r * per) * 8;
+  const unsigned per = (unsigned)(a.Cp / 8), i = (blockIdx.x - (unsigned)a.first[w]) * 256u + threadIdx.x, q = i / per;
+  const long r = q, c = (long)(i - q * per) * 8;
   if (r >= a.Rp[w]) return;
   float v[8];
   if (c < a.C && r < a.R[w]) {
@@ -137,9 +138,8 @@ __global__ __launch_bounds__(256) void gs_gated_slopes_kernel(const typename GsE
                                                               const float* __restrict__ saved, long M, long F,
                                                               typename GfPlane<T, PL>::type* __restrict__ out, long Mp, long Fp, long plane) {
   typedef typename GfPlane<T, PL>::type P;
-  const long per = Fp / 8;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long m = i / per, f = (i - m * per) * 8;
+  const unsigned per = (unsigned)(Fp / 8), i = blockIdx.x * 256u + threadIdx.x, q = i / per;
+  const long m = q, f = (long)(i - q * per) * 8;
   if (m >= Mp) return;
   float dg[8], du[8];
 #pragma unroll
@@ -568,8 +568,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
 template <int T, bool GATED, int ACT>
 __global__ __launch_bounds__(256) void gs_gated_join_kernel(GatedGemm q, int slices) {
   typedef typename GsElt<T>::type E;
-  const long per = (q.N + 3) / 4, i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long m = i / per, n = (i - m * per) * 4;
+  const unsigned per = (unsigned)((q.N + 3) / 4), i = blockIdx.x * 256u + threadIdx.x, r = i / per;
+  const long m = r, n = (long)(i - r * per) * 4;
   if (m >= q.M) return;
   E* row = GATED ? (E*)q.C[0] + m * q.ldc : gf_row<E>(q, m);
   if (!row) return;
@@ -691,7 +691,8 @@ int gf_tile(GatedGemm q, const GatedSplit& sp, float* part, hipStream_t s) {
   kern<<<dim3((unsigned)(gx * gy), (unsigned)sp.slices), dim3(WM * WN * 64), LDS, s>>>(q);
   GS_LAUNCH_CHECK();
   if (sp.slices > 1) {
-    const long blocks = (q.M * ((q.N + 3) / 4) + 255) / 256;
+    const long blocks = (q.M * ((q.N + 3) / 4) + 255) / 256;   // (a product that is cut has few tiles)
+    if (blocks > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", q.M, q.N);
     gs_gated_join_kernel<T, GATED, ACT><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(q, sp.slices);
     GS_LAUNCH_CHECK();
   }
@@ -741,7 +742,7 @@ int gf_operands(const GatedCall& c, const GatedPlan& p, GatedOperands* o, hipStr
     P* sc = (P*)c.scratch;
     *o = {sc + p.x, {sc + p.wg, sc + p.wu}, p.Dp, p.Dp, p.Mp * p.Dp, p.Fp * p.Dp};
     const long bx = (p.Mp * (p.Dp / 8) + 255) / 256, bw = (p.Fp * (p.Dp / 8) + 255) / 256;
-    if (bx + 2 * bw > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: operands of width %ld are beyond one launch", c.D);
+    if (bx + 2 * bw > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: operands of width %ld are beyond one launch", c.D);
     const GatedPack a = {{c.x, c.wg, c.wu}, {sc + p.x, sc + p.wg, sc + p.wu}, {c.ldx, c.ldw, c.ldw}, {c.M, c.F, c.F}, {p.Mp, p.Fp, p.Fp},
                          {0, bx, bx + bw}, c.D, p.Dp};
     gs_gated_pack_kernel<T, PL><<<dim3((unsigned)(bx + 2 * bw)), dim3(256), 0, s>>>(a);
@@ -792,7 +793,7 @@ int gf_bwd(const GatedCall& c, hipStream_t s) {
   const GatedPlan p = gf_plan(c.M, c.D, c.F, T);
   P* dgu = (P*)c.scratch + p.dgu;
   const long plane = p.Mp * 2 * p.Fp, blocks = (p.Mp * (p.Fp / 8) + 255) / 256;
-  if (blocks > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated_bwd: %ld x %ld is beyond one launch", c.M, c.F);
+  if (blocks > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated_bwd: %ld x %ld is beyond one launch", c.M, c.F);
   GatedOperands o;
   GS_TRY((gf_operands<T, PL>(c, p, &o, s)));
   gs_gated_slopes_kernel<T, PL, ACT><<<dim3((unsigned)blocks), dim3(256), 0, s>>>((const E*)c.dh, c.lddh, c.saved, c.M, c.F, dgu, p.Mp, p.Fp, plane);
@@ -827,6 +828,7 @@ __global__ void gs_gated_zero_kernel(E* a, E* b, long R, long C, long ld) {
 template <int T>
 int gf_empty(const GatedCall& c, hipStream_t s) {
   typedef typename GsElt<T>::type E;
+  if ((c.F * c.D + 255) / 256 > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated_bwd: weights of %ld x %ld are beyond one launch", c.F, c.D);
   gs_gated_zero_kernel<E><<<dim3((unsigned)((c.F * c.D + 255) / 256)), dim3(256), 0, s>>>((E*)c.dwg, (E*)c.dwu, c.F, c.D, c.lddw);
   GS_LAUNCH_CHECK();
   return GS_OK;
