@@ -495,6 +495,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
             constexpr int p = decltype(p_)::value;
             gf_tr_read4<p * TILE_A * 2 + ks * 64 * BM, BM>(tra + buf * STAGE * 2, i0, &a[p][i0]);
           });
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = i0; i < i0 + 4; ++i)
 #pragma unroll
@@ -508,6 +509,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
             }
             acc[i][j] = gf_mfma(b[0][j], a[0][i], acc[i][j]);
           }
+        __builtin_amdgcn_s_setprio(0);
       });
     });
     if (k0 + BK < k_end) land(buf ^ 1);
