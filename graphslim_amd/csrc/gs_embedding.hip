@@ -104,8 +104,14 @@ __device__ __forceinline__ unsigned long long emb_match(int key, bool on, int bi
   return m;
 }
 
+// an id's row in the V rows from id0 on, or -1
+__device__ __forceinline__ int emb_row(int id, long id0, long V) {
+  const long r = (long)id - id0;
+  return id >= 0 && r >= 0 && r < V ? (int)r : -1;
+}
+
 // cnt[tile][bucket]: tokens of the tile in the bucket (rows of nbp = nb rounded up to 8 counts)
-__global__ __launch_bounds__(1024) void gs_embedding_count_kernel(const int* __restrict__ ids, long n, long V, int rshift, int nbp,
+__global__ __launch_bounds__(1024) void gs_embedding_count_kernel(const int* __restrict__ ids, long n, long id0, long V, int rshift, int nbp,
                                                                   int* __restrict__ cnt) {
   __shared__ int h[EM_MAX_BUCKETS];
   constexpr int Q = EM_TILE / 1024;
@@ -114,13 +120,13 @@ __global__ __launch_bounds__(1024) void gs_embedding_count_kernel(const int* __r
 #pragma unroll
   for (int i = 0; i < Q; ++i) {
     const long t = t0 + i * 1024 + threadIdx.x;
-    id[i] = t < n ? ids[t] : -1;
+    id[i] = t < n ? emb_row(ids[t], id0, V) : -1;
   }
   for (int b = threadIdx.x; b < nbp; b += 1024) h[b] = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < Q; ++i)
-    if (id[i] >= 0 && id[i] < V) atomicAdd(&h[id[i] >> rshift], 1);
+    if (id[i] >= 0) atomicAdd(&h[id[i] >> rshift], 1);
   __syncthreads();
   for (int b = threadIdx.x; b < nbp; b += 1024) cnt[(long)blockIdx.x * nbp + b] = h[b];
 }
@@ -128,7 +134,7 @@ __global__ __launch_bounds__(1024) void gs_embedding_count_kernel(const int* __r
 // Stable: a tile's place in a bucket follows from the counts of the tiles before it, a wave's from those of the waves before it, a
 // lane's from the lanes before it.  start[b]: where bucket b begins in the list; xs[b]: further spans of the buckets before b; owner[e]:
 // the bucket of further span e, or -1.
-__global__ __launch_bounds__(1024) void gs_embedding_place_kernel(const int* __restrict__ ids, long n, long V, int rshift, int nb, int nbp,
+__global__ __launch_bounds__(1024) void gs_embedding_place_kernel(const int* __restrict__ ids, long n, long id0, long V, int rshift, int nb, int nbp,
                                                                   int bits, const int* __restrict__ cnt, int tiles,
                                                                   int* __restrict__ start, int* __restrict__ xs, int* __restrict__ owner,
                                                                   int extra, int2* __restrict__ list) {
@@ -142,8 +148,7 @@ __global__ __launch_bounds__(1024) void gs_embedding_place_kernel(const int* __r
   int id[Q];
 #pragma unroll
   for (int i = 0; i < Q; ++i) {
-    id[i] = t0 + i * 64 < n ? ids[t0 + i * 64] : -1;
-    if (id[i] >= V) id[i] = -1;
+    id[i] = t0 + i * 64 < n ? emb_row(ids[t0 + i * 64], id0, V) : -1;
   }
   int before[PER] = {}, all[PER] = {};
   if (tid * PER < nbp) {
@@ -238,7 +243,7 @@ struct EmbSum {
   long ldd;
   void* dW;
   long ldw;
-  long n, V;
+  long n, id0, V;
   int F, R, rshift, nb, extra, slot_rows, cap, cw, cws, rbits;
   float scale;
   int accumulate;
@@ -319,14 +324,13 @@ __global__ __launch_bounds__(W * 64) void gs_embedding_sum_kernel(EmbSum a) {
     if (i < i1) {
       long row;
       if (DIRECT) {
-        row = a.ids[i];
+        row = emb_row(a.ids[i], a.id0, a.V);
       } else {
         const int2 v = a.list[i];
         t[j] = v.x;
         row = v.y;
       }
-      row -= row0;
-      if (row >= 0 && row < rows) r[j] = (int)row;
+      if (row >= row0 && row < row0 + rows) r[j] = (int)(row - row0);
     }
   }
   for (int i = tid; i < W * a.R; i += W * 64) cnt[i] = 0;
@@ -548,11 +552,11 @@ int emb_sum(const EmbPlan& p, EmbSum a, hipStream_t s) {
 }
 
 template <int T, int TO>
-int emb_bwd(const void* dout, long ldd, const int* ids, long n, long V, int F, float scale, int accumulate, void* dW, long ldw,
+int emb_bwd_rows(const void* dout, long ldd, const int* ids, long n, long id0, long V, int F, float scale, int accumulate, void* dW, long ldw,
             char* scratch, hipStream_t s) {
   const EmbPlan p = emb_plan(n, V, F);
   EmbSum a = {};
-  a.ids = ids; a.dout = dout; a.ldd = ldd; a.dW = dW; a.ldw = ldw; a.n = n; a.V = V; a.F = F; a.scale = scale; a.accumulate = accumulate;
+  a.ids = ids; a.dout = dout; a.ldd = ldd; a.dW = dW; a.ldw = ldw; a.n = n; a.id0 = id0; a.V = V; a.F = F; a.scale = scale; a.accumulate = accumulate;
   a.R = p.R; a.nb = p.nb; a.extra = p.extra; a.slot_rows = p.R < EM_SPAN ? p.R : EM_SPAN;
   while ((1 << a.rbits) < p.R) ++a.rbits;
   a.rshift = a.rbits;
@@ -564,9 +568,9 @@ int emb_bwd(const void* dout, long ldd, const int* ids, long n, long V, int F, f
     int* cnt = (int*)(scratch + p.cnt);
     int bits = 0;
     while ((1 << bits) < p.nb) ++bits;
-    gs_embedding_count_kernel<<<dim3((unsigned)p.tiles), dim3(1024), 0, s>>>(ids, n, V, a.rshift, p.nbp, cnt);
+    gs_embedding_count_kernel<<<dim3((unsigned)p.tiles), dim3(1024), 0, s>>>(ids, n, id0, V, a.rshift, p.nbp, cnt);
     GS_LAUNCH_CHECK();
-    gs_embedding_place_kernel<<<dim3((unsigned)p.tiles), dim3(1024), 0, s>>>(ids, n, V, a.rshift, p.nb, p.nbp, bits, cnt, p.tiles, start, xs, owner, p.extra, list);
+    gs_embedding_place_kernel<<<dim3((unsigned)p.tiles), dim3(1024), 0, s>>>(ids, n, id0, V, a.rshift, p.nb, p.nbp, bits, cnt, p.tiles, start, xs, owner, p.extra, list);
     GS_LAUNCH_CHECK();
     a.start = start; a.xs = xs; a.owner = owner; a.list = list; a.ptrs = (int*)(scratch + p.ptrs); a.part = (float*)(scratch + p.part);
   }
@@ -575,6 +579,16 @@ int emb_bwd(const void* dout, long ldd, const int* ids, long n, long V, int F, f
   if (F >= 64 * N) return emb_sum<T, TO, N>(p, a, s);
   if (F >= 128) return emb_sum<T, TO, 2>(p, a, s);
   return emb_sum<T, TO, 1>(p, a, s);
+}
+
+// tables of more rows than the buckets hold: a band of rows after the other
+template <int T, int TO>
+int emb_bwd(const void* dout, long ldd, const int* ids, long n, long V, int F, float scale, int accumulate, void* dW, long ldw,
+            char* scratch, hipStream_t s) {
+  for (long v0 = 0; v0 < V; v0 += EM_MAX_V)
+    GS_TRY((emb_bwd_rows<T, TO>(dout, ldd, ids, n, v0, std::min(V - v0, EM_MAX_V), F, scale, accumulate,
+                                (typename GsElt<TO>::type*)dW + v0 * ldw, ldw, scratch, s)));
+  return GS_OK;
 }
 
 int emb_check(const char* who, long n, long V, int F, int type, long ld0, long ld1) {
@@ -599,7 +613,7 @@ extern "C" int gs_embedding_fwd(const void* W, long ldw, long V, int F, int type
 }
 
 extern "C" size_t gs_embedding_bwd_scratch_bytes(long n, long V, int F) {
-  return n < 0 || V < 1 || F < 1 || V > EM_MAX_V || n > 0x7fffffffL ? 0 : emb_plan(n, V, F).bytes;
+  return n < 0 || V < 1 || F < 1 || n > 0x7fffffffL ? 0 : emb_plan(n, std::min(V, EM_MAX_V), F).bytes;
 }
 
 extern "C" int gs_embedding_bwd(const void* dout, long ldd, int type, const int* ids, long n, long V, int F, float scale, int accumulate,
@@ -607,7 +621,6 @@ extern "C" int gs_embedding_bwd(const void* dout, long ldd, int type, const int*
   GS_TRY(emb_check("gs_embedding_bwd", n, V, F, type, ldd, ldw));
   if (type_dw != type && type_dw != GS_TYPE_F32)
     GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: the gradient is held in the type of d_out or in fp32 (got %d for %d)", type_dw, type);
-  if (V > EM_MAX_V) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_embedding_bwd: tables of at most %ld rows (got %ld)", EM_MAX_V, V);
   if (!dW || (n > 0 && (!dout || !ids))) GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: null pointer");
   if (gs_embedding_bwd_scratch_bytes(n, V, F) > 0 && (!scratch || ((size_t)scratch & 15)))
     GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: the scratch is missing or not 16-byte aligned");

@@ -332,7 +332,9 @@ size_t gs_gated_fwd_scratch_bytes(long M, long D, long F, int type);
 int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, long ldw, int type, long M, long D, long F, int act,
                  void* h, long ldh, float* saved, void* scratch, gs_stream_t stream);
 /* dg = dh * u * act'(g), du = dh * act(g) (rounded to the operands' type: the products take them there); dx = dg Wg + du Wu,
- * dw_gate = dg^T x, dw_up = du^T x. */
+ * dw_gate = dg^T x, dw_up = du^T x.
+ * fp32 products of more than a few rows are six products of bf16 parts: as exact as fp32 (parts have a smallest step of 2^-133), but an
+ * infinite operand gives NaN where it meets a zero part. */
 size_t gs_gated_bwd_scratch_bytes(long M, long D, long F, int type);
 int gs_gated_bwd(const void* dh, long lddh, const void* x, long ldx, const void* w_gate, const void* w_up, long ldw, const float* saved,
                  int type, long M, long D, long F, int act, void* dx, long lddx, void* dw_gate, void* dw_up, long lddw, void* scratch,
@@ -343,7 +345,7 @@ int gs_gated_bwd(const void* dh, long lddh, const void* x, long ldx, const void*
  *   loss[i] = tau^2 sum_j p_j (log p_j - log q_{c_j}),   dZ[i][v] = d_loss[i] tau (q_v - sum_{j : c_j = v} p_j).
  * An entry whose class is outside [0, V) or whose logit is -inf is not there.  A row without entries has loss 0 and gradient 0, and
  * its logits do not matter; a row with d_loss 0 has gradient 0.  Where all logits of a row are -inf, q is 0.  The soft-label
- * counterpart of gs_softmax_nll_grad_f32; dZ may be Z.
+ * counterpart of gs_softmax_nll_grad_f32; dZ may be Z (with its stride).
  * gs_distill_fwd also writes lse[i] = log sum_v exp(Z[i][v] / tau), which gs_distill_bwd takes; gs_distill_loss_grad is both at
  * once for row weights that are known beforehand (1 / n).  (lse is one fp32: the gradient from it resolves q to about 2^-24 |lse|,
  * which says nothing for a row whose every logit is the type's lowest value; gs_distill_loss_grad has no such limit.) */

@@ -75,7 +75,7 @@ def test_embedding_shapes_and_padding(ops):
 
 GRAD_SHAPES = [(1, 1, 1), (1, 9, 5), (3, 2, 64), (64, 100, 8), (257, 33, 127), (1000, 1000, 602), (4099, 300, 40), (4096, 5, 130),
                (9001, 2500, 65), (20000, 70, 33), (300, 140001, 9),
-               (7000, 270001, 5)]
+               (7000, 270001, 5), (20, 2200003, 2), (9000, 2200003, 2)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -82,6 +82,17 @@ def test_gated_refusals(ops):
             call()
 
 
+def test_shared_and_broadcast_rows_are_refused(ops):
+    """A broadcast gradient or input has rows that overlap: it is made dense by the caller, not read with a stride of 0."""
+    w, ids = torch.zeros(6, 4), torch.zeros(3, dtype=torch.int32)
+    row = torch.zeros(1, 4)
+    for call in (lambda: ops.embedding_grad(row.expand(3, 4), ids, 5), lambda: ops.gated_ffn(row.expand(3, 4), w, w),
+                 lambda: ops.gated_ffn(row.expand(3, 4), w, row.expand(6, 4)),
+                 lambda: ops.distill(row.expand(3, 4), torch.zeros(3, 1), torch.zeros(3, 1, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+
+
 def test_distill_refusals(ops):
     z, tv, ti, v = torch.zeros(3, 9), torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3)
     for match, call in [("one row a row", lambda: ops.distill(z, tv[:2], ti)), ("top_values are", lambda: ops.distill(z, tv.half(), ti)),
@@ -120,6 +131,8 @@ def test_c_entry_points_refuse(L):
     assert L.gs_distill_fwd(buf, 9, 0, 3, 9, buf, buf, 1025, 1.0, buf, buf, N) == UNSUPPORTED
     assert L.gs_distill_fwd(buf, 9, 0, 3, 9, buf, buf, 2, 0.0, buf, buf, N) == ARG and b"temperature" in L.gs_last_error()
     assert L.gs_distill_fwd(buf, 8, 0, 3, 9, buf, buf, 2, 1.0, buf, buf, N) == ARG and b"stride" in L.gs_last_error()
+    assert L.gs_distill_fwd(buf, 9, 0, 3, 9, buf, buf, 2, 1e-40, buf, buf, N) == ARG and b"reciprocal" in L.gs_last_error()
+    assert L.gs_distill_loss_grad(buf, 12, 0, 3, 9, buf, buf, 2, 1.0, buf, buf, buf, 9, N) == ARG and b"in place" in L.gs_last_error()
     assert L.gs_distill_bwd(N, 9, 0, 3, 9, N, N, 2, 1.0, N, N, N, 9, N) == ARG
     assert L.gs_distill_loss_grad(N, 9, 0, 0, 9, N, N, 2, 1.0, N, N, N, 9, N) == 0
 
