@@ -7,6 +7,7 @@
 // (Parts have bf16's smallest step, 2^-133: a value is represented to 2^-134 or to 24 bits, whichever is coarser.)
 // The parts of fp32 operands, and [dg | du], are laid out in the caller's scratch first, rows padded with zeros to a multiple of 64;
 // 16-bit operands are read where they are, whatever their alignment and width.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -38,13 +39,19 @@ __device__ __forceinline__ void gf_act(float g, float& a, float& da) {
     da = cdf + g * __expf(-0.5f * g * g) * 0.39894228040143268f;
   } else {
     const float sig = 1.f / (1.f + __expf(-g));
-    if constexpr (ACT == GS_ACT_SILU) {
-      a = g * sig;
-      da = sig * (1.f + g * (1.f - sig));
-    } else {
-      a = sig;
-      da = sig * (1.f - sig);
-    }
+    a = ACT == GS_ACT_SILU ? g * sig : sig;
+    da = ACT == GS_ACT_SILU ? sig * (1.f + g * (1.f - sig)) : sig * (1.f - sig);
+  }
+}
+
+// f(activation as a constant); act is the same for a whole launch, and the choice is made once, outside of all loops
+template <typename Fn>
+__device__ __forceinline__ void gf_with_act(int act, Fn f) {
+  switch (act) {
+    case GS_ACT_SILU: f(std::integral_constant<int, GS_ACT_SILU>{}); break;
+    case GS_ACT_GELU: f(std::integral_constant<int, GS_ACT_GELU>{}); break;
+    case GS_ACT_RELU: f(std::integral_constant<int, GS_ACT_RELU>{}); break;
+    default: f(std::integral_constant<int, GS_ACT_SIGMOID>{}); break;
   }
 }
 
@@ -133,8 +140,8 @@ __global__ __launch_bounds__(256) void gs_gated_pack_kernel(GatedPack a) {
 }
 
 // dg, du from dh and the saved g, u: [PL][Mp][2 Fp], columns [0, Fp) dg, [Fp, 2 Fp) du, zeros in the padding of both
-template <int T, int PL, int ACT>
-__global__ __launch_bounds__(256) void gs_gated_slopes_kernel(const typename GsElt<T>::type* __restrict__ dh, long lddh,
+template <int T, int PL>
+__global__ __launch_bounds__(256) void gs_gated_slopes_kernel(int act, const typename GsElt<T>::type* __restrict__ dh, long lddh,
                                                               const float* __restrict__ saved, long M, long F,
                                                               typename GfPlane<T, PL>::type* __restrict__ out, long Mp, long Fp, long plane) {
   typedef typename GfPlane<T, PL>::type P;
@@ -149,13 +156,15 @@ __global__ __launch_bounds__(256) void gs_gated_slopes_kernel(const typename GsE
     gs_load<typename GsElt<T>::type, 8>(dh + m * lddh + f, F - f, 0.f, d);
     gs_load<float, 8>(saved + m * F + f, F - f, 0.f, g);
     gs_load<float, 8>(saved + (M + m) * F + f, F - f, 0.f, u);
+    gf_with_act(act, [&](auto ac) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float a, da;
-      gf_act<ACT>(g[j], a, da);
-      du[j] = d[j] * a;
-      dg[j] = d[j] * u[j] * da;
-    }
+      for (int j = 0; j < 8; ++j) {
+        float a, da;
+        gf_act<decltype(ac)::value>(g[j], a, da);
+        du[j] = d[j] * a;
+        dg[j] = d[j] * u[j] * da;
+      }
+    });
   }
   P* o = out + m * 2 * Fp + f;
   gf_put8<T, PL>(dg, o, plane);
@@ -170,9 +179,10 @@ struct GatedRows {
   long ldx, ldw, M, D, F, ldh;
   void* h;
   float* saved;
+  int act;
 };
 
-template <int T, int MB, int RF, int ACT>
+template <int T, int MB, int RF>
 __global__ __launch_bounds__(256) void gs_gated_rows_kernel(GatedRows q) {
   typedef typename GsElt<T>::type E;
   constexpr int N = 16 / sizeof(E);
@@ -223,21 +233,23 @@ __global__ __launch_bounds__(256) void gs_gated_rows_kernel(GatedRows q) {
   for (int m = 0; m < MB; ++m)
 #pragma unroll
     for (int r = 0; r < 2 * RF; ++r) acc[m][r] = gs_wave_sum(acc[m][r]);
+  gf_with_act(q.act, [&](auto ac) {
 #pragma unroll
-  for (int m = 0; m < MB; ++m)
+    for (int m = 0; m < MB; ++m)
 #pragma unroll
-    for (int r = 0; r < RF; ++r) {
-      const long f = f0 + r;
-      if (lane == m * RF + r && m0 + m < q.M && f < q.F) {
-        float a, da;
-        gf_act<ACT>(acc[m][r], a, da);
-        ((E*)q.h)[(m0 + m) * q.ldh + f] = (E)(a * acc[m][RF + r]);
-        if (q.saved) {
-          q.saved[(m0 + m) * q.F + f] = acc[m][r];
-          q.saved[(q.M + m0 + m) * q.F + f] = acc[m][RF + r];
+      for (int r = 0; r < RF; ++r) {
+        const long f = f0 + r;
+        if (lane == m * RF + r && m0 + m < q.M && f < q.F) {
+          float a, da;
+          gf_act<decltype(ac)::value>(acc[m][r], a, da);
+          ((E*)q.h)[(m0 + m) * q.ldh + f] = (E)(a * acc[m][RF + r]);
+          if (q.saved) {
+            q.saved[(m0 + m) * q.F + f] = acc[m][r];
+            q.saved[(q.M + m0 + m) * q.F + f] = acc[m][RF + r];
+          }
         }
       }
-    }
+  });
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------------------
@@ -253,6 +265,7 @@ struct GatedGemm {
   void* C[2];           // plain form: rows [0, rows) go to C[0], rows [rows1, rows1 + rows) to C[1], others nowhere
   long ldc, rows, rows1;
   float* saved;         // gated form: g [M][N] and u [M][N], or null
+  int act;
   float* part;          // k cut into slices: slice z writes its sums to part + z * slice ([M][N]; gated: two of them), nothing to C
   long slice;
   int gx;               // tiles of m
@@ -340,8 +353,8 @@ __device__ __forceinline__ void gf_tr_read4(unsigned addr, int first, Frag* x) {
 // index is contiguous, not k.  RAW: x and the weights are read where they are though their rows begin at any element or end inside a
 // step of k: through registers, with zeros behind a row's end.  GATED: rows of B alternate between gate and up every 16, so that a lane holds both sums of its outputs
 // and the activation is applied in registers.
-template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED, int ACT>
-__global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q) {
+template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED>
+__device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, unsigned slice, char* smem) {
   typedef typename GfPlane<T, PL>::type P;
   typedef typename GfFrag<P>::type Frag;
   typedef typename GsElt<T>::type E;
@@ -350,16 +363,15 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
   constexpr int TILE_A = BM * BK, TILE_B = BN * BK, STAGE = PL * (TILE_A + TILE_B);
   constexpr int ITA = TILE_A / 8 / NT, ITB = TILE_B / 8 / NT;
   static_assert(TILE_A / 8 % NT == 0 && TILE_B / 8 % NT == 0, "whole waves load a tile");
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
   P* lds = (P*)smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave / WN, wn = wave % WN;
   // Tiles of m first: what runs at a time on an XCD (every eighth workgroup) shares four rows of tiles and their columns in its L2.
   // (8192 x 2048 x 8192: giving each XCD a run of consecutive tiles instead changes nothing without `saved`, and with it costs 100 us
   // of 560, since neighbouring pieces of its rows are then written far apart in time.)
-  const long m0 = (long)(blockIdx.x % q.gx) * BM;
-  const long n0 = (long)(blockIdx.x / q.gx) * (GATED ? BN / 2 : BN);
-  const long k_begin = blockIdx.y * q.kslice, k_end = min(k_begin + q.kslice, q.K);
+  const long m0 = (long)(block % q.gx) * BM;
+  const long n0 = (long)(block / q.gx) * (GATED ? BN / 2 : BN);
+  const long k_begin = slice * q.kslice, k_end = min(k_begin + q.kslice, q.K);
   const P* A = (const P*)q.A;
 
   const P* srcA[ITA];
@@ -517,60 +529,86 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
 
   // B is the first operand, so a lane holds four consecutive n of one m
   const int lr = lane & 15, lc = lane >> 4;
+  auto finish = [&](auto ac) {
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const long m = m0 + (wm * FM + i) * 16 + lr;
-    if (m >= q.M) continue;
-    if constexpr (GATED) {
+    for (int i = 0; i < FM; ++i) {
+      const long m = m0 + (wm * FM + i) * 16 + lr;
+      if (m >= q.M) continue;
+      if constexpr (GATED) {
 #pragma unroll
-      for (int j = 0; j < FN; j += 2) {
-        const long n = n0 + (wn * FN + j) * 8 + lc * 4;
-        if (n >= q.N) continue;
-        float g[4], u[4], h[4], da;
+        for (int j = 0; j < FN; j += 2) {
+          const long n = n0 + (wn * FN + j) * 8 + lc * 4;
+          if (n >= q.N) continue;
+          float g[4], u[4], h[4], da;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          g[e] = acc[i][j][e];
-          u[e] = acc[i][j + 1][e];
+          for (int e = 0; e < 4; ++e) {
+            g[e] = acc[i][j][e];
+            u[e] = acc[i][j + 1][e];
+          }
+          if constexpr (decltype(ac)::value < 0) {
+            float* o = q.part + slice * q.slice + m * q.N + n;
+            gs_store<float, 4>(o, q.N - n, g);
+            gs_store<float, 4>(o + q.M * q.N, q.N - n, u);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              gf_act<decltype(ac)::value>(g[e], h[e], da);
+              h[e] *= u[e];
+            }
+            gs_store<E, 4>((E*)q.C[0] + m * q.ldc + n, q.N - n, h);
+            if (q.saved) {
+              gs_store<float, 4>(q.saved + m * q.N + n, q.N - n, g);
+              gs_store<float, 4>(q.saved + (q.M + m) * q.N + n, q.N - n, u);
+            }
+          }
         }
-        if (q.part) {
-          float* o = q.part + blockIdx.y * q.slice + m * q.N + n;
-          gs_store<float, 4>(o, q.N - n, g);
-          gs_store<float, 4>(o + q.M * q.N, q.N - n, u);
-          continue;
-        }
+      } else {
+        E* row = gf_row<E>(q, m);
+        if (!row) continue;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          gf_act<ACT>(g[e], h[e], da);
-          h[e] *= u[e];
-        }
-        gs_store<E, 4>((E*)q.C[0] + m * q.ldc + n, q.N - n, h);
-        if (q.saved) {
-          gs_store<float, 4>(q.saved + m * q.N + n, q.N - n, g);
-          gs_store<float, 4>(q.saved + (q.M + m) * q.N + n, q.N - n, u);
-        }
-      }
-    } else {
-      E* row = gf_row<E>(q, m);
-      if (!row) continue;
+        for (int j = 0; j < FN; ++j) {
+          const long n = n0 + (wn * FN + j) * 16 + lc * 4;
+          if (n >= q.N) continue;
+          float v[4];
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const long n = n0 + (wn * FN + j) * 16 + lc * 4;
-        if (n >= q.N) continue;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
-        if (q.part) gs_store<float, 4>(q.part + blockIdx.y * q.slice + m * q.N + n, q.N - n, v);
-        else gs_store<E, 4>(row + n, q.N - n, v);
+          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
+          if (q.part) gs_store<float, 4>(q.part + slice * q.slice + m * q.N + n, q.N - n, v);
+          else gs_store<E, 4>(row + n, q.N - n, v);
+        }
       }
     }
+  };
+  if constexpr (GATED) {
+    if (q.part) finish(std::integral_constant<int, -1>{});
+    else gf_with_act(q.act, finish);
+  } else {
+    finish(std::integral_constant<int, -1>{});
+  }
+}
+
+template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED>
+__global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  gf_product<T, PL, WM, WN, FM, FN, BK, TA, TB, RAW, GATED>(q, blockIdx.x, blockIdx.y, smem);
+}
+
+// dx and dW in one launch, where neither fills the chip alone: blocks [0, a_blocks) are dx's tiles and slices, the others dW's.
+template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool RAW>
+__global__ __launch_bounds__(WM * WN * 64) void gs_gated_pair_kernel(GatedGemm a, unsigned a_tiles, unsigned a_blocks, GatedGemm b, unsigned b_tiles) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  if (blockIdx.x < a_blocks) {
+    gf_product<T, PL, WM, WN, FM, FN, BK, false, true, RAW, false>(a, blockIdx.x % a_tiles, blockIdx.x / a_tiles, smem);
+  } else {
+    const unsigned i = blockIdx.x - a_blocks;
+    gf_product<T, PL, WM, WN, FM, FN, BK, true, true, RAW, false>(b, i % b_tiles, i / b_tiles, smem);
   }
 }
 
 // Sums the slices of k in their order and finishes what the product's epilogue does.  A thread takes four columns of a row.
-template <int T, bool GATED, int ACT>
-__global__ __launch_bounds__(256) void gs_gated_join_kernel(GatedGemm q, int slices) {
+template <int T, bool GATED>
+__device__ __forceinline__ void gf_join(const GatedGemm& q, int slices, unsigned block) {
   typedef typename GsElt<T>::type E;
-  const unsigned per = (unsigned)((q.N + 3) / 4), i = blockIdx.x * 256u + threadIdx.x, r = i / per;
+  const unsigned per = (unsigned)((q.N + 3) / 4), i = block * 256u + threadIdx.x, r = i / per;
   const long m = r, n = (long)(i - r * per) * 4;
   if (m >= q.M) return;
   E* row = GATED ? (E*)q.C[0] + m * q.ldc : gf_row<E>(q, m);
@@ -593,14 +631,27 @@ __global__ __launch_bounds__(256) void gs_gated_join_kernel(GatedGemm q, int sli
       gs_store<float, 4>(q.saved + m * q.N + n, q.N - n, g);
       gs_store<float, 4>(q.saved + (q.M + m) * q.N + n, q.N - n, u);
     }
-    float da;
+    gf_with_act(q.act, [&](auto ac) {
+      float da;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      gf_act<ACT>(g[e], g[e], da);
-      g[e] *= u[e];
-    }
+      for (int e = 0; e < 4; ++e) {
+        gf_act<decltype(ac)::value>(g[e], g[e], da);
+        g[e] *= u[e];
+      }
+    });
   }
   gs_store<E, 4>(row + n, q.N - n, g);
+}
+
+template <int T, bool GATED>
+__global__ __launch_bounds__(256) void gs_gated_join_kernel(GatedGemm q, int slices) {
+  gf_join<T, GATED>(q, slices, blockIdx.x);
+}
+
+template <int T>
+__global__ __launch_bounds__(256) void gs_gated_join_pair_kernel(GatedGemm a, int a_slices, unsigned a_blocks, GatedGemm b, int b_slices) {
+  if (blockIdx.x < a_blocks) gf_join<T, false>(a, a_slices, blockIdx.x);
+  else gf_join<T, false>(b, b_slices, blockIdx.x - a_blocks);
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------
@@ -610,6 +661,7 @@ struct GatedSplit {
   int slices;
   long kslice;        // in elements
   size_t part;        // floats
+  double cost;
 };
 
 // 16-bit operands: 128 x 128 (two workgroups on a compute unit) or 256 x 256 (one), which takes 1.75 times as long a step of 64 for twice
@@ -631,8 +683,39 @@ GatedSplit gf_split_of(long M, long N, long K, bool gated, int pl) {
       if (slices > 1) cost += 4 + (double)slices * M * cols * 8 / 4e6;
       if (cost < least) {
         least = cost;
-        best = {big != 0, (int)slices, per * bk, slices > 1 ? (size_t)slices * M * cols : 0};
+        best = {big != 0, (int)slices, per * bk, slices > 1 ? (size_t)slices * M * cols : 0, cost};
       }
+    }
+  }
+  return best;
+}
+
+// dx (M x D, k over 2 Fp) and dW (2 Fp x D, k over Mp): one launch of both, cut into pieces of about equal length, where that costs less
+// than one after the other (the same units, a launch about 3).
+struct GatedPair {
+  bool together;
+  GatedSplit dx, dw;
+};
+
+GatedPair gf_pair_of(long M, long D, long Fp, long Mp, int pl) {
+  GatedPair best = {false, gf_split_of(M, D, 2 * Fp, false, pl), gf_split_of(2 * Fp, D, Mp, false, pl)};
+  double least = best.dx.cost + best.dw.cost + 3;
+  for (int big = 0; big < 2; ++big) {
+    const long bm = big ? 256 : 128, bn = big && pl == 1 ? 256 : 128, bk = pl == 3 ? 32 : 64, gy = (D + bn - 1) / bn;
+    const long tx = (M + bm - 1) / bm * gy, tw = (2 * Fp + bm - 1) / bm * gy, slots = big || pl == 3 ? 256 : 512;
+    const long sx = 2 * Fp / bk, sw = Mp / bk, most = std::max(sx, sw);
+    const double step = big ? (pl == 3 ? 1.4 : 1.75) : 1.0;
+    for (long len = most;; len = (len * 3 + 3) / 4) {
+      const long nx = std::min(64L, (sx + len - 1) / len), nw = std::min(64L, (sw + len - 1) / len);
+      const long px = (sx + nx - 1) / nx, pw = (sw + nw - 1) / nw, cx = (sx + px - 1) / px, cw = (sw + pw - 1) / pw;
+      const double all = (double)(tx * cx * (px + 2) + tw * cw * (pw + 2)) / slots, one = (double)std::max(px, pw) + 2;
+      double cost = step * (tx * cx + tw * cw <= slots ? one : std::max(all + 0.35 * one, one));
+      if (cx > 1 || cw > 1) cost += 4 + (double)((cx > 1 ? cx * M : 0) + (cw > 1 ? cw * 2 * Fp : 0)) * D * 8 / 4e6;
+      if (cost < least) {
+        least = cost;
+        best = {true, {big != 0, (int)cx, px * bk, cx > 1 ? (size_t)cx * M * D : 0, 0}, {big != 0, (int)cw, pw * bk, cw > 1 ? (size_t)cw * 2 * Fp * D : 0, 0}};
+      }
+      if (len <= 4 || tx * cx + tw * cw > 2 * slots) break;
     }
   }
   return best;
@@ -645,10 +728,12 @@ struct GatedPlan {
   size_t x, wg, wu, fwd;              // fp32: the parts of x, Wg, Wu with padded rows (both passes)
   size_t dgu, bwd;                    // backward: [dg | du]
   size_t part_fwd, part_bwd;          // partial sums of products that are cut along k, behind the operands
+  GatedSplit split;                   // of the forward product
+  GatedPair pair;                     // of the backward ones
 };
 
-GatedPlan gf_plan(long M, long D, long F, int type) {
-  GatedPlan p;
+GatedPlan gf_plan(long M, long D, long F, int type, bool bwd) {
+  GatedPlan p = {};
   p.pl = type == GS_TYPE_F32 ? 3 : 1;
   p.Dp = gf_up(D);
   p.Fp = gf_up(F);
@@ -661,58 +746,111 @@ GatedPlan gf_plan(long M, long D, long F, int type) {
     p.wu = take((size_t)p.Fp * p.Dp);
   }
   p.part_fwd = o;
-  p.fwd = o + 2 * gf_split_of(M, F, p.Dp, true, p.pl).part;
+  if (!bwd) {
+    p.split = gf_split_of(M, F, p.Dp, true, p.pl);
+    p.fwd = o + 2 * p.split.part;
+  }
   p.dgu = take((size_t)p.Mp * 2 * p.Fp);
   p.part_bwd = o;
-  const size_t dx = gf_split_of(M, D, 2 * p.Fp, false, p.pl).part, dw = gf_split_of(2 * p.Fp, D, p.Mp, false, p.pl).part;
-  p.bwd = o + 2 * (dx > dw ? dx : dw);
+  if (bwd) {
+    p.pair = gf_pair_of(M, D, p.Fp, p.Mp, p.pl);
+    const size_t dx = p.pair.dx.part, dw = p.pair.dw.part;
+    p.bwd = o + 2 * (p.pair.together ? dx + dw : std::max(dx, dw));
+  }
   return p;
 }
 
-template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED, int ACT>
-int gf_tile(GatedGemm q, const GatedSplit& sp, float* part, hipStream_t s) {
-  constexpr int BM = WM * FM * 16, BN = WN * FN * 16 / (GATED ? 2 : 1), LDS = 2 * PL * (WM * FM + WN * FN) * 16 * BK * 2;
-  auto kern = gs_gated_gemm_kernel<T, PL, WM, WN, FM, FN, BK, TA, TB, RAW, GATED, ACT>;
-  if (LDS > 65536) {   // once for each device
-    static std::atomic<unsigned long long> known{0};
-    int dev = 0;
-    GS_HIP(hipGetDevice(&dev));
-    if (dev > 63 || !(known.load(std::memory_order_relaxed) >> dev & 1)) {
-      GS_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-      if (dev <= 63) known.fetch_or(1ull << dev, std::memory_order_relaxed);
-    }
-  }
+// dynamic LDS beyond 64 KB is asked for once for each kernel and device
+template <typename Kernel>
+int gf_lds(Kernel kern, int bytes, std::atomic<unsigned long long>& known) {
+  if (bytes <= 65536) return GS_OK;
+  int dev = 0;
+  GS_HIP(hipGetDevice(&dev));
+  if (dev <= 63 && (known.load(std::memory_order_relaxed) >> dev & 1)) return GS_OK;
+  GS_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev <= 63) known.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return GS_OK;
+}
+
+// Sets a product's slices; its tiles of BM x BN, or an error
+int gf_prepare(GatedGemm& q, const GatedSplit& sp, int BM, int BN, bool gated, float* part, long* tiles) {
   const long gx = (q.M + BM - 1) / BM, gy = (q.N + BN - 1) / BN;
-  if (gx * gy > 0x1fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", q.M, q.N);
+  if (gx * gy * sp.slices > 0x1fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", q.M, q.N);
   q.gx = (int)gx;
   q.kslice = sp.kslice;
   if (sp.slices > 1) {
     q.part = part;
-    q.slice = q.M * q.N * (GATED ? 2 : 1);
+    q.slice = q.M * q.N * (gated ? 2 : 1);
   }
-  kern<<<dim3((unsigned)(gx * gy), (unsigned)sp.slices), dim3(WM * WN * 64), LDS, s>>>(q);
+  *tiles = gx * gy;
+  return GS_OK;
+}
+
+inline long gf_join_blocks(const GatedGemm& q) { return (q.M * ((q.N + 3) / 4) + 255) / 256; }   // (a product that is cut has few tiles)
+
+template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED>
+int gf_tile(GatedGemm q, const GatedSplit& sp, float* part, hipStream_t s) {
+  constexpr int BM = WM * FM * 16, BN = WN * FN * 16 / (GATED ? 2 : 1), LDS = 2 * PL * (WM * FM + WN * FN) * 16 * BK * 2;
+  auto kern = gs_gated_gemm_kernel<T, PL, WM, WN, FM, FN, BK, TA, TB, RAW, GATED>;
+  static std::atomic<unsigned long long> known{0};
+  GS_TRY(gf_lds(kern, LDS, known));
+  long tiles;
+  GS_TRY(gf_prepare(q, sp, BM, BN, GATED, part, &tiles));
+  kern<<<dim3((unsigned)tiles, (unsigned)sp.slices), dim3(WM * WN * 64), LDS, s>>>(q);
   GS_LAUNCH_CHECK();
   if (sp.slices > 1) {
-    const long blocks = (q.M * ((q.N + 3) / 4) + 255) / 256;   // (a product that is cut has few tiles)
-    if (blocks > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", q.M, q.N);
-    gs_gated_join_kernel<T, GATED, ACT><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(q, sp.slices);
+    if (gf_join_blocks(q) > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", q.M, q.N);
+    gs_gated_join_kernel<T, GATED><<<dim3((unsigned)gf_join_blocks(q)), dim3(256), 0, s>>>(q, sp.slices);
     GS_LAUNCH_CHECK();
   }
   return GS_OK;
 }
 
-template <int T, int PL, bool TA, bool TB, bool GATED, int ACT>
-int gf_gemm(const GatedGemm& q, bool raw, float* part, hipStream_t s) {
-  const GatedSplit sp = gf_split_of(q.M, q.N, q.K, GATED, PL);
+template <int T, int PL, bool TA, bool TB, bool GATED>
+int gf_gemm(const GatedGemm& q, const GatedSplit& sp, bool raw, float* part, hipStream_t s) {
   if constexpr (PL == 3) {
-    if (sp.big) return gf_tile<T, PL, 4, 2, 4, 4, 32, TA, TB, false, GATED, ACT>(q, sp, part, s);
-    return gf_tile<T, PL, 2, 2, 4, 4, 32, TA, TB, false, GATED, ACT>(q, sp, part, s);
+    if (sp.big) return gf_tile<T, PL, 4, 2, 4, 4, 32, TA, TB, false, GATED>(q, sp, part, s);
+    return gf_tile<T, PL, 2, 2, 4, 4, 32, TA, TB, false, GATED>(q, sp, part, s);
   } else if (raw) {
-    if (sp.big) return gf_tile<T, PL, 2, 4, 8, 4, 64, TA, TB, true, GATED, ACT>(q, sp, part, s);
-    return gf_tile<T, PL, 2, 2, 4, 4, 64, TA, TB, true, GATED, ACT>(q, sp, part, s);
+    if (sp.big) return gf_tile<T, PL, 2, 4, 8, 4, 64, TA, TB, true, GATED>(q, sp, part, s);
+    return gf_tile<T, PL, 2, 2, 4, 4, 64, TA, TB, true, GATED>(q, sp, part, s);
   } else {
-    if (sp.big) return gf_tile<T, PL, 2, 4, 8, 4, 64, TA, TB, false, GATED, ACT>(q, sp, part, s);
-    return gf_tile<T, PL, 2, 2, 4, 4, 64, TA, TB, false, GATED, ACT>(q, sp, part, s);
+    if (sp.big) return gf_tile<T, PL, 2, 4, 8, 4, 64, TA, TB, false, GATED>(q, sp, part, s);
+    return gf_tile<T, PL, 2, 2, 4, 4, 64, TA, TB, false, GATED>(q, sp, part, s);
+  }
+}
+
+template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool RAW>
+int gf_pair_tile(GatedGemm a, GatedGemm b, const GatedPair& p, float* part, hipStream_t s) {
+  constexpr int BM = WM * FM * 16, BN = WN * FN * 16, LDS = 2 * PL * (WM * FM + WN * FN) * 16 * BK * 2;
+  auto kern = gs_gated_pair_kernel<T, PL, WM, WN, FM, FN, BK, RAW>;
+  static std::atomic<unsigned long long> known{0};
+  GS_TRY(gf_lds(kern, LDS, known));
+  long ta, tb;
+  GS_TRY(gf_prepare(a, p.dx, BM, BN, false, part, &ta));
+  GS_TRY(gf_prepare(b, p.dw, BM, BN, false, part + p.dx.part, &tb));
+  kern<<<dim3((unsigned)(ta * p.dx.slices + tb * p.dw.slices)), dim3(WM * WN * 64), LDS, s>>>(a, (unsigned)ta, (unsigned)(ta * p.dx.slices), b, (unsigned)tb);
+  GS_LAUNCH_CHECK();
+  const long ja = p.dx.slices > 1 ? gf_join_blocks(a) : 0, jb = p.dw.slices > 1 ? gf_join_blocks(b) : 0;
+  if (std::max(ja, jb) > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", b.M, b.N);
+  if (ja + jb) {
+    gs_gated_join_pair_kernel<T><<<dim3((unsigned)(ja + jb)), dim3(256), 0, s>>>(a, p.dx.slices, (unsigned)ja, b, p.dw.slices);
+    GS_LAUNCH_CHECK();
+  }
+  return GS_OK;
+}
+
+template <int T, int PL>
+int gf_pair(const GatedGemm& a, const GatedGemm& b, const GatedPair& p, bool raw, float* part, hipStream_t s) {
+  if constexpr (PL == 3) {
+    if (p.dx.big) return gf_pair_tile<T, PL, 4, 2, 4, 4, 32, false>(a, b, p, part, s);
+    return gf_pair_tile<T, PL, 2, 2, 4, 4, 32, false>(a, b, p, part, s);
+  } else if (raw) {
+    if (p.dx.big) return gf_pair_tile<T, PL, 2, 4, 8, 4, 64, true>(a, b, p, part, s);
+    return gf_pair_tile<T, PL, 2, 2, 4, 4, 64, true>(a, b, p, part, s);
+  } else {
+    if (p.dx.big) return gf_pair_tile<T, PL, 2, 4, 8, 4, 64, false>(a, b, p, part, s);
+    return gf_pair_tile<T, PL, 2, 2, 4, 4, 64, false>(a, b, p, part, s);
   }
 }
 
@@ -757,24 +895,24 @@ int gf_operands(const GatedCall& c, const GatedPlan& p, GatedOperands* o, hipStr
 // matrix pipe; fp32, 24 rows 96 us against 115, of which laying out the split weights is most.
 inline bool gf_few(long M, int type) { return M <= (type == GS_TYPE_F32 ? 24 : 4); }
 
-template <int T, int MB, int ACT>
+template <int T, int MB>
 int gf_rows(const GatedCall& c, hipStream_t s) {
   constexpr int RF = 2;
-  GatedRows q = {c.x, c.wg, c.wu, c.ldx, c.ldw, c.M, c.D, c.F, c.ldh, c.h, c.saved};
-  gs_gated_rows_kernel<T, MB, RF, ACT><<<dim3((unsigned)((c.F + 4 * RF - 1) / (4 * RF)), (unsigned)((c.M + MB - 1) / MB)), dim3(256), 0, s>>>(q);
+  GatedRows q = {c.x, c.wg, c.wu, c.ldx, c.ldw, c.M, c.D, c.F, c.ldh, c.h, c.saved, c.act};
+  gs_gated_rows_kernel<T, MB, RF><<<dim3((unsigned)((c.F + 4 * RF - 1) / (4 * RF)), (unsigned)((c.M + MB - 1) / MB)), dim3(256), 0, s>>>(q);
   GS_LAUNCH_CHECK();
   return GS_OK;
 }
 
-template <int T, int PL, int ACT>
+template <int T, int PL>
 int gf_fwd(const GatedCall& c, hipStream_t s) {
   typedef typename GfPlane<T, PL>::type P;
   if (gf_few(c.M, T)) {
-    if (c.M == 1) return gf_rows<T, 1, ACT>(c, s);
-    if (c.M == 2) return gf_rows<T, 2, ACT>(c, s);
-    return c.M <= 4 ? gf_rows<T, 4, ACT>(c, s) : gf_rows<T, 8, ACT>(c, s);
+    if (c.M == 1) return gf_rows<T, 1>(c, s);
+    if (c.M == 2) return gf_rows<T, 2>(c, s);
+    return c.M <= 4 ? gf_rows<T, 4>(c, s) : gf_rows<T, 8>(c, s);
   }
-  const GatedPlan p = gf_plan(c.M, c.D, c.F, T);
+  const GatedPlan p = gf_plan(c.M, c.D, c.F, T, false);
   GatedOperands o;
   GS_TRY((gf_operands<T, PL>(c, p, &o, s)));
   const bool raw = PL == 1 && !(gf_plain(c.x, c.ldx, c.D, GF_PAD) && gf_plain(c.wg, c.ldw, c.D, GF_PAD) && gf_plain(c.wu, c.ldw, c.D, GF_PAD));
@@ -783,22 +921,22 @@ int gf_fwd(const GatedCall& c, hipStream_t s) {
   q.B[0] = o.w[0]; q.B[1] = o.w[1]; q.ldb = o.ldw; q.plane_b = o.plane_w;
   q.M = c.M; q.N = c.F; q.K = p.Dp;
   q.C[0] = c.h; q.ldc = c.ldh;
-  q.saved = c.saved;
+  q.saved = c.saved; q.act = c.act;
   q.k_end = c.D;
-  return gf_gemm<T, PL, false, false, true, ACT>(q, raw, (float*)((P*)c.scratch + p.part_fwd), s);
+  return gf_gemm<T, PL, false, false, true>(q, p.split, raw, (float*)((P*)c.scratch + p.part_fwd), s);
 }
 
-template <int T, int PL, int ACT>
+template <int T, int PL>
 int gf_bwd(const GatedCall& c, hipStream_t s) {
   typedef typename GsElt<T>::type E;
   typedef typename GfPlane<T, PL>::type P;
-  const GatedPlan p = gf_plan(c.M, c.D, c.F, T);
+  const GatedPlan p = gf_plan(c.M, c.D, c.F, T, true);
   P* dgu = (P*)c.scratch + p.dgu;
   const long plane = p.Mp * 2 * p.Fp, blocks = (p.Mp * (p.Fp / 8) + 255) / 256;
   if (blocks > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated_bwd: %ld x %ld is beyond one launch", c.M, c.F);
   GatedOperands o;
   GS_TRY((gf_operands<T, PL>(c, p, &o, s)));
-  gs_gated_slopes_kernel<T, PL, ACT><<<dim3((unsigned)blocks), dim3(256), 0, s>>>((const E*)c.dh, c.lddh, c.saved, c.M, c.F, dgu, p.Mp, p.Fp, plane);
+  gs_gated_slopes_kernel<T, PL><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(c.act, (const E*)c.dh, c.lddh, c.saved, c.M, c.F, dgu, p.Mp, p.Fp, plane);
   GS_LAUNCH_CHECK();
   // dx: k runs over the columns of dg, then of du, and over the rows of Wg, then of Wu
   GatedGemm q = {};
@@ -809,13 +947,15 @@ int gf_bwd(const GatedCall& c, hipStream_t s) {
   q.C[0] = c.dx; q.ldc = c.lddx; q.rows = q.rows1 = c.M;
   float* part = (float*)((P*)c.scratch + p.part_bwd);
   const bool raw_w = PL == 1 && !(gf_plain(c.wg, c.ldw, c.D, 8) && gf_plain(c.wu, c.ldw, c.D, 8)), raw_x = PL == 1 && !gf_plain(c.x, c.ldx, c.D, 8);
-  GS_TRY((gf_gemm<T, PL, false, true, false, GS_ACT_SILU>(q, raw_w, part, s)));
   // dWg, dWu: k runs over the tokens
-  q.B[0] = o.x; q.ldb = o.ldx; q.plane_b = o.plane_x;
-  q.M = 2 * p.Fp; q.K = p.Mp; q.kb = p.Mp; q.brows = o.plane_x ? p.Mp : c.M;
-  q.bcols = o.plane_x ? p.Dp : c.D;
-  q.C[0] = c.dwg; q.C[1] = c.dwu; q.ldc = c.lddw; q.rows = c.F; q.rows1 = p.Fp;
-  return gf_gemm<T, PL, true, true, false, GS_ACT_SILU>(q, raw_x, part, s);
+  GatedGemm w = q;
+  w.B[0] = o.x; w.ldb = o.ldx; w.plane_b = o.plane_x;
+  w.M = 2 * p.Fp; w.K = p.Mp; w.kb = p.Mp; w.brows = o.plane_x ? p.Mp : c.M;
+  w.bcols = o.plane_x ? p.Dp : c.D;
+  w.C[0] = c.dwg; w.C[1] = c.dwu; w.ldc = c.lddw; w.rows = c.F; w.rows1 = p.Fp;
+  if (p.pair.together) return gf_pair<T, PL>(q, w, p.pair, raw_w || raw_x, part, s);
+  GS_TRY((gf_gemm<T, PL, false, true, false>(q, p.pair.dx, raw_w, part, s)));
+  return gf_gemm<T, PL, true, true, false>(w, p.pair.dw, raw_x, part, s);
 }
 
 // dW = 0 where there are no tokens
@@ -839,12 +979,7 @@ int gf_empty(const GatedCall& c, hipStream_t s) {
 template <int T, int PL>
 int gf_dispatch(const GatedCall& c, bool bwd, hipStream_t s) {
   if (bwd && c.M == 0) return gf_empty<T>(c, s);
-  switch (c.act) {
-    case GS_ACT_SILU: return bwd ? gf_bwd<T, PL, GS_ACT_SILU>(c, s) : gf_fwd<T, PL, GS_ACT_SILU>(c, s);
-    case GS_ACT_GELU: return bwd ? gf_bwd<T, PL, GS_ACT_GELU>(c, s) : gf_fwd<T, PL, GS_ACT_GELU>(c, s);
-    case GS_ACT_RELU: return bwd ? gf_bwd<T, PL, GS_ACT_RELU>(c, s) : gf_fwd<T, PL, GS_ACT_RELU>(c, s);
-    default: return bwd ? gf_bwd<T, PL, GS_ACT_SIGMOID>(c, s) : gf_fwd<T, PL, GS_ACT_SIGMOID>(c, s);
-  }
+  return bwd ? gf_bwd<T, PL>(c, s) : gf_fwd<T, PL>(c, s);
 }
 
 int gf_check(const char* who, const GatedCall& c, int type) {
@@ -865,13 +1000,13 @@ int gf_run(const GatedCall& c, int type, bool bwd, hipStream_t s) {
 }  // namespace
 
 extern "C" size_t gs_gated_fwd_scratch_bytes(long M, long D, long F, int type) {
-  if (M < 0 || D < 1 || F < 1 || !gs_type_bytes(type)) return 0;
-  return gf_few(M, type) ? 0 : gf_plan(M, D, F, type).fwd * 2;
+  if (M < 1 || D < 1 || F < 1 || !gs_type_bytes(type)) return 0;
+  return gf_few(M, type) ? 0 : gf_plan(M, D, F, type, false).fwd * 2;
 }
 
 extern "C" size_t gs_gated_bwd_scratch_bytes(long M, long D, long F, int type) {
-  if (M < 0 || D < 1 || F < 1 || !gs_type_bytes(type)) return 0;
-  return gf_plan(M, D, F, type).bwd * 2;
+  if (M < 1 || D < 1 || F < 1 || !gs_type_bytes(type)) return 0;
+  return gf_plan(M, D, F, type, true).bwd * 2;
 }
 
 extern "C" int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, long ldw, int type, long M, long D, long F, int act,

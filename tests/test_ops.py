@@ -125,6 +125,7 @@ def test_c_entry_points_refuse(L):
     assert L.gs_gated_fwd(N, 4, N, N, 4, 0, 2, 4, 6, 0, N, 6, N, N, N) == ARG and b"null" in L.gs_last_error()
     assert L.gs_gated_fwd(N, 4, N, N, 4, 0, 0, 4, 6, 0, N, 6, N, N, N) == 0
     assert L.gs_gated_bwd(N, 6, N, 4, N, N, 4, N, 0, 2, 4, 6, 0, N, 4, N, N, 4, N, N) == ARG
+    assert L.gs_gated_fwd_scratch_bytes(0, 4, 6, 0) == L.gs_gated_bwd_scratch_bytes(0, 4, 6, 1) == 0
     assert L.gs_gated_fwd_scratch_bytes(-1, 4, 6, 0) == 0 and L.gs_gated_fwd_scratch_bytes(2, 4, 6, 5) == 0
     assert L.gs_distill_fwd(N, 9, 0, 3, 9, N, N, 2, 1.0, N, N, N) == ARG
     buf = 4096                                          # never read: the checks below come first
@@ -135,6 +136,21 @@ def test_c_entry_points_refuse(L):
     assert L.gs_distill_loss_grad(buf, 12, 0, 3, 9, buf, buf, 2, 1.0, buf, buf, buf, 9, N) == ARG and b"in place" in L.gs_last_error()
     assert L.gs_distill_bwd(N, 9, 0, 3, 9, N, N, 2, 1.0, N, N, N, 9, N) == ARG
     assert L.gs_distill_loss_grad(N, 9, 0, 0, 9, N, N, 2, 1.0, N, N, N, 9, N) == 0
+
+
+def test_scratch_sizes(L):
+    """For every shape from one row to a large batch: enough for the laid-out operands, and no more than a small multiple of them."""
+    for typ, parts in ((0, 3), (1, 1), (2, 1)):
+        for M in (1, 5, 33, 128, 1000, 8192):
+            for D, F in ((1, 1), (64, 64), (500, 1024), (1433, 4096), (2048, 8192)):
+                up = lambda n: (n + 63) // 64 * 64
+                slopes = up(M) * 2 * up(F) * 2 * parts
+                bwd = L.gs_gated_bwd_scratch_bytes(M, D, F, typ)
+                assert bwd >= slopes
+                laid = slopes + (parts > 1) * (up(M) + 2 * up(F)) * up(D) * 2 * parts
+                outputs = 4 * (M * D + 2 * up(F) * D)
+                assert bwd <= laid + 64 * outputs, (typ, M, D, F, bwd)
+                assert L.gs_gated_fwd_scratch_bytes(M, D, F, typ) <= (parts > 1) * (up(M) + 2 * up(F)) * up(D) * 2 * parts + 64 * 8 * M * F
 
 
 def _slope(f, x, v, e=1e-6):
