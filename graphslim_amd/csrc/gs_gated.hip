@@ -363,6 +363,7 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
   constexpr int TILE_A = BM * BK, TILE_B = BN * BK, STAGE = PL * (TILE_A + TILE_B);
   constexpr int ITA = TILE_A / 8 / NT, ITB = TILE_B / 8 / NT;
   static_assert(TILE_A / 8 % NT == 0 && TILE_B / 8 % NT == 0, "whole waves load a tile");
+  constexpr bool PHASES = WM * WN == 8 && BK == 64 && !RAW;       // eight waves that take turns, see below
   P* lds = (P*)smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave / WN, wn = wave % WN;
@@ -476,55 +477,96 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
   stage(0, k_begin);
   land(0);
   int buf = 0;
-  for (long k0 = k_begin; k0 < k_end; k0 += BK, buf ^= 1) {
-    __syncthreads();   // this step's tile has landed; the other buffer has been read by all
-    const P* ta = lds + buf * STAGE;
-    const P* tb = ta + PL * TILE_A;
-    if (k0 + BK < k_end) stage(buf ^ 1, k0 + BK);
-    gf_static_for<BK / 32>([&](auto ks_) {
-      constexpr int ks = decltype(ks_)::value;
-      Frag a[PL][FM], b[PL][FN];
-      gf_static_for<PL>([&](auto p_) {
-        constexpr int p = decltype(p_)::value;
-        if constexpr (TB) {
-          gf_static_for<FN / 4>([&](auto j_) {
-            constexpr int j = decltype(j_)::value * 4;
-            gf_tr_read4<p * TILE_B * 2 + ks * 64 * BN, BN>(trb + buf * STAGE * 2, j, &b[p][j]);
-          });
-        } else {
+  Frag a[PL][FM], b[PL][FN];
+  const P* ta = lds;
+  const P* tb = lds;
+  // the fragments of 32 of k; those of a transposed A are read four rows of tiles at a time, before their products
+  auto read = [&](auto ks_, int at) {
+    constexpr int ks = decltype(ks_)::value;
+    gf_static_for<PL>([&](auto p_) {
+      constexpr int p = decltype(p_)::value;
+      if constexpr (TB) {
+        gf_static_for<FN / 4>([&](auto j_) {
+          constexpr int j = decltype(j_)::value * 4;
+          gf_tr_read4<p * TILE_B * 2 + ks * 64 * BN, BN>(trb + at * STAGE * 2, j, &b[p][j]);
+        });
+      } else {
 #pragma unroll
-          for (int j = 0; j < FN; ++j) b[p][j] = gf_frag<Frag, BK>(tb + p * TILE_B, (wn * FN + j) * 16, ks, lane);
-        }
-        if constexpr (!TA) {
+        for (int j = 0; j < FN; ++j) b[p][j] = gf_frag<Frag, BK>(tb + p * TILE_B, (wn * FN + j) * 16, ks, lane);
+      }
+      if constexpr (TA) {
+        gf_static_for<FM / 4>([&](auto i_) {
+          constexpr int i0 = decltype(i_)::value * 4;
+          gf_tr_read4<p * TILE_A * 2 + ks * 64 * BM, BM>(tra + at * STAGE * 2, i0, &a[p][i0]);
+        });
+      } else {
 #pragma unroll
-          for (int i = 0; i < FM; ++i) a[p][i] = gf_frag<Frag, BK>(ta + p * TILE_A, (wm * FM + i) * 16, ks, lane);
-        }
-      });
-      gf_static_for<FM / 4>([&](auto i_) {
-        constexpr int i0 = decltype(i_)::value * 4;
-        if constexpr (TA)
-          gf_static_for<PL>([&](auto p_) {
-            constexpr int p = decltype(p_)::value;
-            gf_tr_read4<p * TILE_A * 2 + ks * 64 * BM, BM>(tra + buf * STAGE * 2, i0, &a[p][i0]);
-          });
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int i = i0; i < i0 + 4; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j) {
-            if constexpr (PL == 3) {   // small terms first
-              acc[i][j] = gf_mfma(b[2][j], a[0][i], acc[i][j]);
-              acc[i][j] = gf_mfma(b[0][j], a[2][i], acc[i][j]);
-              acc[i][j] = gf_mfma(b[1][j], a[1][i], acc[i][j]);
-              acc[i][j] = gf_mfma(b[1][j], a[0][i], acc[i][j]);
-              acc[i][j] = gf_mfma(b[0][j], a[1][i], acc[i][j]);
-            }
-            acc[i][j] = gf_mfma(b[0][j], a[0][i], acc[i][j]);
-          }
-        __builtin_amdgcn_s_setprio(0);
-      });
+        for (int i = 0; i < FM; ++i) a[p][i] = gf_frag<Frag, BK>(ta + p * TILE_A, (wm * FM + i) * 16, ks, lane);
+      }
     });
-    if (k0 + BK < k_end) land(buf ^ 1);
+  };
+  auto multiply = [&] {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        if constexpr (PL == 3) {   // small terms first
+          acc[i][j] = gf_mfma(b[2][j], a[0][i], acc[i][j]);
+          acc[i][j] = gf_mfma(b[0][j], a[2][i], acc[i][j]);
+          acc[i][j] = gf_mfma(b[1][j], a[1][i], acc[i][j]);
+          acc[i][j] = gf_mfma(b[1][j], a[0][i], acc[i][j]);
+          acc[i][j] = gf_mfma(b[0][j], a[1][i], acc[i][j]);
+        }
+        acc[i][j] = gf_mfma(b[0][j], a[0][i], acc[i][j]);
+      }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  if constexpr (PHASES) {
+    // Two waves share a SIMD, one of each group.  A step of k is four phases with a barrier behind each: read 32 of k, multiply, read the
+    // other 32, multiply; the second group is one phase behind, so that one group's reads run beside the other's products.  In phases
+    // of the first group, P0 .. P3 of step n: the next tile is asked for at P0 (P1 by the second group), when the buffer's last reader,
+    // the second group's second read, was done at the P3 before; it has to be there at the next P0, so the first group waits for its
+    // part at the end of P3 and the second at the end of its second read, which is P3 too.  Every wave passes the same number of
+    // barriers: one more at the beginning for the second group, one more at the end for the first.
+    const bool second = __builtin_amdgcn_readfirstlane(wave) >= WM * WN / 2;   // (a scalar: a wave branches around a barrier, or not)
+    auto phase_end = [&](bool landed) {
+      // (a fence would wait for the tile that is on its way, too: what has to be waited for is this wave's reads)
+      if (landed) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");
+    };
+    __syncthreads();                                      // the first tile has landed
+    if (second) phase_end(false);
+    for (long k0 = k_begin; k0 < k_end; k0 += BK, buf ^= 1) {
+      ta = lds + buf * STAGE;
+      tb = ta + PL * TILE_A;
+      if (k0 + BK < k_end) stage(buf ^ 1, k0 + BK);
+      read(std::integral_constant<int, 0>{}, buf);
+      phase_end(false);
+      multiply();
+      phase_end(false);
+      read(std::integral_constant<int, 1>{}, buf);
+      phase_end(second);
+      multiply();
+      phase_end(!second);
+    }
+    if (!second) phase_end(false);
+  } else {
+    for (long k0 = k_begin; k0 < k_end; k0 += BK, buf ^= 1) {
+      __syncthreads();   // this step's tile has landed; the other buffer has been read by all
+      ta = lds + buf * STAGE;
+      tb = ta + PL * TILE_A;
+      if (k0 + BK < k_end) stage(buf ^ 1, k0 + BK);
+      gf_static_for<BK / 32>([&](auto ks) {
+        read(ks, buf);
+        multiply();
+      });
+      if (k0 + BK < k_end) land(buf ^ 1);
+    }
   }
 
   // B is the first operand, so a lane holds four consecutive n of one m
@@ -557,8 +599,8 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
             }
             gs_store<E, 4>((E*)q.C[0] + m * q.ldc + n, q.N - n, h);
             if (q.saved) {
-              gs_store<float, 4>(q.saved + m * q.N + n, q.N - n, g);
-              gs_store<float, 4>(q.saved + (q.M + m) * q.N + n, q.N - n, u);
+              gs_store_past<float, 4>(q.saved + m * q.N + n, q.N - n, g);
+              gs_store_past<float, 4>(q.saved + (q.M + m) * q.N + n, q.N - n, u);
             }
           }
         }

@@ -63,4 +63,19 @@ __device__ __forceinline__ void gs_store(E* __restrict__ p, long n, const float*
   }
 }
 
+// the same past the caches, for what is read again only after more than they hold
+template <typename E, int N>
+__device__ __forceinline__ void gs_store_past(E* __restrict__ p, long n, const float* __restrict__ v) {
+  if (n >= N) {
+    typename GsVec<E, N>::type r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = (E)v[i];
+    __builtin_nontemporal_store(r, (typename GsVec<E, N>::type*)p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) p[i] = (E)v[i];
+  }
+}
+
 static inline int gs_type_bytes(int t) { return t == GS_TYPE_F32 ? 4 : (t == GS_TYPE_F16 || t == GS_TYPE_BF16 ? 2 : 0); }
