@@ -53,6 +53,10 @@ __global__ __launch_bounds__(256) void gs_embedding_fwd_kernel(const typename Gs
 //                cut into spans with a workgroup each, whose sums gs_embedding_join adds in the spans' order.
 constexpr int EM_TILE = 4096;      // ids per workgroup of the sort: four a thread, all loaded at once
 constexpr int EM_SPAN = 256;       // tokens of a bucket per workgroup
+// Tiles up to which the sort's workgroups each add up all tiles' counts; beyond, a launch of its own makes prefix sums of them, since the
+// adding grows with the square of the tokens (32000 rows of 16, fp32: 140 000 tokens 32 us either way, 1 000 000 100 against 92,
+// 4 000 000 490 against 307).
+constexpr int EM_SCAN = 64;
 constexpr int EM_MAX_BUCKETS = 2048;
 constexpr int EM_MAX_R = 1024;     // rows of a bucket at most
 constexpr long EM_MAX_V = (long)EM_MAX_R * EM_MAX_BUCKETS;
@@ -82,7 +86,7 @@ EmbPlan emb_plan(long n, long V, int F) {
   size_t o = 0;
   auto take = [&](size_t bytes) { size_t at = o; o += (bytes + 255) / 256 * 256; return at; };
   p.nbp = (p.nb + 7) / 8 * 8;
-  p.cnt = take((size_t)p.tiles * p.nbp * 4);
+  p.cnt = take((size_t)(p.tiles + 1) * p.nbp * 4);
   p.start = take((size_t)(p.nb + 1) * 4);
   p.xs = take((size_t)(p.nb + 1) * 4);
   p.owner = take((size_t)p.extra * 4);
@@ -131,6 +135,38 @@ __global__ __launch_bounds__(1024) void gs_embedding_count_kernel(const int* __r
   for (int b = threadIdx.x; b < nbp; b += 1024) cnt[(long)blockIdx.x * nbp + b] = h[b];
 }
 
+// cnt[tile][bucket] becomes the count of the tiles before, cnt[tiles][bucket] that of all.  A workgroup takes 64 buckets, its waves
+// consecutive parts of the tiles: every part is summed, then walked again from the sum of the parts before it.
+__global__ __launch_bounds__(1024) void gs_embedding_scan_kernel(int* __restrict__ cnt, int tiles, int nbp) {
+  __shared__ int sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.x * 64 + lane;
+  const int per = (tiles + 15) / 16, t0 = min(wave * per, tiles), t1 = min(t0 + per, tiles);
+  const bool on = b < nbp;
+  int* c = cnt + b;
+  int sum = 0;
+  if (on) {
+#pragma unroll 8
+    for (int t = t0; t < t1; ++t) sum += c[(long)t * nbp];
+  }
+  sums[wave][lane] = sum;
+  __syncthreads();
+  if (!on) return;
+  int run = 0;
+  for (int w = 0; w < wave; ++w) run += sums[w][lane];
+  for (int t = t0; t < t1; t += 8) {
+    int v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c[(long)min(t + j, t1 - 1) * nbp];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (t + j < t1) {
+        c[(long)(t + j) * nbp] = run;
+        run += v[j];
+      }
+  }
+  if (wave == 15) c[(long)tiles * nbp] = run;
+}
+
 // Stable: a tile's place in a bucket follows from the counts of the tiles before it, a wave's from those of the waves before it, a
 // lane's from the lanes before it.  start[b]: where bucket b begins in the list; xs[b]: further spans of the buckets before b; owner[e]:
 // the bucket of further span e, or -1.
@@ -151,7 +187,14 @@ __global__ __launch_bounds__(1024) void gs_embedding_place_kernel(const int* __r
     id[i] = t0 + i * 64 < n ? emb_row(ids[t0 + i * 64], id0, V) : -1;
   }
   int before[PER] = {}, all[PER] = {};
-  if (tid * PER < nbp) {
+  if (tid * PER < nbp && tiles > EM_SCAN) {
+    const int2* c = (const int2*)cnt + tid;
+    const int2 u = c[(long)blockIdx.x * (nbp / 2)], v = c[(long)tiles * (nbp / 2)];
+    before[0] = u.x;
+    before[1] = u.y;
+    all[0] = v.x;
+    all[1] = v.y;
+  } else if (tid * PER < nbp) {
     const int2* c = (const int2*)cnt + tid;
 #pragma unroll 8
     for (int t = 0; t < tiles; ++t) {
@@ -570,6 +613,10 @@ int emb_bwd_rows(const void* dout, long ldd, const int* ids, long n, long id0, l
     while ((1 << bits) < p.nb) ++bits;
     gs_embedding_count_kernel<<<dim3((unsigned)p.tiles), dim3(1024), 0, s>>>(ids, n, id0, V, a.rshift, p.nbp, cnt);
     GS_LAUNCH_CHECK();
+    if (p.tiles > EM_SCAN) {
+      gs_embedding_scan_kernel<<<dim3((unsigned)gs_cdiv(p.nbp, 64)), dim3(1024), 0, s>>>(cnt, p.tiles, p.nbp);
+      GS_LAUNCH_CHECK();
+    }
     gs_embedding_place_kernel<<<dim3((unsigned)p.tiles), dim3(1024), 0, s>>>(ids, n, id0, V, a.rshift, p.nb, p.nbp, bits, cnt, p.tiles, start, xs, owner, p.extra, list);
     GS_LAUNCH_CHECK();
     a.start = start; a.xs = xs; a.owner = owner; a.list = list; a.ptrs = (int*)(scratch + p.ptrs); a.part = (float*)(scratch + p.part);
