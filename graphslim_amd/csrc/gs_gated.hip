@@ -154,8 +154,17 @@ __global__ __launch_bounds__(256) void gs_gated_slopes_kernel(int act, const typ
   if (m < M && f < F) {
     float d[8], g[8], u[8];
     gs_load<typename GsElt<T>::type, 8>(dh + m * lddh + f, F - f, 0.f, d);
-    gs_load<float, 8>(saved + m * F + f, F - f, 0.f, g);
-    gs_load<float, 8>(saved + (M + m) * F + f, F - f, 0.f, u);
+    if (f + 8 <= F) {
+      const auto x = gs_load_past<float, 8>(saved + m * F + f), y = gs_load_past<float, 8>(saved + (M + m) * F + f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        g[j] = x[j];
+        u[j] = y[j];
+      }
+    } else {
+      gs_load<float, 8>(saved + m * F + f, F - f, 0.f, g);
+      gs_load<float, 8>(saved + (M + m) * F + f, F - f, 0.f, u);
+    }
     gf_with_act(act, [&](auto ac) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {

@@ -78,4 +78,10 @@ __device__ __forceinline__ void gs_store_past(E* __restrict__ p, long n, const f
   }
 }
 
+// N elements that are read once, past the caches
+template <typename E, int N>
+__device__ __forceinline__ typename GsVec<E, N>::type gs_load_past(const E* __restrict__ p) {
+  return __builtin_nontemporal_load((const typename GsVec<E, N>::type*)p);
+}
+
 static inline int gs_type_bytes(int t) { return t == GS_TYPE_F32 ? 4 : (t == GS_TYPE_F16 || t == GS_TYPE_BF16 ? 2 : 0); }
