@@ -235,10 +235,10 @@ def lib():
     L.gs_embedding_bwd_scratch_bytes.argtypes = [l, l, i]
     L.gs_embedding_bwd_scratch_bytes.restype = C.c_size_t
     L.gs_embedding_bwd.argtypes = [vp, l, i, vp, l, l, i, f, i, vp, l, i, vp, vp]
-    L.gs_gated_fwd_scratch_bytes.argtypes = [l, l, l, i]
+    L.gs_gated_fwd_scratch_bytes.argtypes = [l, l, l, i, i]
     L.gs_gated_fwd_scratch_bytes.restype = C.c_size_t
     L.gs_gated_fwd.argtypes = [vp, l, vp, vp, l, i, l, l, l, i, vp, l, vp, vp, vp]
-    L.gs_gated_bwd_scratch_bytes.argtypes = [l, l, l, i]
+    L.gs_gated_bwd_scratch_bytes.argtypes = [l, l, l, i, i]
     L.gs_gated_bwd_scratch_bytes.restype = C.c_size_t
     L.gs_gated_bwd.argtypes = [vp, l, vp, l, vp, vp, l, vp, i, l, l, l, i, vp, l, vp, vp, l, vp, vp]
     L.gs_distill_fwd.argtypes = [vp, l, i, l, i, vp, vp, i, f, vp, vp, vp]

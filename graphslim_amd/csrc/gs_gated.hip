@@ -6,7 +6,7 @@
 // (x = h + m + l, 8 + 8 + 8 significant bits), and six products of parts make one product: what they leave out is below 2^-23 of it.
 // (Parts have bf16's smallest step, 2^-133: a value is represented to 2^-134 or to 24 bits, whichever is coarser.)
 // The parts of fp32 operands, and [dg | du], are laid out in the caller's scratch first, rows padded with zeros to a multiple of 64;
-// 16-bit operands are read where they are, whatever their alignment and width.
+// so are 16-bit operands whose rows do not consist of whole, aligned chunks of 16 bytes, unless it is cheaper to read them as they are.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -268,7 +268,7 @@ struct GatedGemm {
   const void* B[2];     // gated: gate and up projection; n contiguous: rows of k below `kb` in the first, the others in the second
   long ldb, plane_b;
   long M, N, K;         // K a multiple of 64
-  long k_end;           // RAW: elements that a row of k has (A's and B's)
+  long k_end;           // k contiguous in both: elements that a row of k has (K or less; RAW: 8 or more)
   long bcols;           // n contiguous: columns that rows of B have (a multiple of 8, N or more)
   long kb, brows;       // n contiguous: rows that B[0] stands for (a multiple of 64), and rows that each of B has; behind them A is 0
   void* C[2];           // plain form: rows [0, rows) go to C[0], rows [rows1, rows1 + rows) to C[1], others nowhere
@@ -358,9 +358,11 @@ __device__ __forceinline__ void gf_tr_read4(unsigned addr, int first, Frag* x) {
   x[3] = __builtin_bit_cast(Frag, __builtin_shufflevector(l3, h3, 0, 1, 2, 3));
 }
 
+__device__ const int gf_zeros[4] = {};   // a chunk behind the end of a row
+
 // T: type of the outputs (and of 16-bit operands), PL: parts, WM x WN waves of (16 FM) x (16 FN) results.  TA, TB: the operand's other
-// index is contiguous, not k.  RAW: x and the weights are read where they are though their rows begin at any element or end inside a
-// step of k: through registers, with zeros behind a row's end.  GATED: rows of B alternate between gate and up every 16, so that a lane holds both sums of its outputs
+// index is contiguous, not k.  RAW: x and the weights are read where they are though their rows begin or end inside a 16-byte chunk:
+// through registers, with zeros behind a row's end.  GATED: rows of B alternate between gate and up every 16, so that a lane holds both sums of its outputs
 // and the activation is applied in registers.
 template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED>
 __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, unsigned slice, char* smem) {
@@ -386,43 +388,33 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
 
   const P* srcA[ITA];
   int colA[ITA];
-  long colB[ITB];       // of a chunk in its row: of k, or of n
+  int colB[ITB];        // of a chunk in its row
   long srcB[ITB], endB[ITB];   // offsets from B's base; from that of the step with B's last rows, where they are fewer than BK
 #pragma unroll
   for (int i = 0; i < ITA; ++i) {
     const int s = i * NT + tid, r = s / CA, c = (s % CA) ^ gf_swz<TA, BK>(r);
     colA[i] = c * 8;
-    srcA[i] = TA ? A + r * q.lda + min(m0 + c * 8, q.M - 8) : A + min(m0 + r, q.M - 1) * q.lda + (RAW && !TB ? 0 : c * 8);
+    srcA[i] = TA ? A + r * q.lda + min(m0 + c * 8, q.M - 8) : A + min(m0 + r, q.M - 1) * q.lda + (RAW ? 0 : c * 8);
   }
 #pragma unroll
   for (int i = 0; i < ITB; ++i) {
     const int s = i * NT + tid, r = s / CB, c = (s % CB) ^ gf_swz<TB, BK>(r);
     const long n = GATED ? n0 + (r >> 5) * 16 + (r & 15) : n0 + r;
     const P* base = (const P*)q.B[GATED ? (r >> 4) & 1 : 0];
-    // (RAW: offsets of rows, the column comes when they are read)
-    const long col = RAW ? n0 + c * 8 : min(n0 + c * 8, q.bcols - 8), in_row = RAW ? 0 : (TB ? col : c * 8);
-    colB[i] = TB ? col : c * 8;
+    const long in_row = TB ? min(n0 + c * 8, q.bcols - 8) : (RAW ? 0 : c * 8);   // (RAW, k contiguous: the column comes with the step)
+    colB[i] = c * 8;
     srcB[i] = (TB ? r * q.ldb : (long)(base + min(n, q.N - 1) * q.ldb - (const P*)q.B[0])) + in_row;
     endB[i] = TB ? min((long)r, (q.brows - 1) % BK) * q.ldb + in_row : 0;
   }
+  static_assert(!RAW || (!TA && !TB), "rows of k");
   // RAW: the chunks of the next tile on their way through registers.  A chunk that reaches behind its row's end is loaded from the
-  // row's last 8 elements and shifted down when it goes to LDS, zeros behind (rows of fewer than 8 elements are taken one by one).
+  // row's last 8 elements and shifted down when it goes to LDS, zeros behind.
   typedef typename GsVec<P, 8>::type Chunk;
-  constexpr bool RAW_A = RAW && !TA && !TB;                        // (behind TB, A is the laid-out [dg | du])
-  Chunk ra[RAW_A ? ITA : 1], rb[RAW ? ITB : 1];
-  const long row_end = TB ? q.bcols : q.k_end;                     // of a row that is read raw
-  const bool narrow = row_end < 8;
+  Chunk ra[RAW ? ITA : 1], rb[RAW ? ITB : 1];
   long k_raw = 0;                                                  // the step that is on its way
-  auto raw_load = [&](const P* row, long at) {
-    if (!narrow) return *(const Chunk*)(row + min(at, row_end - 8));
-    Chunk v;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = at + e < row_end ? row[at + e] : (P)0.f;
-    return v;
-  };
   auto raw_shift = [&](Chunk v, long at) {
-    if (narrow || at <= row_end - 8) return v;
-    const int by = (int)(at - (row_end - 8));
+    if (at <= q.k_end - 8) return v;
+    const int by = (int)(at - (q.k_end - 8));
     unsigned __int128 x = __builtin_bit_cast(unsigned __int128, v);
     x = by >= 8 ? (unsigned __int128)0 : x >> (16 * by);
     return __builtin_bit_cast(Chunk, x);
@@ -438,25 +430,38 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
       end = kk + BK > q.brows;
     }
     k_raw = k0;
-    if constexpr (RAW_A) {
+    if constexpr (RAW) {
+      const long last = q.k_end - 8 - k0;                          // (of the step's elements, where its last chunks would pass the end)
 #pragma unroll
-      for (int i = 0; i < ITA; ++i) ra[i] = raw_load(srcA[i], k0 + colA[i]);
+      for (int i = 0; i < ITA; ++i) ra[i] = *(const Chunk*)(srcA[i] + (k0 + min((long)colA[i], last)));
 #pragma unroll
-      for (int i = 0; i < ITB; ++i) rb[i] = raw_load((const P*)q.B[0] + srcB[i], k0 + colB[i]);
+      for (int i = 0; i < ITB; ++i) rb[i] = *(const Chunk*)((const P*)q.B[0] + srcB[i] + (k0 + min((long)colB[i], last)));
       return;
+    }
+    if constexpr (PL == 1 && !TA && !TB) {
+      if (k0 + BK > q.k_end) {
+        // The last step: from chunks behind the end of a row zeros are read.  (The assembly keeps this a branch; selected address by
+        // address in every step it costs a tenth of the whole, 8192 x 2048 x 8192 bf16 500 us against 454.)
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < ITA; ++i)
+          if (k0 + colA[i] >= q.k_end) srcA[i] = (const P*)gf_zeros - k0;
+#pragma unroll
+        for (int i = 0; i < ITB; ++i)
+          if (k0 + colB[i] >= q.k_end) srcB[i] = (const P*)gf_zeros - b0;
+      }
     }
 #pragma unroll
     for (int p = 0; p < PL; ++p) {
 #pragma unroll
-      for (int i = 0; i < ITA; ++i)
-        __builtin_amdgcn_global_load_lds((gbl_ptr)(srcA[i] + p * q.plane_a + (TA ? k0 * q.lda : k0)),
-                                         (lds_ptr)(base + p * TILE_A + (i * NT + wave * 64) * 8), 16, 0, 0);
+      for (int i = 0; i < ITA; ++i) {
+        const P* at = srcA[i] + p * q.plane_a + (TA ? k0 * q.lda : k0);
+        __builtin_amdgcn_global_load_lds((gbl_ptr)at, (lds_ptr)(base + p * TILE_A + (i * NT + wave * 64) * 8), 16, 0, 0);
+      }
 #pragma unroll
       for (int i = 0; i < ITB; ++i) {
-        const long off = TB && end ? endB[i] : srcB[i];
-        if constexpr (RAW) rb[i] = raw_load(b0 + off, colB[i]);
-        else
-          __builtin_amdgcn_global_load_lds((gbl_ptr)(b0 + p * q.plane_b + off), (lds_ptr)(base + PL * TILE_A + p * TILE_B + (i * NT + wave * 64) * 8), 16, 0, 0);
+        const P* at = b0 + p * q.plane_b + (TB && end ? endB[i] : srcB[i]);
+        __builtin_amdgcn_global_load_lds((gbl_ptr)at, (lds_ptr)(base + PL * TILE_A + p * TILE_B + (i * NT + wave * 64) * 8), 16, 0, 0);
       }
     }
   };
@@ -464,14 +469,11 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
     typedef P Whole __attribute__((ext_vector_type(8)));
     P* base = lds + buf * STAGE;
     if constexpr (RAW) {
-      const bool ends = TB ? n0 + BN > row_end : k_raw + BK > row_end;   // (the whole workgroup's)
-      if constexpr (RAW_A) {
+      const bool ends = k_raw + BK > q.k_end;                      // (the whole workgroup's)
 #pragma unroll
-        for (int i = 0; i < ITA; ++i) *(Whole*)(base + (i * NT + tid) * 8) = ends ? raw_shift(ra[i], k_raw + colA[i]) : ra[i];
-      }
+      for (int i = 0; i < ITA; ++i) *(Whole*)(base + (i * NT + tid) * 8) = ends ? raw_shift(ra[i], k_raw + colA[i]) : ra[i];
 #pragma unroll
-      for (int i = 0; i < ITB; ++i)
-        *(Whole*)(base + TILE_A + (i * NT + tid) * 8) = ends ? raw_shift(rb[i], TB ? colB[i] : k_raw + colB[i]) : rb[i];
+      for (int i = 0; i < ITB; ++i) *(Whole*)(base + TILE_A + (i * NT + tid) * 8) = ends ? raw_shift(rb[i], k_raw + colB[i]) : rb[i];
     }
   };
 
@@ -644,14 +646,14 @@ __global__ __launch_bounds__(WM * WN * 64) void gs_gated_gemm_kernel(GatedGemm q
 }
 
 // dx and dW in one launch, where neither fills the chip alone: blocks [0, a_blocks) are dx's tiles and slices, the others dW's.
-template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool RAW>
+template <int T, int PL, int WM, int WN, int FM, int FN, int BK>
 __global__ __launch_bounds__(WM * WN * 64) void gs_gated_pair_kernel(GatedGemm a, unsigned a_tiles, unsigned a_blocks, GatedGemm b, unsigned b_tiles) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   if (blockIdx.x < a_blocks) {
-    gf_product<T, PL, WM, WN, FM, FN, BK, false, true, RAW, false>(a, blockIdx.x % a_tiles, blockIdx.x / a_tiles, smem);
+    gf_product<T, PL, WM, WN, FM, FN, BK, false, true, false, false>(a, blockIdx.x % a_tiles, blockIdx.x / a_tiles, smem);
   } else {
     const unsigned i = blockIdx.x - a_blocks;
-    gf_product<T, PL, WM, WN, FM, FN, BK, true, true, RAW, false>(b, i % b_tiles, i / b_tiles, smem);
+    gf_product<T, PL, WM, WN, FM, FN, BK, true, true, false, false>(b, i % b_tiles, i / b_tiles, smem);
   }
 }
 
@@ -775,15 +777,23 @@ GatedPair gf_pair_of(long M, long D, long Fp, long Mp, int pl) {
 // Where the laid-out operands lie in the scratch (elements of 2 bytes).  The sizes go by the shapes and the type alone.
 struct GatedPlan {
   int pl;
+  bool pack;                          // x, Wg and Wu are laid out in the scratch (both passes)
   long Dp, Fp, Mp;
-  size_t x, wg, wu, fwd;              // fp32: the parts of x, Wg, Wu with padded rows (both passes)
+  size_t x, wg, wu, fwd;              // their places, with padded rows
   size_t dgu, bwd;                    // backward: [dg | du]
   size_t part_fwd, part_bwd;          // partial sums of products that are cut along k, behind the operands
   GatedSplit split;                   // of the forward product
   GatedPair pair;                     // of the backward ones
 };
 
-GatedPlan gf_plan(long M, long D, long F, int type, bool bwd) {
+// Whether a forward call lays out 16-bit operands whose rows do not consist of whole, aligned chunks, as every backward call does, rather
+// than read them through registers: laying out takes a launch and its traffic, reading so 1.6 ns more for a million products (fp16:
+// 300 x 2047 x 8192 read 54 us, laid out 81; 8000 x 301 x 500 21.5 and 24.7; 2000 x 1433 x 4096 72 and 69; 4000 x 2047 x 8192 377 and 307).
+inline bool gf_lay_out(long M, long D, long F) {
+  return D < 8 || 1.6e-9 * M * D * F > 4 + 0.9e-6 * (M + 2 * F) * D;
+}
+
+GatedPlan gf_plan(long M, long D, long F, int type, bool plain, bool bwd) {
   GatedPlan p = {};
   p.pl = type == GS_TYPE_F32 ? 3 : 1;
   p.Dp = gf_up(D);
@@ -791,7 +801,8 @@ GatedPlan gf_plan(long M, long D, long F, int type, bool bwd) {
   p.Mp = gf_up(M);
   size_t o = 0;
   auto take = [&](size_t n) { size_t at = o; o += n * p.pl; return at; };
-  if (p.pl > 1) {
+  p.pack = p.pl > 1 || (!plain && (bwd || gf_lay_out(M, D, F)));
+  if (p.pack) {
     p.x = take((size_t)p.Mp * p.Dp);
     p.wg = take((size_t)p.Fp * p.Dp);
     p.wu = take((size_t)p.Fp * p.Dp);
@@ -862,19 +873,20 @@ int gf_gemm(const GatedGemm& q, const GatedSplit& sp, bool raw, float* part, hip
   if constexpr (PL == 3) {
     if (sp.big) return gf_tile<T, PL, 4, 2, 4, 4, 32, TA, TB, false, GATED>(q, sp, part, s);
     return gf_tile<T, PL, 2, 2, 4, 4, 32, TA, TB, false, GATED>(q, sp, part, s);
-  } else if (raw) {
-    if (sp.big) return gf_tile<T, PL, 2, 4, 8, 4, 64, TA, TB, true, GATED>(q, sp, part, s);
-    return gf_tile<T, PL, 2, 2, 4, 4, 64, TA, TB, true, GATED>(q, sp, part, s);
   } else {
+    if constexpr (!TA && !TB) {
+      if (raw) return sp.big ? gf_tile<T, PL, 2, 4, 8, 4, 64, TA, TB, true, GATED>(q, sp, part, s)
+                             : gf_tile<T, PL, 2, 2, 4, 4, 64, TA, TB, true, GATED>(q, sp, part, s);
+    }
     if (sp.big) return gf_tile<T, PL, 2, 4, 8, 4, 64, TA, TB, false, GATED>(q, sp, part, s);
     return gf_tile<T, PL, 2, 2, 4, 4, 64, TA, TB, false, GATED>(q, sp, part, s);
   }
 }
 
-template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool RAW>
+template <int T, int PL, int WM, int WN, int FM, int FN, int BK>
 int gf_pair_tile(GatedGemm a, GatedGemm b, const GatedPair& p, float* part, hipStream_t s) {
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16, LDS = 2 * PL * (WM * FM + WN * FN) * 16 * BK * 2;
-  auto kern = gs_gated_pair_kernel<T, PL, WM, WN, FM, FN, BK, RAW>;
+  auto kern = gs_gated_pair_kernel<T, PL, WM, WN, FM, FN, BK>;
   static std::atomic<unsigned long long> known{0};
   GS_TRY(gf_lds(kern, LDS, known));
   long ta, tb;
@@ -892,21 +904,23 @@ int gf_pair_tile(GatedGemm a, GatedGemm b, const GatedPair& p, float* part, hipS
 }
 
 template <int T, int PL>
-int gf_pair(const GatedGemm& a, const GatedGemm& b, const GatedPair& p, bool raw, float* part, hipStream_t s) {
+int gf_pair(const GatedGemm& a, const GatedGemm& b, const GatedPair& p, float* part, hipStream_t s) {
   if constexpr (PL == 3) {
-    if (p.dx.big) return gf_pair_tile<T, PL, 4, 2, 4, 4, 32, false>(a, b, p, part, s);
-    return gf_pair_tile<T, PL, 2, 2, 4, 4, 32, false>(a, b, p, part, s);
-  } else if (raw) {
-    if (p.dx.big) return gf_pair_tile<T, PL, 2, 4, 8, 4, 64, true>(a, b, p, part, s);
-    return gf_pair_tile<T, PL, 2, 2, 4, 4, 64, true>(a, b, p, part, s);
+    if (p.dx.big) return gf_pair_tile<T, PL, 4, 2, 4, 4, 32>(a, b, p, part, s);
+    return gf_pair_tile<T, PL, 2, 2, 4, 4, 32>(a, b, p, part, s);
   } else {
-    if (p.dx.big) return gf_pair_tile<T, PL, 2, 4, 8, 4, 64, false>(a, b, p, part, s);
-    return gf_pair_tile<T, PL, 2, 2, 4, 4, 64, false>(a, b, p, part, s);
+    if (p.dx.big) return gf_pair_tile<T, PL, 2, 4, 8, 4, 64>(a, b, p, part, s);
+    return gf_pair_tile<T, PL, 2, 2, 4, 4, 64>(a, b, p, part, s);
   }
 }
 
-// whether rows of `n` elements with stride ld can be read as they are: in chunks of 16 bytes, whole steps of 64 where k is contiguous
-inline bool gf_plain(const void* p, long ld, long n, int step) { return n % step == 0 && ld % 8 == 0 && ((size_t)p & 15) == 0; }
+// whether rows of `n` 16-bit elements with stride ld consist of whole, aligned chunks of 16 bytes
+inline bool gf_plain(const void* p, long ld, long n) { return n % 8 == 0 && ld % 8 == 0 && ((size_t)p & 15) == 0; }
+
+// whether x and the weights can be read as they are
+inline bool gf_plain(const void* x, long ldx, const void* wg, const void* wu, long ldw, long D) {
+  return gf_plain(x, ldx, D) && gf_plain(wg, ldw, D) && gf_plain(wu, ldw, D);
+}
 
 struct GatedCall {
   const void *x, *wg, *wu, *dh;
@@ -929,7 +943,7 @@ template <int T, int PL>
 int gf_operands(const GatedCall& c, const GatedPlan& p, GatedOperands* o, hipStream_t s) {
   typedef typename GfPlane<T, PL>::type P;
   *o = {c.x, {c.wg, c.wu}, c.ldx, c.ldw, 0, 0};
-  if constexpr (PL > 1) {
+  if (p.pack) {
     P* sc = (P*)c.scratch;
     *o = {sc + p.x, {sc + p.wg, sc + p.wu}, p.Dp, p.Dp, p.Mp * p.Dp, p.Fp * p.Dp};
     const long bx = (p.Mp * (p.Dp / 8) + 255) / 256, bw = (p.Fp * (p.Dp / 8) + 255) / 256;
@@ -963,17 +977,18 @@ int gf_fwd(const GatedCall& c, hipStream_t s) {
     if (c.M == 2) return gf_rows<T, 2>(c, s);
     return c.M <= 4 ? gf_rows<T, 4>(c, s) : gf_rows<T, 8>(c, s);
   }
-  const GatedPlan p = gf_plan(c.M, c.D, c.F, T, false);
+  const bool plain = gf_plain(c.x, c.ldx, c.wg, c.wu, c.ldw, c.D);
+  const GatedPlan p = gf_plan(c.M, c.D, c.F, T, plain, false);
   GatedOperands o;
   GS_TRY((gf_operands<T, PL>(c, p, &o, s)));
-  const bool raw = PL == 1 && !(gf_plain(c.x, c.ldx, c.D, GF_PAD) && gf_plain(c.wg, c.ldw, c.D, GF_PAD) && gf_plain(c.wu, c.ldw, c.D, GF_PAD));
+  const bool raw = !p.pack && !plain;
   GatedGemm q = {};
   q.A = o.x; q.lda = o.ldx; q.plane_a = o.plane_x;
   q.B[0] = o.w[0]; q.B[1] = o.w[1]; q.ldb = o.ldw; q.plane_b = o.plane_w;
   q.M = c.M; q.N = c.F; q.K = p.Dp;
   q.C[0] = c.h; q.ldc = c.ldh;
   q.saved = c.saved; q.act = c.act;
-  q.k_end = c.D;
+  q.k_end = p.pack ? p.Dp : c.D;
   return gf_gemm<T, PL, false, false, true>(q, p.split, raw, (float*)((P*)c.scratch + p.part_fwd), s);
 }
 
@@ -981,7 +996,7 @@ template <int T, int PL>
 int gf_bwd(const GatedCall& c, hipStream_t s) {
   typedef typename GsElt<T>::type E;
   typedef typename GfPlane<T, PL>::type P;
-  const GatedPlan p = gf_plan(c.M, c.D, c.F, T, true);
+  const GatedPlan p = gf_plan(c.M, c.D, c.F, T, gf_plain(c.x, c.ldx, c.wg, c.wu, c.ldw, c.D), true);
   P* dgu = (P*)c.scratch + p.dgu;
   const long plane = p.Mp * 2 * p.Fp, blocks = (p.Mp * (p.Fp / 8) + 255) / 256;
   if (blocks > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated_bwd: %ld x %ld is beyond one launch", c.M, c.F);
@@ -993,20 +1008,19 @@ int gf_bwd(const GatedCall& c, hipStream_t s) {
   GatedGemm q = {};
   q.A = dgu; q.lda = 2 * p.Fp; q.plane_a = plane;
   q.B[0] = o.w[0]; q.B[1] = o.w[1]; q.ldb = o.ldw; q.plane_b = o.plane_w;
-  q.M = c.M; q.K = 2 * p.Fp; q.kb = p.Fp; q.brows = o.plane_w ? p.Fp : c.F;
-  q.N = c.D; q.bcols = o.plane_w ? p.Dp : c.D;
+  q.M = c.M; q.K = 2 * p.Fp; q.kb = p.Fp; q.brows = p.pack ? p.Fp : c.F;
+  q.N = c.D; q.bcols = p.pack ? p.Dp : c.D;
   q.C[0] = c.dx; q.ldc = c.lddx; q.rows = q.rows1 = c.M;
   float* part = (float*)((P*)c.scratch + p.part_bwd);
-  const bool raw_w = PL == 1 && !(gf_plain(c.wg, c.ldw, c.D, 8) && gf_plain(c.wu, c.ldw, c.D, 8)), raw_x = PL == 1 && !gf_plain(c.x, c.ldx, c.D, 8);
   // dWg, dWu: k runs over the tokens
   GatedGemm w = q;
   w.B[0] = o.x; w.ldb = o.ldx; w.plane_b = o.plane_x;
-  w.M = 2 * p.Fp; w.K = p.Mp; w.kb = p.Mp; w.brows = o.plane_x ? p.Mp : c.M;
-  w.bcols = o.plane_x ? p.Dp : c.D;
+  w.M = 2 * p.Fp; w.K = p.Mp; w.kb = p.Mp; w.brows = p.pack ? p.Mp : c.M;
+  w.bcols = p.pack ? p.Dp : c.D;
   w.C[0] = c.dwg; w.C[1] = c.dwu; w.ldc = c.lddw; w.rows = c.F; w.rows1 = p.Fp;
-  if (p.pair.together) return gf_pair<T, PL>(q, w, p.pair, raw_w || raw_x, part, s);
-  GS_TRY((gf_gemm<T, PL, false, true, false>(q, p.pair.dx, raw_w, part, s)));
-  return gf_gemm<T, PL, true, true, false>(w, p.pair.dw, raw_x, part, s);
+  if (p.pair.together) return gf_pair<T, PL>(q, w, p.pair, part, s);
+  GS_TRY((gf_gemm<T, PL, false, true, false>(q, p.pair.dx, false, part, s)));
+  return gf_gemm<T, PL, true, true, false>(w, p.pair.dw, false, part, s);
 }
 
 // dW = 0 where there are no tokens
@@ -1050,14 +1064,14 @@ int gf_run(const GatedCall& c, int type, bool bwd, hipStream_t s) {
 
 }  // namespace
 
-extern "C" size_t gs_gated_fwd_scratch_bytes(long M, long D, long F, int type) {
+extern "C" size_t gs_gated_fwd_scratch_bytes(long M, long D, long F, int type, int plain) {
   if (M < 1 || D < 1 || F < 1 || !gs_type_bytes(type)) return 0;
-  return gf_few(M, type) ? 0 : gf_plan(M, D, F, type, false).fwd * 2;
+  return gf_few(M, type) ? 0 : gf_plan(M, D, F, type, plain != 0, false).fwd * 2;
 }
 
-extern "C" size_t gs_gated_bwd_scratch_bytes(long M, long D, long F, int type) {
+extern "C" size_t gs_gated_bwd_scratch_bytes(long M, long D, long F, int type, int plain) {
   if (M < 1 || D < 1 || F < 1 || !gs_type_bytes(type)) return 0;
-  return gf_plan(M, D, F, type, true).bwd * 2;
+  return gf_plan(M, D, F, type, plain != 0, true).bwd * 2;
 }
 
 extern "C" int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, long ldw, int type, long M, long D, long F, int act,
@@ -1068,7 +1082,7 @@ extern "C" int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const v
   GS_TRY(gf_check("gs_gated_fwd", c, type));
   if (ldh < F) GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: a row stride is below the width %ld", F);
   if (M == 0) return GS_OK;
-  if (!x || !w_gate || !w_up || !h || (!scratch && gs_gated_fwd_scratch_bytes(M, D, F, type) > 0))
+  if (!x || !w_gate || !w_up || !h || (!scratch && gs_gated_fwd_scratch_bytes(M, D, F, type, gf_plain(x, ldx, w_gate, w_up, ldw, D)) > 0))
     GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: null pointer");
   if ((size_t)scratch & 15) GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: the scratch is not 16-byte aligned");
   return gf_run(c, type, false, (hipStream_t)stream);

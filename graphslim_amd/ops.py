@@ -187,6 +187,11 @@ def _gated_args(x, w_gate, w_up, act):
     return dev, ldx, ldw, M, D, F
 
 
+def _plain(ldx, ldw, D, *matrices):
+    """Whether rows of D elements consist of whole, aligned chunks of 16 bytes (the library asks it of 16-bit types)."""
+    return (D | ldx | ldw) % 8 == 0 and not any(t.data_ptr() % 16 for t in matrices)
+
+
 def gated_ffn(x, w_gate, w_up, act="silu", save=False):
     """act(x w_gate^T) * (x w_up^T) for x [M, D] and w_gate, w_up [F, D].  save=True returns (h, saved): `saved` holds the two
     projections, [2, M, F] in fp32, for `gated_ffn_grad`."""
@@ -194,7 +199,7 @@ def gated_ffn(x, w_gate, w_up, act="silu", save=False):
     h = torch.empty(M, F, dtype=x.dtype, device=dev)
     saved = torch.empty(2, M, F, dtype=torch.float32, device=dev) if save else None
     L = _lib.lib()
-    scratch = _scratch(L.gs_gated_fwd_scratch_bytes(M, D, F, TYPES[x.dtype]), dev)
+    scratch = _scratch(L.gs_gated_fwd_scratch_bytes(M, D, F, TYPES[x.dtype], _plain(ldx, ldw, D, x, w_gate, w_up)), dev)
     _launch(dev, L.gs_gated_fwd, x.data_ptr(), ldx, w_gate.data_ptr(), w_up.data_ptr(), ldw, TYPES[x.dtype], M, D, F, ACTIVATIONS[act],
             h.data_ptr(), F, _ptr(saved), _ptr(scratch))
     return (h, saved) if save else h
@@ -210,7 +215,7 @@ def gated_ffn_grad(d_h, x, w_gate, w_up, saved, act="silu"):
     d_x = torch.empty(M, D, dtype=x.dtype, device=dev)
     d_wg, d_wu = (torch.empty(F, D, dtype=x.dtype, device=dev) for _ in range(2))
     L = _lib.lib()
-    scratch = _scratch(L.gs_gated_bwd_scratch_bytes(M, D, F, TYPES[x.dtype]), dev)
+    scratch = _scratch(L.gs_gated_bwd_scratch_bytes(M, D, F, TYPES[x.dtype], _plain(ldx, ldw, D, x, w_gate, w_up)), dev)
     _launch(dev, L.gs_gated_bwd, d_h.data_ptr(), lddh, x.data_ptr(), ldx, w_gate.data_ptr(), w_up.data_ptr(), ldw, saved.data_ptr(),
             TYPES[x.dtype], M, D, F, ACTIVATIONS[act], d_x.data_ptr(), D, d_wg.data_ptr(), d_wu.data_ptr(), D, _ptr(scratch))
     return d_x, d_wg, d_wu

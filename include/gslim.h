@@ -328,14 +328,16 @@ int gs_embedding_bwd(const void* dout, long ldd, int type, const int* ids, long 
 #define GS_ACT_GELU 1      /* the exact one: x Phi(x) */
 #define GS_ACT_RELU 2
 #define GS_ACT_SIGMOID 3
-size_t gs_gated_fwd_scratch_bytes(long M, long D, long F, int type);
+/* `plain` (16-bit types): whether rows of x, Wg and Wu consist of whole, 16-byte-aligned chunks (D and the strides multiples of 8, the
+ * matrices 16-byte aligned).  The calls find it out by themselves; where they are not, the scratch also takes copies that are. */
+size_t gs_gated_fwd_scratch_bytes(long M, long D, long F, int type, int plain);
 int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, long ldw, int type, long M, long D, long F, int act,
                  void* h, long ldh, float* saved, void* scratch, gs_stream_t stream);
 /* dg = dh * u * act'(g), du = dh * act(g) (rounded to the operands' type: the products take them there); dx = dg Wg + du Wu,
  * dw_gate = dg^T x, dw_up = du^T x.
  * fp32 products of more than a few rows are six products of bf16 parts: as exact as fp32 (parts have a smallest step of 2^-133), but an
  * infinite operand gives NaN where it meets a zero part. */
-size_t gs_gated_bwd_scratch_bytes(long M, long D, long F, int type);
+size_t gs_gated_bwd_scratch_bytes(long M, long D, long F, int type, int plain);
 int gs_gated_bwd(const void* dh, long lddh, const void* x, long ldx, const void* w_gate, const void* w_up, long ldw, const float* saved,
                  int type, long M, long D, long F, int act, void* dx, long lddx, void* dw_gate, void* dw_up, long lddw, void* scratch,
                  gs_stream_t stream);

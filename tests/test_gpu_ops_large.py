@@ -9,13 +9,13 @@ from test_gpu_ops import BF16, DEV, F16, F32, gen, normal, ops, zipf  # noqa: F4
 pytestmark = pytest.mark.gpu
 
 # What each shape is for: the tile of 256 rows in the forward product (fwd), in dx and dW one after the other (dx, dw) or in one launch
-# (pair), cut along k (/) or not; 16-bit widths that are no multiple of 8 are read through registers (raw).
-WIDE_16 = [(6000, 64, 700), (2050, 72, 2050),                       # fwd; fwd raw
-           (6000, 4104, 16), (6000, 4100, 9),                       # dx; dx raw
-           (70, 4104, 8200), (70, 4100, 8200),                      # dw; dw raw
+# (pair), cut along k (/) or not; 16-bit rows that do not consist of whole chunks are laid out first, or read through registers (raw).
+WIDE_16 = [(6000, 64, 700), (2050, 72, 2050), (2000, 75, 2100), (2050, 1035, 2050),   # fwd; rows that end inside a step of k; raw; laid out
+           (6000, 4104, 16), (6000, 4100, 9),                       # dx; laid out
+           (70, 4104, 8200), (70, 4100, 8200),                      # dw; laid out, forward raw and cut
            (700, 4104, 4104),                                       # dx/
-           (1300, 4104, 1032), (1300, 4100, 1027),                  # pair; pair raw
-           (4100, 4104, 9), (70, 2056, 4104), (70, 2060, 4100)]     # pair, dw/; pair, dx/; the same raw
+           (1300, 4104, 1032), (1300, 4100, 1027),                  # pair; laid out, forward raw
+           (4100, 4104, 9), (70, 2056, 4104), (70, 2060, 4100)]     # pair, dw/; pair, dx/; the same laid out
 WIDE_32 = [(3000, 64, 700), (8200, 515, 9),                         # fwd; fwd/
            (3000, 4100, 9), (260, 1032, 8200),                      # dx, dw/; dx/
            (70, 515, 8200), (4100, 4100, 70),                       # dw; dw/

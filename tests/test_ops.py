@@ -125,8 +125,8 @@ def test_c_entry_points_refuse(L):
     assert L.gs_gated_fwd(N, 4, N, N, 4, 0, 2, 4, 6, 0, N, 6, N, N, N) == ARG and b"null" in L.gs_last_error()
     assert L.gs_gated_fwd(N, 4, N, N, 4, 0, 0, 4, 6, 0, N, 6, N, N, N) == 0
     assert L.gs_gated_bwd(N, 6, N, 4, N, N, 4, N, 0, 2, 4, 6, 0, N, 4, N, N, 4, N, N) == ARG
-    assert L.gs_gated_fwd_scratch_bytes(0, 4, 6, 0) == L.gs_gated_bwd_scratch_bytes(0, 4, 6, 1) == 0
-    assert L.gs_gated_fwd_scratch_bytes(-1, 4, 6, 0) == 0 and L.gs_gated_fwd_scratch_bytes(2, 4, 6, 5) == 0
+    assert L.gs_gated_fwd_scratch_bytes(0, 4, 6, 0, 1) == L.gs_gated_bwd_scratch_bytes(0, 4, 6, 1, 1) == 0
+    assert L.gs_gated_fwd_scratch_bytes(-1, 4, 6, 0, 1) == 0 and L.gs_gated_fwd_scratch_bytes(2, 4, 6, 5, 1) == 0
     assert L.gs_distill_fwd(N, 9, 0, 3, 9, N, N, 2, 1.0, N, N, N) == ARG
     buf = 4096                                          # never read: the checks below come first
     assert L.gs_distill_fwd(buf, 9, 0, 3, 9, buf, buf, 1025, 1.0, buf, buf, N) == UNSUPPORTED
@@ -145,12 +145,16 @@ def test_scratch_sizes(L):
             for D, F in ((1, 1), (64, 64), (500, 1024), (1433, 4096), (2048, 8192)):
                 up = lambda n: (n + 63) // 64 * 64
                 slopes = up(M) * 2 * up(F) * 2 * parts
-                bwd = L.gs_gated_bwd_scratch_bytes(M, D, F, typ)
+                bwd = L.gs_gated_bwd_scratch_bytes(M, D, F, typ, 1)
                 assert bwd >= slopes
                 laid = slopes + (parts > 1) * (up(M) + 2 * up(F)) * up(D) * 2 * parts
                 outputs = 4 * (M * D + 2 * up(F) * D)
                 assert bwd <= laid + 64 * outputs, (typ, M, D, F, bwd)
-                assert L.gs_gated_fwd_scratch_bytes(M, D, F, typ) <= (parts > 1) * (up(M) + 2 * up(F)) * up(D) * 2 * parts + 64 * 8 * M * F
+                fwd = L.gs_gated_fwd_scratch_bytes(M, D, F, typ, 1)
+                assert fwd <= (parts > 1) * (up(M) + 2 * up(F)) * up(D) * 2 * parts + 64 * 8 * M * F
+                copies = (typ > 0) * (up(M) + 2 * up(F)) * up(D) * 2      # of 16-bit operands whose rows are not whole chunks
+                assert L.gs_gated_bwd_scratch_bytes(M, D, F, typ, 0) == bwd + copies
+                assert L.gs_gated_fwd_scratch_bytes(M, D, F, typ, 0) - fwd in (0, copies)
 
 
 def _slope(f, x, v, e=1e-6):
