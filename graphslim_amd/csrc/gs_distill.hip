@@ -155,7 +155,8 @@ struct DistillTeacher {
   }
 };
 
-// The row in registers, EP logits a thread: read once, written once.
+// The row in registers, EP logits a thread: read once, written once.  Bound by HBM: 8192 x 32000 bf16, loss and gradient, 1.05 GB, 195 us
+// = 5.4 TB/s; 454 x 40 fp32 12.5 us, a launch and its host call.
 template <int T, int G, int EP, bool LOSS, bool GRAD, bool PAST>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void gs_distill_regs_kernel(DistillArgs a) {
   typedef typename GsElt<T>::type E;
@@ -247,7 +248,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void gs_distill_regs_kernel(Dist
 }
 
 // Rows of any length, a workgroup each.  STATS: the log-sum is taken from z (a running maximum and sum per thread, one pass), else it is
-// given.
+// given.  Bound by HBM: losses, 2047 x 100003 fp16, 410 MB, 89 us = 4.6 TB/s; the gradient alone, 1024 x 50001 fp32, 411 MB,
+// 100 us = 4.1 TB/s (rows of odd length: three of four are read and written across cache lines).
 template <int T, int G, bool STATS, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(G) void gs_distill_row_kernel(DistillArgs a) {
   typedef typename GsElt<T>::type E;

@@ -139,7 +139,8 @@ __global__ __launch_bounds__(256) void gs_gated_pack_kernel(GatedPack a) {
   gf_put8<T, PL>(v, (P*)a.out[w] + r * a.Cp + c, a.Rp[w] * a.Cp);
 }
 
-// dg, du from dh and the saved g, u: [PL][Mp][2 Fp], columns [0, Fp) dg, [Fp, 2 Fp) du, zeros in the padding of both
+// dg, du from dh and the saved g, u: [PL][Mp][2 Fp], columns [0, Fp) dg, [Fp, 2 Fp) du, zeros in the padding of both.  Bound by HBM
+// (8192 x 8192 bf16: 134 + 537 MB read, 268 MB written), so `saved`, which nobody reads again, passes the caches by.
 template <int T, int PL>
 __global__ __launch_bounds__(256) void gs_gated_slopes_kernel(int act, const typename GsElt<T>::type* __restrict__ dh, long lddh,
                                                               const float* __restrict__ saved, long M, long F,
@@ -182,7 +183,8 @@ __global__ __launch_bounds__(256) void gs_gated_slopes_kernel(int act, const typ
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------------
 // For a few rows (eight at a time) the weights are all there is to read, and the vector units keep up: a wave takes RF rows of both weights,
-// its lanes 16 bytes each of a stretch of k, and adds across the lanes at the end.  Exact fp32 products for every type.
+// its lanes 16 bytes each of a stretch of k, and adds across the lanes at the end.  Exact fp32 products for every type.  Bound by the
+// reading of the weights: one row, 2048 x 8192 bf16, 67 MB, 11.7 us = 5.7 TB/s (from the 256 MB cache when repeated, as here).
 struct GatedRows {
   const void *x, *wg, *wu;
   long ldx, ldw, M, D, F, ldh;
@@ -364,6 +366,11 @@ __device__ const int gf_zeros[4] = {};   // a chunk behind the end of a row
 // index is contiguous, not k.  RAW: x and the weights are read where they are though their rows begin or end inside a 16-byte chunk:
 // through registers, with zeros behind a row's end.  GATED: rows of B alternate between gate and up every 16, so that a lane holds both sums of its outputs
 // and the activation is applied in registers.
+// Bound by the matrix pipe where tiles are many: 16 FM x 16 FN results of a wave need FM + FN fragments from LDS a step for FM FN
+// instructions, so that 8 x 4 fragments (256 x 256 by eight waves) keep LDS reads below the pipe's time, and 4 x 4 do not quite.
+// 8192 x 2048 x 8192 bf16: forward 452 us = 1.22 PFLOP/s (a library's product of 8192^3 reaches 1.32), 516 with `saved` (537 MB more),
+// backward 1055 us = 1.04 PFLOP/s with the pass that makes [dg | du].  fp32, six products of bf16 parts, 2708 x 500 x 1024: 150 us for
+// both passes = 111 TFLOP/s (the library: 153): the forward product has 176 large tiles for 256 compute units.
 template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED>
 __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, unsigned slice, char* smem) {
   typedef typename GfPlane<T, PL>::type P;
@@ -933,7 +940,7 @@ struct GatedCall {
   char* scratch;
 };
 
-// x, Wg and Wu as operands: as they are, or split and laid out in the scratch
+// x, Wg and Wu as operands: as they are, or laid out (fp32: split) in the scratch
 struct GatedOperands {
   const void *x, *w[2];
   long ldx, ldw, plane_x, plane_w;
