@@ -360,7 +360,7 @@ __device__ __forceinline__ void gf_tr_read4(unsigned addr, int first, Frag* x) {
   x[3] = __builtin_bit_cast(Frag, __builtin_shufflevector(l3, h3, 0, 1, 2, 3));
 }
 
-__device__ const int gf_zeros[4] = {};   // a chunk behind the end of a row
+__device__ const int gf_zeros[4] __attribute__((aligned(16))) = {};   // a chunk behind the end of a row
 
 // T: type of the outputs (and of 16-bit operands), PL: parts, WM x WN waves of (16 FM) x (16 FN) results.  TA, TB: the operand's other
 // index is contiguous, not k.  RAW: x and the weights are read where they are though their rows begin or end inside a 16-byte chunk:

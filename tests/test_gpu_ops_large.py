@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import ops_reference as R
-from test_gpu_ops import BF16, DEV, F16, F32, gen, normal, ops, zipf  # noqa: F401 (ops is a fixture)
+from test_gpu_ops import BF16, DEV, F16, F32, gen, normal, ops, strided, zipf  # noqa: F401 (ops is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -22,12 +22,12 @@ WIDE_32 = [(3000, 64, 700), (8200, 515, 9),                         # fwd; fwd/
            (515, 4100, 260), (4100, 515, 9), (70, 515, 2056), (515, 64, 4100)]   # pair; dw/; dx/; both/
 
 
-def gated_case(ops, M, D, F, dtype):
+def gated_case(ops, M, D, F, dtype, place=lambda t: t.to(DEV)):
     g = gen("wide", M, D, F)
     act = ["silu", "gelu", "relu", "sigmoid"][(M + D + F) % 4]
     x, wg, wu = normal(g, M, D, dtype=dtype), normal(g, F, D, std=D ** -0.5, dtype=dtype), normal(g, F, D, std=D ** -0.5, dtype=dtype)
     d_h = normal(g, M, F, dtype=dtype)
-    xd, wgd, wud, dd = (t.to(DEV) for t in (x, wg, wu, d_h))
+    xd, wgd, wud, dd = (place(t) for t in (x, wg, wu, d_h))
     want = {key: tuple(t.cpu() for t in pair) for key, pair in R.gated(xd, wgd, wud, act, dd).items()}
     h, saved = ops.gated_ffn(xd, wgd, wud, act, save=True)
     R.within(h, want["h"], "h")
@@ -50,6 +50,19 @@ def test_gated_wide_16(ops, M, D, F, dtype):
 @pytest.mark.parametrize("M,D,F", WIDE_32)
 def test_gated_wide_32(ops, M, D, F):
     gated_case(ops, M, D, F, F32)
+
+
+@pytest.mark.parametrize("M,D,F", [(2000, 128, 2100), (130, 128, 70), (2100, 1032, 2050)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gated_wide_unaligned(ops, M, D, F, dtype):
+    """Whole chunks in a row, but rows that begin anywhere: read through registers, read so in the small tile, laid out."""
+    gated_case(ops, M, D, F, dtype, lambda t: strided(t, 3, 5))
+
+
+@pytest.mark.parametrize("M,D,F", [(5, 1, 1), (40, 3, 70), (300, 7, 130), (9, 8, 130), (30, 9, 66), (260, 15, 300)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_gated_narrow(ops, M, D, F, dtype):
+    gated_case(ops, M, D, F, dtype)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
