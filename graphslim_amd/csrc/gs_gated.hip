@@ -795,7 +795,7 @@ struct GatedPlan {
 
 // Whether a forward call lays out 16-bit operands whose rows do not consist of whole, aligned chunks, as every backward call does, rather
 // than read them through registers: laying out takes a launch and its traffic, reading so 1.6 ns more for a million products (fp16:
-// 300 x 2047 x 8192 read 54 us, laid out 81; 8000 x 301 x 500 21.5 and 24.7; 2000 x 1433 x 4096 72 and 69; 4000 x 2047 x 8192 377 and 307).
+// 300 x 2047 x 8192 read 54 us, laid out 81; 8000 x 301 x 500 21.5 and 24.7; 2000 x 1433 x 4096 72 and 66; 4000 x 2047 x 8192 377 and 307).
 inline bool gf_lay_out(long M, long D, long F) {
   return D < 8 || 1.6e-9 * M * D * F > 4 + 0.9e-6 * (M + 2 * F) * D;
 }

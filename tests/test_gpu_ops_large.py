@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 # What each shape is for: the tile of 256 rows in the forward product (fwd), in dx and dW one after the other (dx, dw) or in one launch
 # (pair), cut along k (/) or not; 16-bit rows that do not consist of whole chunks are laid out first, or read through registers (raw).
-WIDE_16 = [(6000, 64, 700), (2050, 72, 2050), (2000, 75, 2100), (2050, 1035, 2050),   # fwd; rows that end inside a step of k; raw; laid out
+WIDE_16 = [(6000, 64, 700), (2050, 72, 2050), (2000, 75, 2100), (4100, 1035, 2050),   # fwd; rows that end inside a step of k; raw; laid out
            (6000, 4104, 16), (6000, 4100, 9),                       # dx; laid out
            (70, 4104, 8200), (70, 4100, 8200),                      # dw; laid out, forward raw and cut
            (700, 4104, 4104),                                       # dx/
@@ -52,7 +52,7 @@ def test_gated_wide_32(ops, M, D, F):
     gated_case(ops, M, D, F, F32)
 
 
-@pytest.mark.parametrize("M,D,F", [(2000, 128, 2100), (130, 128, 70), (2100, 1032, 2050)])
+@pytest.mark.parametrize("M,D,F", [(2000, 128, 2100), (130, 128, 70), (4100, 1032, 2050)])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_gated_wide_unaligned(ops, M, D, F, dtype):
     """Whole chunks in a row, but rows that begin anywhere: read through registers, read so in the small tile, laid out."""
