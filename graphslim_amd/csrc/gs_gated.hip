@@ -5,6 +5,11 @@
 // latter are transposed on their way from LDS to the registers.  16-bit operands enter as they are; an fp32 operand is the exact sum of three bf16 parts
 // (x = h + m + l, 8 + 8 + 8 significant bits), and six products of parts make one product: what they leave out is below 2^-23 of it.
 // (Parts have bf16's smallest step, 2^-133: a value is represented to 2^-134 or to 24 bits, whichever is coarser.)
+// dg and du of 16-bit operands are computed in fp32 and enter as two bf16 parts (17 bits and fp32's range).  Rounded to the operands'
+// type they would cost the gradients a second rounding as large as that of the result, and in fp16 dh u act'(g) can lie outside of the
+// type though the gradients do not.  The parts lie one behind the other along k, against the same weights or x a second time:
+//   bf16:  dg W = lo W + hi W;      fp16:  W = V + R, bf16 parts that hold all of its 11 bits, dg W = lo V + hi R + hi V
+// (lo R is below 2^-17 of the product and left out).
 // The parts of fp32 operands, and [dg | du], are laid out in the caller's scratch first, rows padded with zeros to a multiple of 64;
 // so are 16-bit operands whose rows do not consist of whole, aligned chunks of 16 bytes, unless it is cheaper to read them as they are.
 #include <algorithm>
@@ -87,6 +92,17 @@ template <>
 struct GfPlane<GS_TYPE_F32, 3> {
   typedef __bf16 type;
 };
+template <>
+struct GfPlane<GS_TYPE_F16, 2> {   // 2: dg, du of 16-bit types
+  typedef __bf16 type;
+};
+template <>
+struct GfPlane<GS_TYPE_BF16, 2> {
+  typedef __bf16 type;
+};
+
+// stretches of k that a product of such parts has
+constexpr int gf_stretches(int type, int pl) { return pl != 2 ? 1 : (type == GS_TYPE_F16 ? 3 : 2); }
 
 template <int T, int PL, typename P>
 __device__ __forceinline__ void gf_put8(const float* v, P* __restrict__ o, long plane) {
@@ -108,7 +124,7 @@ __device__ __forceinline__ void gf_put8(const float* v, P* __restrict__ o, long 
     }
     *(V*)o = h;
     *(V*)(o + plane) = m;
-    *(V*)(o + 2 * plane) = l;
+    if constexpr (PL == 3) *(V*)(o + 2 * plane) = l;
   }
 }
 
@@ -140,7 +156,7 @@ __global__ __launch_bounds__(256) void gs_gated_pack_kernel(GatedPack a) {
 }
 
 // dg, du from dh and the saved g, u: [PL][Mp][2 Fp], columns [0, Fp) dg, [Fp, 2 Fp) du, zeros in the padding of both.  Bound by HBM
-// (8192 x 8192 bf16: 134 + 537 MB read, 268 MB written), so `saved`, which nobody reads again, passes the caches by.
+// (8192 x 8192 bf16: 134 + 537 MB read, 537 MB written), so `saved`, which nobody reads again, passes the caches by.
 template <int T, int PL>
 __global__ __launch_bounds__(256) void gs_gated_slopes_kernel(int act, const typename GsElt<T>::type* __restrict__ dh, long lddh,
                                                               const float* __restrict__ saved, long M, long F,
@@ -269,7 +285,8 @@ struct GatedGemm {
   long lda, plane_a;
   const void* B[2];     // gated: gate and up projection; n contiguous: rows of k below `kb` in the first, the others in the second
   long ldb, plane_b;
-  long M, N, K;         // K a multiple of 64
+  long M, N, K;         // K a multiple of 64, all stretches together
+  long stretch;         // of k; a multiple of 64
   long k_end;           // k contiguous in both: elements that a row of k has (K or less; RAW: 8 or more)
   long bcols;           // n contiguous: columns that rows of B have (a multiple of 8, N or more)
   long kb, brows;       // n contiguous: rows that B[0] stands for (a multiple of 64), and rows that each of B has; behind them A is 0
@@ -292,6 +309,19 @@ __device__ __forceinline__ E* gf_row(const GatedGemm& q, long m) {
 
 __device__ __forceinline__ f32x4 gf_mfma(h16x8 a, h16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 gf_mfma(b16x8 a, b16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// eight fp16 as bf16: what a bf16 holds of them, or the rest
+__device__ __forceinline__ b16x8 gf_part(b16x8 bits, bool rest) {
+  const h16x8 w = __builtin_bit_cast(h16x8, bits);
+  b16x8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float f = (float)w[e];
+    r[e] = (__bf16)f;
+    if (rest) r[e] = (__bf16)(f - (float)r[e]);
+  }
+  return r;
+}
 
 template <int N, typename Fn>
 __device__ __forceinline__ void gf_static_for(Fn f) {
@@ -362,23 +392,26 @@ __device__ __forceinline__ void gf_tr_read4(unsigned addr, int first, Frag* x) {
 
 __device__ const int gf_zeros[4] __attribute__((aligned(16))) = {};   // a chunk behind the end of a row
 
-// T: type of the outputs (and of 16-bit operands), PL: parts, WM x WN waves of (16 FM) x (16 FN) results.  TA, TB: the operand's other
+// T: type of the outputs (and of 16-bit operands), PL: parts (3: side by side; 2: those of A one behind the other along k), WM x WN waves of (16 FM) x (16 FN) results.  TA, TB: the operand's other
 // index is contiguous, not k.  RAW: x and the weights are read where they are though their rows begin or end inside a 16-byte chunk:
 // through registers, with zeros behind a row's end.  GATED: rows of B alternate between gate and up every 16, so that a lane holds both sums of its outputs
 // and the activation is applied in registers.
 // Bound by the matrix pipe where tiles are many: 16 FM x 16 FN results of a wave need FM + FN fragments from LDS a step for FM FN
 // instructions, so that 8 x 4 fragments (256 x 256 by eight waves) keep LDS reads below the pipe's time, and 4 x 4 do not quite.
 // 8192 x 2048 x 8192 bf16: forward 452 us = 1.22 PFLOP/s (a library's product of 8192^3 reaches 1.32), 516 with `saved` (537 MB more),
-// backward 1055 us = 1.04 PFLOP/s with the pass that makes [dg | du].  fp32, six products of bf16 parts, 2708 x 500 x 1024: 150 us for
+// backward 2070 us = 1.06 PFLOP/s of the doubled products with the pass that makes [dg | du] (dg and du rounded to bf16: 1055).  fp32, six products of bf16 parts, 2708 x 500 x 1024: 150 us for
 // both passes = 111 TFLOP/s (the library: 153): the forward product has 176 large tiles for 256 compute units.
 template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED>
 __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, unsigned slice, char* smem) {
   typedef typename GfPlane<T, PL>::type P;
   typedef typename GfFrag<P>::type Frag;
   typedef typename GsElt<T>::type E;
+  constexpr int NP = PL == 3 ? 3 : 1;   // parts that are in LDS at a time
+  constexpr int STRETCHES = gf_stretches(T, PL);
+  static_assert(PL != 2 || (TB && !RAW && !GATED), "the backward products");
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16, NT = WM * WN * 64;
   constexpr int CA = (TA ? BM : BK) / 8, CB = (TB ? BN : BK) / 8;   // 16-byte chunks of a row
-  constexpr int TILE_A = BM * BK, TILE_B = BN * BK, STAGE = PL * (TILE_A + TILE_B);
+  constexpr int TILE_A = BM * BK, TILE_B = BN * BK, STAGE = NP * (TILE_A + TILE_B);
   constexpr int ITA = TILE_A / 8 / NT, ITB = TILE_B / 8 / NT;
   static_assert(TILE_A / 8 % NT == 0 && TILE_B / 8 % NT == 0, "whole waves load a tile");
   constexpr bool PHASES = WM * WN == 8 && BK == 64 && !RAW;       // eight waves that take turns, see below
@@ -428,6 +461,12 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
   };
   auto stage = [&](int buf, long k0) {
     P* base = lds + buf * STAGE;
+    long a_at = 0;                                                 // of the stretch's part of A
+    if constexpr (STRETCHES > 1) {                                 // the low part of A first, then the high one (fp16: twice)
+      if (k0 < q.stretch) a_at = q.plane_a;
+      k0 -= k0 >= q.stretch ? q.stretch : 0;
+      if constexpr (STRETCHES > 2) k0 -= k0 >= q.stretch ? q.stretch : 0;
+    }
     const P* b0 = (const P*)q.B[0] + k0;
     bool end = false;
     if constexpr (TB) {
@@ -459,16 +498,16 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
       }
     }
 #pragma unroll
-    for (int p = 0; p < PL; ++p) {
+    for (int p = 0; p < NP; ++p) {
 #pragma unroll
       for (int i = 0; i < ITA; ++i) {
-        const P* at = srcA[i] + p * q.plane_a + (TA ? k0 * q.lda : k0);
+        const P* at = srcA[i] + p * q.plane_a + (a_at + (TA ? k0 * q.lda : k0));
         __builtin_amdgcn_global_load_lds((gbl_ptr)at, (lds_ptr)(base + p * TILE_A + (i * NT + wave * 64) * 8), 16, 0, 0);
       }
 #pragma unroll
       for (int i = 0; i < ITB; ++i) {
         const P* at = b0 + p * q.plane_b + (TB && end ? endB[i] : srcB[i]);
-        __builtin_amdgcn_global_load_lds((gbl_ptr)at, (lds_ptr)(base + PL * TILE_A + p * TILE_B + (i * NT + wave * 64) * 8), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gbl_ptr)at, (lds_ptr)(base + NP * TILE_A + p * TILE_B + (i * NT + wave * 64) * 8), 16, 0, 0);
       }
     }
   };
@@ -491,17 +530,17 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
     for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
   const unsigned tra = TA ? gf_tr_addr<BM, BK>(lds, wm * FM * 16, lane) : 0u;
-  const unsigned trb = TB ? gf_tr_addr<BN, BK>(lds + PL * TILE_A, wn * FN * 16, lane) : 0u;
+  const unsigned trb = TB ? gf_tr_addr<BN, BK>(lds + NP * TILE_A, wn * FN * 16, lane) : 0u;
   stage(0, k_begin);
   land(0);
   int buf = 0;
-  Frag a[PL][FM], b[PL][FN];
+  Frag a[NP][FM], b[NP][FN];
   const P* ta = lds;
   const P* tb = lds;
   // the fragments of 32 of k; those of a transposed A are read four rows of tiles at a time, before their products
-  auto read = [&](auto ks_, int at) {
+  auto read = [&](auto ks_, int at, long k0) {
     constexpr int ks = decltype(ks_)::value;
-    gf_static_for<PL>([&](auto p_) {
+    gf_static_for<NP>([&](auto p_) {
       constexpr int p = decltype(p_)::value;
       if constexpr (TB) {
         gf_static_for<FN / 4>([&](auto j_) {
@@ -522,6 +561,14 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
         for (int i = 0; i < FM; ++i) a[p][i] = gf_frag<Frag, BK>(ta + p * TILE_A, (wm * FM + i) * 16, ks, lane);
       }
     });
+    if constexpr (STRETCHES == 3) {
+      const bool rest = k0 >= q.stretch && k0 < 2 * q.stretch;
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        b[0][j] = gf_part(b[0][j], rest);
+        asm volatile("" : "+v"(b[0][j]));                          // (one after the other: all at once would take more registers than there are)
+      }
+    }
   };
   auto multiply = [&] {
     __builtin_amdgcn_s_setprio(1);
@@ -561,13 +608,13 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
     if (second) phase_end(false);
     for (long k0 = k_begin; k0 < k_end; k0 += BK, buf ^= 1) {
       ta = lds + buf * STAGE;
-      tb = ta + PL * TILE_A;
+      tb = ta + NP * TILE_A;
       if (k0 + BK < k_end) stage(buf ^ 1, k0 + BK);
-      read(std::integral_constant<int, 0>{}, buf);
+      read(std::integral_constant<int, 0>{}, buf, k0);
       phase_end(false);
       multiply();
       phase_end(false);
-      read(std::integral_constant<int, 1>{}, buf);
+      read(std::integral_constant<int, 1>{}, buf, k0);
       phase_end(second);
       multiply();
       phase_end(!second);
@@ -577,10 +624,10 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
     for (long k0 = k_begin; k0 < k_end; k0 += BK, buf ^= 1) {
       __syncthreads();   // this step's tile has landed; the other buffer has been read by all
       ta = lds + buf * STAGE;
-      tb = ta + PL * TILE_A;
+      tb = ta + NP * TILE_A;
       if (k0 + BK < k_end) stage(buf ^ 1, k0 + BK);
       gf_static_for<BK / 32>([&](auto ks) {
-        read(ks, buf);
+        read(ks, buf, k0);
         multiply();
       });
       if (k0 + BK < k_end) land(buf ^ 1);
@@ -733,7 +780,7 @@ GatedSplit gf_split_of(long M, long N, long K, bool gated, int pl) {
   double least = 1e300;
   const long cols = gated ? 2 * N : N;
   for (int big = 0; big < 2; ++big) {
-    const long bm = big ? 256 : 128, bn = big && pl == 1 ? 256 : 128, bk = pl == 3 ? 32 : 64;
+    const long bm = big ? 256 : 128, bn = big && pl != 3 ? 256 : 128, bk = pl == 3 ? 32 : 64;
     const long tiles = ((M + bm - 1) / bm) * ((cols + bn - 1) / bn), slots = big || pl == 3 ? 256 : 512, steps = K / bk;
     const double step = big ? (pl == 3 ? 1.4 : 1.75) : 1.0;
     for (long want = 1; want <= 64 && want <= steps; ++want) {
@@ -750,20 +797,20 @@ GatedSplit gf_split_of(long M, long N, long K, bool gated, int pl) {
   return best;
 }
 
-// dx (M x D, k over 2 Fp) and dW (2 Fp x D, k over Mp): one launch of both, cut into pieces of about equal length, where that costs less
+// dx (M x D, k over 2 Fp) and dW (2 Fp x D, k over Mp), each in so many stretches: one launch of both, cut into pieces of about equal length, where that costs less
 // than one after the other (the same units, a launch about 3).
 struct GatedPair {
   bool together;
   GatedSplit dx, dw;
 };
 
-GatedPair gf_pair_of(long M, long D, long Fp, long Mp, int pl) {
-  GatedPair best = {false, gf_split_of(M, D, 2 * Fp, false, pl), gf_split_of(2 * Fp, D, Mp, false, pl)};
+GatedPair gf_pair_of(long M, long D, long Fp, long Mp, int pl, int stretches) {
+  GatedPair best = {false, gf_split_of(M, D, 2 * Fp * stretches, false, pl), gf_split_of(2 * Fp, D, Mp * stretches, false, pl)};
   double least = best.dx.cost + best.dw.cost + 3;
   for (int big = 0; big < 2; ++big) {
-    const long bm = big ? 256 : 128, bn = big && pl == 1 ? 256 : 128, bk = pl == 3 ? 32 : 64, gy = (D + bn - 1) / bn;
+    const long bm = big ? 256 : 128, bn = big && pl != 3 ? 256 : 128, bk = pl == 3 ? 32 : 64, gy = (D + bn - 1) / bn;
     const long tx = (M + bm - 1) / bm * gy, tw = (2 * Fp + bm - 1) / bm * gy, slots = big || pl == 3 ? 256 : 512;
-    const long sx = 2 * Fp / bk, sw = Mp / bk, most = std::max(sx, sw);
+    const long sx = 2 * Fp * stretches / bk, sw = Mp * stretches / bk, most = std::max(sx, sw);
     const double step = big ? (pl == 3 ? 1.4 : 1.75) : 1.0;
     for (long len = most;; len = (len * 3 + 3) / 4) {
       const long nx = std::min(64L, (sx + len - 1) / len), nw = std::min(64L, (sw + len - 1) / len);
@@ -783,7 +830,7 @@ GatedPair gf_pair_of(long M, long D, long Fp, long Mp, int pl) {
 
 // Where the laid-out operands lie in the scratch (elements of 2 bytes).  The sizes go by the shapes and the type alone.
 struct GatedPlan {
-  int pl;
+  int pl, slopes;                     // parts of x and the weights, of dg and du
   bool pack;                          // x, Wg and Wu are laid out in the scratch (both passes)
   long Dp, Fp, Mp;
   size_t x, wg, wu, fwd;              // their places, with padded rows
@@ -803,26 +850,27 @@ inline bool gf_lay_out(long M, long D, long F) {
 GatedPlan gf_plan(long M, long D, long F, int type, bool plain, bool bwd) {
   GatedPlan p = {};
   p.pl = type == GS_TYPE_F32 ? 3 : 1;
+  p.slopes = type == GS_TYPE_F32 ? 3 : 2;
   p.Dp = gf_up(D);
   p.Fp = gf_up(F);
   p.Mp = gf_up(M);
   size_t o = 0;
-  auto take = [&](size_t n) { size_t at = o; o += n * p.pl; return at; };
+  auto take = [&](size_t n, int parts) { size_t at = o; o += n * parts; return at; };
   p.pack = p.pl > 1 || (!plain && (bwd || gf_lay_out(M, D, F)));
   if (p.pack) {
-    p.x = take((size_t)p.Mp * p.Dp);
-    p.wg = take((size_t)p.Fp * p.Dp);
-    p.wu = take((size_t)p.Fp * p.Dp);
+    p.x = take((size_t)p.Mp * p.Dp, p.pl);
+    p.wg = take((size_t)p.Fp * p.Dp, p.pl);
+    p.wu = take((size_t)p.Fp * p.Dp, p.pl);
   }
   p.part_fwd = o;
   if (!bwd) {
     p.split = gf_split_of(M, F, p.Dp, true, p.pl);
     p.fwd = o + 2 * p.split.part;
   }
-  p.dgu = take((size_t)p.Mp * 2 * p.Fp);
+  p.dgu = take((size_t)p.Mp * 2 * p.Fp, p.slopes);
   p.part_bwd = o;
   if (bwd) {
-    p.pair = gf_pair_of(M, D, p.Fp, p.Mp, p.pl);
+    p.pair = gf_pair_of(M, D, p.Fp, p.Mp, p.slopes, gf_stretches(type, p.slopes));
     const size_t dx = p.pair.dx.part, dw = p.pair.dw.part;
     p.bwd = o + 2 * (p.pair.together ? dx + dw : std::max(dx, dw));
   }
@@ -859,7 +907,7 @@ inline long gf_join_blocks(const GatedGemm& q) { return (q.M * ((q.N + 3) / 4) +
 
 template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED>
 int gf_tile(GatedGemm q, const GatedSplit& sp, float* part, hipStream_t s) {
-  constexpr int BM = WM * FM * 16, BN = WN * FN * 16 / (GATED ? 2 : 1), LDS = 2 * PL * (WM * FM + WN * FN) * 16 * BK * 2;
+  constexpr int BM = WM * FM * 16, BN = WN * FN * 16 / (GATED ? 2 : 1), LDS = 2 * (PL == 3 ? 3 : 1) * (WM * FM + WN * FN) * 16 * BK * 2;
   auto kern = gs_gated_gemm_kernel<T, PL, WM, WN, FM, FN, BK, TA, TB, RAW, GATED>;
   static std::atomic<unsigned long long> known{0};
   GS_TRY(gf_lds(kern, LDS, known));
@@ -892,7 +940,7 @@ int gf_gemm(const GatedGemm& q, const GatedSplit& sp, bool raw, float* part, hip
 
 template <int T, int PL, int WM, int WN, int FM, int FN, int BK>
 int gf_pair_tile(GatedGemm a, GatedGemm b, const GatedPair& p, float* part, hipStream_t s) {
-  constexpr int BM = WM * FM * 16, BN = WN * FN * 16, LDS = 2 * PL * (WM * FM + WN * FN) * 16 * BK * 2;
+  constexpr int BM = WM * FM * 16, BN = WN * FN * 16, LDS = 2 * (PL == 3 ? 3 : 1) * (WM * FM + WN * FN) * 16 * BK * 2;
   auto kern = gs_gated_pair_kernel<T, PL, WM, WN, FM, FN, BK>;
   static std::atomic<unsigned long long> known{0};
   GS_TRY(gf_lds(kern, LDS, known));
@@ -992,7 +1040,7 @@ int gf_fwd(const GatedCall& c, hipStream_t s) {
   GatedGemm q = {};
   q.A = o.x; q.lda = o.ldx; q.plane_a = o.plane_x;
   q.B[0] = o.w[0]; q.B[1] = o.w[1]; q.ldb = o.ldw; q.plane_b = o.plane_w;
-  q.M = c.M; q.N = c.F; q.K = p.Dp;
+  q.M = c.M; q.N = c.F; q.K = q.stretch = p.Dp;
   q.C[0] = c.h; q.ldc = c.ldh;
   q.saved = c.saved; q.act = c.act;
   q.k_end = p.pack ? p.Dp : c.D;
@@ -1001,33 +1049,34 @@ int gf_fwd(const GatedCall& c, hipStream_t s) {
 
 template <int T, int PL>
 int gf_bwd(const GatedCall& c, hipStream_t s) {
+  constexpr int SL = PL == 3 ? 3 : 2, STRETCHES = gf_stretches(T, SL);
   typedef typename GsElt<T>::type E;
-  typedef typename GfPlane<T, PL>::type P;
+  typedef typename GfPlane<T, SL>::type P;
   const GatedPlan p = gf_plan(c.M, c.D, c.F, T, gf_plain(c.x, c.ldx, c.wg, c.wu, c.ldw, c.D), true);
   P* dgu = (P*)c.scratch + p.dgu;
   const long plane = p.Mp * 2 * p.Fp, blocks = (p.Mp * (p.Fp / 8) + 255) / 256;
   if (blocks > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated_bwd: %ld x %ld is beyond one launch", c.M, c.F);
   GatedOperands o;
   GS_TRY((gf_operands<T, PL>(c, p, &o, s)));
-  gs_gated_slopes_kernel<T, PL><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(c.act, (const E*)c.dh, c.lddh, c.saved, c.M, c.F, dgu, p.Mp, p.Fp, plane);
+  gs_gated_slopes_kernel<T, SL><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(c.act, (const E*)c.dh, c.lddh, c.saved, c.M, c.F, dgu, p.Mp, p.Fp, plane);
   GS_LAUNCH_CHECK();
   // dx: k runs over the columns of dg, then of du, and over the rows of Wg, then of Wu
   GatedGemm q = {};
   q.A = dgu; q.lda = 2 * p.Fp; q.plane_a = plane;
   q.B[0] = o.w[0]; q.B[1] = o.w[1]; q.ldb = o.ldw; q.plane_b = o.plane_w;
-  q.M = c.M; q.K = 2 * p.Fp; q.kb = p.Fp; q.brows = p.pack ? p.Fp : c.F;
+  q.M = c.M; q.K = 2 * p.Fp * STRETCHES; q.stretch = 2 * p.Fp; q.kb = p.Fp; q.brows = p.pack ? p.Fp : c.F;
   q.N = c.D; q.bcols = p.pack ? p.Dp : c.D;
   q.C[0] = c.dx; q.ldc = c.lddx; q.rows = q.rows1 = c.M;
   float* part = (float*)((P*)c.scratch + p.part_bwd);
   // dWg, dWu: k runs over the tokens
   GatedGemm w = q;
   w.B[0] = o.x; w.ldb = o.ldx; w.plane_b = o.plane_x;
-  w.M = 2 * p.Fp; w.K = p.Mp; w.kb = p.Mp; w.brows = p.pack ? p.Mp : c.M;
+  w.M = 2 * p.Fp; w.K = p.Mp * STRETCHES; w.stretch = p.Mp; w.kb = p.Mp; w.brows = p.pack ? p.Mp : c.M;
   w.bcols = p.pack ? p.Dp : c.D;
   w.C[0] = c.dwg; w.C[1] = c.dwu; w.ldc = c.lddw; w.rows = c.F; w.rows1 = p.Fp;
-  if (p.pair.together) return gf_pair<T, PL>(q, w, p.pair, part, s);
-  GS_TRY((gf_gemm<T, PL, false, true, false>(q, p.pair.dx, false, part, s)));
-  return gf_gemm<T, PL, true, true, false>(w, p.pair.dw, false, part, s);
+  if (p.pair.together) return gf_pair<T, SL>(q, w, p.pair, part, s);
+  GS_TRY((gf_gemm<T, SL, false, true, false>(q, p.pair.dx, false, part, s)));
+  return gf_gemm<T, SL, true, true, false>(w, p.pair.dw, false, part, s);
 }
 
 // dW = 0 where there are no tokens

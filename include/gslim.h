@@ -333,8 +333,8 @@ int gs_embedding_bwd(const void* dout, long ldd, int type, const int* ids, long 
 size_t gs_gated_fwd_scratch_bytes(long M, long D, long F, int type, int plain);
 int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, long ldw, int type, long M, long D, long F, int act,
                  void* h, long ldh, float* saved, void* scratch, gs_stream_t stream);
-/* dg = dh * u * act'(g), du = dh * act(g) (rounded to the operands' type: the products take them there); dx = dg Wg + du Wu,
- * dw_gate = dg^T x, dw_up = du^T x.
+/* dg = dh * u * act'(g), du = dh * act(g); dx = dg Wg + du Wu, dw_gate = dg^T x, dw_up = du^T x.  For 16-bit types dg and du enter the
+ * products as two bf16 parts: to 2^-17 of each and with fp32's range, so that a slope that fp16 does not hold leaves the gradients right.
  * fp32 products of more than a few rows are six products of bf16 parts: as exact as fp32 (parts have a smallest step of 2^-133), but an
  * infinite operand gives NaN where it meets a zero part. */
 size_t gs_gated_bwd_scratch_bytes(long M, long D, long F, int type, int plain);
