@@ -3,6 +3,8 @@
 //   loss = tau^2 sum_j p_j (log p_j - log q_{c_j}),      dz_i = w tau (q_i - sum_{j : c_j = i} p_j)      (w = d total / d loss).
 // An entry whose class is none of the V, or whose logit is -inf, is not there; a row without entries (padding) has loss 0 and gradient 0.
 // Everything is computed in fp32 and rounded once, on the gradient's store.
+#include <algorithm>
+
 #include "gs_types.h"
 
 namespace {
@@ -382,12 +384,28 @@ void ds_stats(const DistillArgs& a, hipStream_t s) {
   gs_distill_row_kernel<T, 1024, true, LOSS, GRAD><<<dim3((unsigned)a.n), dim3(1024), ds_lds(a.k), s>>>(a);
 }
 
+// A launch has fewer than 2^32 threads, and a row takes up to 1024 of them: more rows go in bands
+constexpr long DS_BAND = 1L << 21;
+
 template <int T>
-int ds_launch(const DistillArgs& a, hipStream_t s) {
-  if (!a.dZ) ds_stats<T, true, false>(a, s);
-  else if (a.loss) ds_stats<T, true, true>(a, s);
-  else gs_distill_row_kernel<T, 512, false, false, true><<<dim3((unsigned)a.n), dim3(512), ds_lds(a.k), s>>>(a);
-  GS_LAUNCH_CHECK();
+int ds_launch(const DistillArgs& all, hipStream_t s) {
+  typedef typename GsElt<T>::type E;
+  for (long at = 0; at < all.n; at += DS_BAND) {
+    DistillArgs a = all;
+    a.n = std::min(all.n - at, DS_BAND);
+    a.Z = (const E*)all.Z + at * all.ldz;
+    a.tv = (const E*)all.tv + at * all.k;
+    a.ti = all.ti + at * all.k;
+    if (all.lse_in) a.lse_in = all.lse_in + at;
+    if (all.w) a.w = all.w + at;
+    if (all.loss) a.loss = all.loss + at;
+    if (all.lse) a.lse = all.lse + at;
+    if (all.dZ) a.dZ = (E*)all.dZ + at * all.ldd;
+    if (!a.dZ) ds_stats<T, true, false>(a, s);
+    else if (a.loss) ds_stats<T, true, true>(a, s);
+    else gs_distill_row_kernel<T, 512, false, false, true><<<dim3((unsigned)a.n), dim3(512), ds_lds(a.k), s>>>(a);
+    GS_LAUNCH_CHECK();
+  }
   return GS_OK;
 }
 
