@@ -33,19 +33,22 @@ constexpr long GF_MAX_BLOCKS = 0xffffffL;   // of 256 threads that count their w
 inline long gf_up(long n) { return (n + GF_PAD - 1) / GF_PAD * GF_PAD; }
 
 // ---- activations: the value and its derivative ---------------------------------------------------------------------------------
+// Both tails keep their digits: Phi(g) = erfc(-g / sqrt 2) / 2 (1 + erf(g / sqrt 2) has none left below -5), and the sigmoid and what it
+// leaves of 1 come from e^-|g|, neither by a difference.
 template <int ACT>
 __device__ __forceinline__ void gf_act(float g, float& a, float& da) {
   if constexpr (ACT == GS_ACT_RELU) {
     a = g > 0.f ? g : (g == g ? 0.f : g);
     da = g > 0.f ? 1.f : 0.f;
   } else if constexpr (ACT == GS_ACT_GELU) {
-    const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
     a = g * cdf;
-    da = cdf + g * __expf(-0.5f * g * g) * 0.39894228040143268f;
+    da = cdf + g * expf(-0.5f * g * g) * 0.39894228040143268f;
   } else {
-    const float sig = 1.f / (1.f + __expf(-g));
+    const float e = expf(-fabsf(g)), one = 1.f / (1.f + e), zero = e * one;
+    const float sig = g >= 0.f ? one : zero, rest = g >= 0.f ? zero : one;
     a = ACT == GS_ACT_SILU ? g * sig : sig;
-    da = ACT == GS_ACT_SILU ? sig * (1.f + g * (1.f - sig)) : sig * (1.f - sig);
+    da = ACT == GS_ACT_SILU ? sig * (1.f + g * rest) : sig * rest;
   }
 }
 
