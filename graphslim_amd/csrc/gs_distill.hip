@@ -420,6 +420,17 @@ int ds_run(const char* who, DistillArgs a, int type, long n, hipStream_t s) {
   if (a.dZ && a.dZ == a.Z && a.ldd != a.ldz) GS_FAIL(GS_ERR_ARG, "%s: in place with row strides %ld and %ld", who, a.ldz, a.ldd);
   if (n == 0) return GS_OK;
   if (!a.Z || !a.tv || !a.ti) GS_FAIL(GS_ERR_ARG, "%s: null pointer", who);
+  const int e = gs_type_bytes(type);
+  const GsSpan z = gs_span(a.Z, n, a.ldz, a.V, e), dz = gs_span(a.dZ, n, a.ldd, a.V, e);
+  const GsSpan in[] = {gs_span(a.tv, n * a.k, e), gs_span(a.ti, n * a.k, 4), gs_span(a.lse_in, n, 4), gs_span(a.w, n, 4)};
+  const GsSpan out[] = {dz, gs_span(a.loss, n, 4), gs_span(a.lse, n, 4)};
+  bool clash = a.dZ != a.Z && gs_overlap(dz, z);
+  for (int o = 0; o < 3; ++o) {
+    clash |= o > 0 && gs_overlap(out[o], z);
+    for (const GsSpan& i : in) clash |= gs_overlap(out[o], i);
+    for (int q = 0; q < o; ++q) clash |= gs_overlap(out[o], out[q]);
+  }
+  if (clash) GS_FAIL(GS_ERR_ARG, "%s: an output lies on another operand (only dZ may, on all of Z)", who);
   a.inv_hi = 1.f / a.tau;
   a.inv_lo = (float)(1.0 / (double)a.tau - (double)a.inv_hi);
   if (type == GS_TYPE_F32) return ds_launch<GS_TYPE_F32>(a, s);

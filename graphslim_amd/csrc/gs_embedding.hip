@@ -662,6 +662,10 @@ extern "C" int gs_embedding_fwd(const void* W, long ldw, long V, int F, int type
   GS_TRY(emb_check("gs_embedding_fwd", n, V, F, type, ldw, ldo));
   if (n == 0) return GS_OK;
   if (!W || !ids || !out) GS_FAIL(GS_ERR_ARG, "gs_embedding_fwd: null pointer");
+  const int e = gs_type_bytes(type);
+  const GsSpan o = gs_span(out, n, ldo, F, e);
+  if (gs_overlap(o, gs_span(W, V, ldw, F, e)) || gs_overlap(o, gs_span(ids, n, 4)))
+    GS_FAIL(GS_ERR_ARG, "gs_embedding_fwd: the result lies on another operand");
   hipStream_t s = (hipStream_t)stream;
   if (type == GS_TYPE_F32) return emb_fwd<GS_TYPE_F32>(W, ldw, V, F, ids, n, scale, out, ldo, s);
   if (type == GS_TYPE_F16) return emb_fwd<GS_TYPE_F16>(W, ldw, V, F, ids, n, scale, out, ldo, s);
@@ -678,6 +682,9 @@ extern "C" int gs_embedding_bwd(const void* dout, long ldd, int type, const int*
   if (type_dw != type && type_dw != GS_TYPE_F32)
     GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: the gradient is held in the type of d_out or in fp32 (got %d for %d)", type_dw, type);
   if (!dW || (n > 0 && (!dout || !ids))) GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: null pointer");
+  const GsSpan w = gs_span(dW, V, ldw, F, gs_type_bytes(type_dw));
+  if (n > 0 && (gs_overlap(w, gs_span(dout, n, ldd, F, gs_type_bytes(type))) || gs_overlap(w, gs_span(ids, n, 4))))
+    GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: the gradient lies on another operand");
   if (gs_embedding_bwd_scratch_bytes(n, V, F) > 0 && (!scratch || ((size_t)scratch & 15)))
     GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: the scratch is missing or not 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;

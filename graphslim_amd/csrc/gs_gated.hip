@@ -1115,6 +1115,23 @@ int gf_check(const char* who, const GatedCall& c, int type) {
   return GS_OK;
 }
 
+// Whether an output lies on another operand
+bool gf_clash(const GatedCall& c, int type) {
+  const int e = gs_type_bytes(type);
+  const GsSpan in[] = {gs_span(c.x, c.M, c.ldx, c.D, e), gs_span(c.wg, c.F, c.ldw, c.D, e), gs_span(c.wu, c.F, c.ldw, c.D, e),
+                       gs_span(c.dh, c.M, c.lddh, c.F, e)};
+  const GsSpan saved = gs_span(c.saved, 2 * c.M * c.F, 4);
+  const GsSpan out[] = {gs_span(c.h, c.M, c.ldh, c.F, e), gs_span(c.dx, c.M, c.lddx, c.D, e), gs_span(c.dwg, c.F, c.lddw, c.D, e),
+                        gs_span(c.dwu, c.F, c.lddw, c.D, e)};
+  bool clash = false;
+  for (int o = 0; o < 4; ++o) {
+    clash |= gs_overlap(out[o], saved);
+    for (const GsSpan& i : in) clash |= gs_overlap(out[o], i) || (c.h && gs_overlap(saved, i));
+    for (int q = 0; q < o; ++q) clash |= gs_overlap(out[o], out[q]);
+  }
+  return clash;
+}
+
 int gf_run(const GatedCall& c, int type, bool bwd, hipStream_t s) {
   if (type == GS_TYPE_F32) return gf_dispatch<GS_TYPE_F32, 3>(c, bwd, s);
   if (type == GS_TYPE_F16) return gf_dispatch<GS_TYPE_F16, 1>(c, bwd, s);
@@ -1143,6 +1160,7 @@ extern "C" int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const v
   if (M == 0) return GS_OK;
   if (!x || !w_gate || !w_up || !h || (!scratch && gs_gated_fwd_scratch_bytes(M, D, F, type, gf_plain(x, ldx, w_gate, w_up, ldw, D)) > 0))
     GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: null pointer");
+  if (gf_clash(c, type)) GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: an output lies on another operand");
   if ((size_t)scratch & 15) GS_FAIL(GS_ERR_ARG, "gs_gated_fwd: the scratch is not 16-byte aligned");
   return gf_run(c, type, false, (hipStream_t)stream);
 }
@@ -1157,6 +1175,7 @@ extern "C" int gs_gated_bwd(const void* dh, long lddh, const void* x, long ldx, 
   if (lddh < F || lddx < D || lddw < D) GS_FAIL(GS_ERR_ARG, "gs_gated_bwd: a row stride is below the width");
   if (!dw_gate || !dw_up || (M > 0 && (!dh || !x || !w_gate || !w_up || !saved || !dx || !scratch)))
     GS_FAIL(GS_ERR_ARG, "gs_gated_bwd: null pointer");
+  if (gf_clash(c, type)) GS_FAIL(GS_ERR_ARG, "gs_gated_bwd: an output lies on another operand");
   if ((size_t)scratch & 15) GS_FAIL(GS_ERR_ARG, "gs_gated_bwd: the scratch is not 16-byte aligned");
   return gf_run(c, type, true, (hipStream_t)stream);
 }

@@ -84,4 +84,21 @@ __device__ __forceinline__ typename GsVec<E, N>::type gs_load_past(const E* __re
   return __builtin_nontemporal_load((const typename GsVec<E, N>::type*)p);
 }
 
+// A matrix in memory, in bytes.  What a call writes must not lie on what it reads: workgroups run in any order.
+struct GsSpan {
+  const void* p;
+  long rows, ld, cols;
+};
+static inline GsSpan gs_span(const void* p, long rows, long ld, long cols, int bytes) { return {p, rows, ld * bytes, cols * bytes}; }
+static inline GsSpan gs_span(const void* p, long n, int bytes) { return {p, 1, n * bytes, n * bytes}; }
+
+static inline bool gs_overlap(const GsSpan& a, const GsSpan& b) {
+  if (!a.p || !b.p || a.rows < 1 || b.rows < 1 || a.cols < 1 || b.cols < 1) return false;
+  const long d = (long)((size_t)b.p - (size_t)a.p);
+  if (d >= (a.rows - 1) * a.ld + a.cols || -d >= (b.rows - 1) * b.ld + b.cols) return false;
+  if ((a.rows > 1 && b.rows > 1 && a.ld != b.ld) || (a.rows == 1 && b.rows == 1)) return true;
+  const long ld = a.rows > 1 ? a.ld : b.ld, at = (d % ld + ld) % ld;     // columns of one matrix side by side lie apart
+  return at < a.cols || at + b.cols > ld;
+}
+
 static inline int gs_type_bytes(int t) { return t == GS_TYPE_F32 ? 4 : (t == GS_TYPE_F16 || t == GS_TYPE_BF16 ? 2 : 0); }

@@ -8,7 +8,8 @@ gs_distill.hip; the C entry points are in include/gslim.h):
 Gradients are explicit calls, like everywhere in this package: no autograd.  Every call runs on the current stream of its tensors'
 device (which need not be the current device) and takes its outputs and scratch from torch's allocator there, so it can be captured
 into a graph, and calls on two streams or in two graphs share nothing.  A tensor that another stream writes or frees has to be
-synchronised by the caller, as for any torch call.  Matrices may have any row stride; their rows have to be dense.
+synchronised by the caller, as for any torch call.  Matrices may have any row stride; their rows have to be dense.  An `out` that lies
+on another operand is refused, but for distill_*'s on the whole of the logits.
 """
 from __future__ import annotations
 
@@ -77,6 +78,23 @@ def _vector(name, t, n, dtype):
         _refuse(f"{name} is a dense vector of {n} (got {tuple(t.shape)}, strides {t.stride()})")
 
 
+def _apart(out, ld, **inputs):
+    """Refuses an `out` (row stride ld) that lies on an input: inputs are tensors, dense ones, or (matrix, row stride)."""
+    def span(t, ld=None):
+        e = t.element_size()
+        return (t.data_ptr(), t.shape[0], ld * e, t.shape[1] * e) if ld is not None else (t.data_ptr(), 1, t.numel() * e, t.numel() * e)
+    p, n, s, c = span(out, ld)
+    for name, t in inputs.items():
+        q, m, r, d = span(*t) if isinstance(t, tuple) else span(t)
+        if not (n and m and c and d) or q >= p + (n - 1) * s + c or p >= q + (m - 1) * r + d:
+            continue
+        if (n == 1) != (m == 1) or (n > 1 and s == r):      # columns of one matrix side by side lie apart
+            step = s if n > 1 else r
+            if c <= (q - p) % step <= step - d:
+                continue
+        _refuse(f"out lies on {name}")
+
+
 def _ids(ids):
     if ids.dtype != torch.int32:
         _refuse(f"ids are int32 (got {ids.dtype})")
@@ -123,6 +141,7 @@ def embedding(table, ids, scale=1.0, out=None):
     else:
         _device(table=table, out=out)
         ldo = _matrix("out", out, F, n, table.dtype)
+        _apart(out, ldo, table=(table, ld), ids=ids)
     _launch(dev, _lib.lib().gs_embedding_fwd, table.data_ptr(), ld, table.shape[0], F, TYPES[table.dtype], ids.data_ptr(), n, scale,
             out.data_ptr(), ldo)
     return out
@@ -145,8 +164,9 @@ def embedding_grad(d_out, ids, n_rows, scale=1.0, out=None, accumulate=False, dt
     n_rows, F = int(n_rows), d_out.shape[1]
     if n_rows <= 0:
         _refuse(f"a table of {n_rows} rows")
-    if out is None:
-        if not (not accumulate):
+    given = out is not None
+    if not given:
+        if accumulate:
             _refuse("accumulate=True adds to `out`, which is missing")
         dtype = d_out.dtype if dtype is None else dtype
         if dtype not in (d_out.dtype, torch.float32):
@@ -159,6 +179,8 @@ def embedding_grad(d_out, ids, n_rows, scale=1.0, out=None, accumulate=False, dt
         if out.dtype not in (d_out.dtype, torch.float32):
             _refuse(f"the gradient is {d_out.dtype} or torch.float32 (got {out.dtype})")
     ldw = _matrix("out", out, F, n_rows)
+    if given:
+        _apart(out, ldw, d_out=(d_out, ldd), ids=ids)
     L = _lib.lib()
     scratch = _scratch(L.gs_embedding_bwd_scratch_bytes(n, n_rows, F), dev)
     _launch(dev, L.gs_embedding_bwd, d_out.data_ptr(), ldd, TYPES[d_out.dtype], ids.data_ptr(), n, n_rows, F, scale, bool(accumulate),
@@ -246,11 +268,15 @@ def _distill_args(logits, top_values, top_ids, tau):
     return dev, (logits.data_ptr(), ldz, TYPES[logits.dtype], n, V, top_values.data_ptr(), top_ids.data_ptr(), k, tau), n
 
 
-def _grad_out(logits, out):
+def _grad_out(logits, out, ldz, **inputs):
     if out is None:
         return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[1]
     _device(logits=logits, out=out)
-    return out, _matrix("out", out, logits.shape[1], logits.shape[0], logits.dtype)
+    ld = _matrix("out", out, logits.shape[1], logits.shape[0], logits.dtype)
+    if out.data_ptr() != logits.data_ptr() or ld != ldz:
+        inputs["logits"] = logits, ldz
+    _apart(out, ld, **inputs)
+    return out, ld
 
 
 def distill(logits, top_values, top_ids, tau=1.0):
@@ -270,7 +296,7 @@ def distill_grad(logits, top_values, top_ids, lse, d_loss, tau=1.0, out=None):
     _device(logits=logits, lse=lse, d_loss=d_loss)
     _vector("lse", lse, n, torch.float32)
     _vector("d_loss", d_loss, n, torch.float32)
-    out, ldd = _grad_out(logits, out)
+    out, ldd = _grad_out(logits, out, args[1], top_values=top_values, top_ids=top_ids, lse=lse, d_loss=d_loss)
     _launch(dev, _lib.lib().gs_distill_bwd, *args, lse.data_ptr(), d_loss.data_ptr(), out.data_ptr(), ldd)
     return out
 
@@ -281,7 +307,7 @@ def distill_loss_grad(logits, top_values, top_ids, d_loss, tau=1.0, out=None):
     dev, args, n = _distill_args(logits, top_values, top_ids, tau)
     _device(logits=logits, d_loss=d_loss)
     _vector("d_loss", d_loss, n, torch.float32)
-    out, ldd = _grad_out(logits, out)
+    out, ldd = _grad_out(logits, out, args[1], top_values=top_values, top_ids=top_ids, d_loss=d_loss)
     loss = torch.empty(n, dtype=torch.float32, device=dev)
     _launch(dev, _lib.lib().gs_distill_loss_grad, *args, d_loss.data_ptr(), loss.data_ptr(), out.data_ptr(), ldd)
     return loss, out

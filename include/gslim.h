@@ -305,7 +305,8 @@ int gs_ot_divdiff_f32(float* K, const float* lam, const float* g, const float* g
  * elements; rows may start at any element's address.  `scratch` is device memory of at least the bytes that the call's
  * *_scratch_bytes function names, 16-byte aligned; nothing in it is kept between calls, and calls that may run at the same time
  * (on different streams, or in different captured graphs) need scratch of their own.  No call allocates, synchronises or copies to
- * the host: all of them can be captured into a graph.
+ * the host: all of them can be captured into a graph.  An output that lies on another operand is refused (columns of one matrix side
+ * by side lie apart), but for dZ on the whole of Z.
  * ------------------------------------------------------------------------------------------- */
 #define GS_TYPE_F32 0
 #define GS_TYPE_F16 1
