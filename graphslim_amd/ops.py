@@ -5,7 +5,8 @@ gs_distill.hip; the C entry points are in include/gslim.h):
     gated_ffn, gated_ffn_grad                  h = act(x Wg^T) * (x Wu^T) and its backward pass
     distill, distill_grad, distill_loss_grad   tau^2 KL(teacher's top logits || student) per row and its gradient
 
-Gradients are explicit calls, like everywhere in this package: no autograd.  Every call runs on the current stream of its tensors'
+Gradients are explicit calls, like everywhere in this package: no autograd, and a tensor that requires a gradient is refused while autograd
+records, since its gradient would be lost in silence.  Every call runs on the current stream of its tensors'
 device (which need not be the current device) and takes its outputs and scratch from torch's allocator there, so it can be captured
 into a graph, and calls on two streams or in two graphs share nothing.  A tensor that another stream writes or frees has to be
 synchronised by the caller, as for any torch call.  Matrices may have any row stride; their rows have to be dense.  An `out` that lies
@@ -37,6 +38,8 @@ def _device(**tensors):
     for name, t in tensors.items():
         if not isinstance(t, torch.Tensor):
             _refuse(f"{name} is a tensor (got {type(t).__name__})")
+        if t.requires_grad and torch.is_grad_enabled():
+            _refuse(f"{name} requires a gradient, which these calls do not record: call them under torch.no_grad(), or with {name}.detach()")
         if dev is None:
             dev = t.device
             if dev.type != "cuda":
