@@ -1,6 +1,7 @@
 // Embedding lookup with scaling, and the gradient of its table:
 //   out[t] = s W[id_t]              (0 where id_t is no row of the table: padding)
-//   dW[v]  = s sum_{t : id_t = v} dOut[t], the tokens in ascending order, in fp32, rounded once.
+//   dW[v]  = s sum_{t : id_t = v} dOut[t], in fp32, rounded once: sums of consecutive tokens, in ascending order, added in their order.
+// Where a row's tokens are cut follows from the ids and the sizes, so two runs are bitwise equal.
 #include <algorithm>
 
 #include "gs_types.h"
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(256) void gs_embedding_fwd_kernel(const typename Gs
 // ---- the gradient ---------------------------------------------------------------------------------------------------------------
 // The table is cut into buckets of R consecutive rows.  The tokens of a bucket, sorted by row (stable, so ascending within a row), are
 // walked by the waves of one workgroup, each on columns of its own: a run of one row is summed in registers and written once, rows
-// without tokens are written as zeros, and nothing is joined between waves.
+// without tokens are written as zeros.
 //   few tokens:  one launch, every workgroup picks its bucket's tokens out of all ids itself.
 //   many:        gs_embedding_count / _place sort the tokens by bucket first; a bucket of more than EM_SPAN tokens (a frequent id) is
 //                cut into spans with a workgroup each, whose sums gs_embedding_join adds in the spans' order.

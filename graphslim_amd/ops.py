@@ -151,9 +151,10 @@ def embedding(table, ids, scale=1.0, out=None):
 
 
 def embedding_grad(d_out, ids, n_rows, scale=1.0, out=None, accumulate=False, dtype=None):
-    """Gradient [n_rows, width] of `embedding`'s table: scale times the sum of d_out's rows of each id, in ascending order.  d_out:
-    ids.shape + (width,), or [ids.numel(), width] with any row stride.  dtype: that of d_out (default) or torch.float32.  `out`
-    receives the gradient; with accumulate=True it is added to what `out` holds."""
+    """Gradient [n_rows, width] of `embedding`'s table: scale times the sum of d_out's rows of each id.  The sum is
+    one of partial sums of consecutive tokens, cut where the ids and the sizes say: two runs are bitwise equal.  d_out: ids.shape +
+    (width,), or [ids.numel(), width] with any row stride.  dtype: that of d_out (default) or torch.float32.  `out` receives the gradient;
+    with accumulate=True it is added to what `out` holds."""
     dev = _device(d_out=d_out, ids=ids)
     _ids(ids)
     n = ids.numel()

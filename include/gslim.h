@@ -316,8 +316,9 @@ int gs_ot_divdiff_f32(float* K, const float* lam, const float* g, const float* g
  * The typed, scaled form of gs_gather_rows_f32. */
 int gs_embedding_fwd(const void* W, long ldw, long n_rows, int F, int type, const int* ids, long n, float scale, void* out, long ldo,
                      gs_stream_t stream);
-/* dW[v] = scale * sum of dout[t] over the t with ids[t] == v, in ascending t (+ dW[v] when `accumulate`); rows that no id names get
- * 0 (or stay).  type_dw: that of dout, or GS_TYPE_F32.  gs_segment_sum_rows_f32 with the permutation built on the device. */
+/* dW[v] = scale * sum of dout[t] over the t with ids[t] == v (+ dW[v] when `accumulate`); rows that no id names get 0 (or stay).  The sum
+ * is one of partial sums, each over consecutive t in ascending order, added in that order; where they are cut follows from the ids and
+ * the sizes.  type_dw: that of dout, or GS_TYPE_F32.  gs_segment_sum_rows_f32 with the permutation built on the device. */
 size_t gs_embedding_bwd_scratch_bytes(long n, long n_rows, int F);
 int gs_embedding_bwd(const void* dout, long ldd, int type, const int* ids, long n, long n_rows, int F, float scale, int accumulate,
                      void* dW, long ldw, int type_dw, void* scratch, gs_stream_t stream);
