@@ -337,8 +337,10 @@ int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, 
                  void* h, long ldh, float* saved, void* scratch, gs_stream_t stream);
 /* dg = dh * u * act'(g), du = dh * act(g); dx = dg Wg + du Wu, dw_gate = dg^T x, dw_up = du^T x.  For 16-bit types dg and du enter the
  * products as two bf16 parts: to 2^-17 of each and with fp32's range, so that a slope that fp16 does not hold leaves the gradients right.
- * fp32 products of more than a few rows are six products of bf16 parts: as exact as fp32 (parts have a smallest step of 2^-133), but an
- * infinite operand gives NaN where it meets a zero part. */
+ * fp32 products (forward: of more than 24 rows) are six products of bf16 parts: as exact as fp32 (parts have a smallest step of 2^-133).
+ * Operands that are not finite: what they enter by the formulas is not finite, nothing else is touched.  Where products are made of
+ * parts (fp32, and the backward call in every type), or a size is no multiple of 64, it can be NaN where the formula gives an infinity,
+ * since an infinity meets a zero there; the forward call keeps infinities in 16 bits, and in fp32 up to 24 rows. */
 size_t gs_gated_bwd_scratch_bytes(long M, long D, long F, int type, int plain);
 int gs_gated_bwd(const void* dh, long lddh, const void* x, long ldx, const void* w_gate, const void* w_up, long ldw, const float* saved,
                  int type, long M, long D, long F, int act, void* dx, long lddx, void* dw_gate, void* dw_up, long lddw, void* scratch,
