@@ -62,7 +62,7 @@ template <typename E>
 struct DistillTeacher {
   static constexpr int WORDS = 4;   // of LDS per entry
   int* c;       // [k rounded up to 4] class or -1
-  float* v;     // [k] t / tau, then log p
+  float* v;     // [k] t, then log p
   float* r;     // [k] gradient at the entry's class, if the entry is the first of that class
   int* at;      // [k] that class, else -1
   int c0;       // the first 64 entries: their loads come before the row's, so that they need not wait for it
@@ -98,7 +98,6 @@ struct DistillTeacher {
       const bool ok = cj >= 0 && cj < a.V && vj != -INFINITY;
       have |= ok;
       if (first && j < k4) {
-        vj /= a.tau;
         c[j] = ok ? cj : -1;
         v[j] = vj;
         if (ok) top = fmaxf(top, vj);
@@ -108,19 +107,25 @@ struct DistillTeacher {
     if (!first) return;
     top = gs_wave_max(top);
     float s = 0.f;
-    for (int j = lane; j < a.k; j += 64)
-      if (c[j] >= 0) s += ds_exp(v[j] - top);
+    for (int j = lane; j < a.k; j += 64) {
+      v[j] = (v[j] - top) / a.tau;                        // (in this order: t / tau may lie beyond fp32)
+      if (c[j] >= 0) s += ds_exp(v[j]);
+    }
     const float log_sum = logf(gs_wave_sum(s));
-    for (int j = lane; j < a.k; j += 64) v[j] = v[j] - top - log_sum;
+    for (int j = lane; j < a.k; j += 64) v[j] -= log_sum;
   }
 
-  // sum of p (log p - log q) over the entries
-  __device__ __forceinline__ float loss(const DistillArgs& a, const E* z, int lane, float lse) {
+  // sum of p (log p - log q) over the entries, with log q = (z - m) / tau - log_s from the row's maximum m and its sum: the log-sum m / tau
+  // + log_s may lie beyond fp32, or hold nothing of log_s
+  __device__ __forceinline__ float loss(const DistillArgs& a, const E* z, int lane, float m, float log_s) {
     float s = 0.f;
     for (int j = lane; j < a.k; j += 64)
       if (c[j] >= 0) {
         const float p = ds_exp(v[j]);
-        if (p != 0.f) s += p * (v[j] - ds_logq(a, (float)z[c[j]], lse));
+        const float zc = (float)z[c[j]], d = zc - m;
+        float logq = fmaf(d, a.inv_lo, fmaf(d, a.inv_hi, -log_s));
+        if (d == -INFINITY) logq = zc == -INFINITY ? zc : d - log_s;   // a masked class; a difference beyond fp32
+        if (p != 0.f) s += p * (v[j] - logq);
       }
     return gs_wave_sum(s);
   }
@@ -219,8 +224,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void gs_distill_regs_kernel(Dist
   s += end;
   s = ds_reduce<G, false>(s, red[1]);
   if (first) {
-    const float lse = m / a.tau + logf(s);
-    const float sum = t.loss(a, z, lane, lse);
+    const float log_s = logf(s), lse = m / a.tau + log_s;
+    const float sum = t.loss(a, z, lane, m, log_s);
     if (lane == 0 && live) {
       a.loss[row] = t.any ? a.tau * a.tau * sum : 0.f;
       if (a.lse) a.lse[row] = lse;
@@ -271,7 +276,7 @@ __global__ __launch_bounds__(G) void gs_distill_row_kernel(DistillArgs a) {
   t.look(a, row, lane, first);
   const bool zero = GRAD && (!t.any || w == 0.f);
   const float c = a.inv_hi * DS_LOG2E;
-  float m = 0.f, s = 0.f;
+  float m = 0.f, s = 0.f, log_s = 0.f;
   if (STATS) {
     m = -INFINITY;
     auto add = [&](float mx, auto each) {                 // values whose maximum is mx
@@ -309,7 +314,8 @@ __global__ __launch_bounds__(G) void gs_distill_row_kernel(DistillArgs a) {
     if (all == -INFINITY) all = 0.f;
     s = ds_reduce<G, false>(s * __builtin_amdgcn_exp2f((m - all) * c), red[1]);
     m = all;
-    lse = m / a.tau + logf(s);
+    log_s = logf(s);
+    lse = m / a.tau + log_s;
   }
   auto q_of = [&](float v) {
     if (STATS) return __builtin_amdgcn_exp2f((v - m) * c);
@@ -318,7 +324,7 @@ __global__ __launch_bounds__(G) void gs_distill_row_kernel(DistillArgs a) {
   const float over = STATS ? (s == 0.f ? 0.f : 1.f / s) : (lse == -INFINITY ? 0.f : (lse == lse ? 1.f : lse)), ws = w * over;
   if (first) {
     if (LOSS) {
-      const float sum = t.loss(a, z, lane, lse);
+      const float sum = t.loss(a, z, lane, m, log_s);
       if (lane == 0) {
         a.loss[row] = t.any ? a.tau * a.tau * sum : 0.f;
         if (a.lse) a.lse[row] = lse;

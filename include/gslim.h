@@ -354,7 +354,7 @@ int gs_gated_bwd(const void* dh, long lddh, const void* x, long ldx, const void*
  * counterpart of gs_softmax_nll_grad_f32; dZ may be Z (with its stride).
  * gs_distill_fwd also writes lse[i] = log sum_v exp(Z[i][v] / tau), which gs_distill_bwd takes; gs_distill_loss_grad is both at
  * once for row weights that are known beforehand (1 / n).  (lse is one fp32: the gradient from it resolves q to about 2^-24 |lse|,
- * which says nothing for a row whose every logit is the type's lowest value; gs_distill_loss_grad has no such limit.) */
+ * which says nothing for a row whose every logit is the type's lowest value; the losses and gs_distill_loss_grad have no such limit.) */
 int gs_distill_fwd(const void* Z, long ldz, int type, long n, int V, const void* top_val, const int* top_cls, int k, float tau,
                    float* loss, float* lse, gs_stream_t stream);
 int gs_distill_bwd(const void* Z, long ldz, int type, long n, int V, const void* top_val, const int* top_cls, int k, float tau,
