@@ -422,7 +422,7 @@ int ds_run(const char* who, DistillArgs a, int type, long n, hipStream_t s) {
   if (n > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "%s: rows are counted in 32 bits", who);
   if (!(a.tau > 0.f) || !(a.tau < INFINITY)) GS_FAIL(GS_ERR_ARG, "%s: temperature %g", who, (double)a.tau);
   if (a.ldz < a.V || (a.dZ && a.ldd < a.V)) GS_FAIL(GS_ERR_ARG, "%s: a row stride is below the %d classes", who, a.V);
-  if (!(1.f / a.tau < INFINITY)) GS_FAIL(GS_ERR_ARG, "%s: temperature %g has no reciprocal in fp32", who, (double)a.tau);
+  if (!(1.f / a.tau * DS_LOG2E < INFINITY)) GS_FAIL(GS_ERR_ARG, "%s: temperature %g has no reciprocal in fp32", who, (double)a.tau);
   if (a.dZ && a.dZ == a.Z && a.ldd != a.ldz) GS_FAIL(GS_ERR_ARG, "%s: in place with row strides %ld and %ld", who, a.ldz, a.ldd);
   if (n == 0) return GS_OK;
   if (!a.Z || !a.tv || !a.ti) GS_FAIL(GS_ERR_ARG, "%s: null pointer", who);

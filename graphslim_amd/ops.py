@@ -267,7 +267,7 @@ def _distill_args(logits, top_values, top_ids, tau):
         _refuse(f"top_ids are {tuple(top_ids.shape)}, top_values {(n, k)}")
     _ids(top_ids)
     tau = float(tau)
-    if not (0 < tau < math.inf):
+    if not (0 < tau <= torch.finfo(torch.float32).max and math.log2(math.e) / tau < torch.finfo(torch.float32).max):   # what fp32 holds
         _refuse(f"a temperature of {tau}")
     return dev, (logits.data_ptr(), ldz, TYPES[logits.dtype], n, V, top_values.data_ptr(), top_ids.data_ptr(), k, tau), n
 
