@@ -686,6 +686,9 @@ extern "C" int gs_embedding_bwd(const void* dout, long ldd, int type, const int*
   const GsSpan w = gs_span(dW, V, ldw, F, gs_type_bytes(type_dw));
   if (n > 0 && (gs_overlap(w, gs_span(dout, n, ldd, F, gs_type_bytes(type))) || gs_overlap(w, gs_span(ids, n, 4))))
     GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: the gradient lies on another operand");
+  const EmbPlan p = emb_plan(n, std::min(V, EM_MAX_V), F);
+  if (((p.direct ? 0L : p.extra) + p.nb) * (p.direct ? 1024 : 512) > 0xffffffffL)
+    GS_FAIL(GS_ERR_UNSUPPORTED, "gs_embedding_bwd: %ld ids are beyond one launch", n);
   if (gs_embedding_bwd_scratch_bytes(n, V, F) > 0 && (!scratch || ((size_t)scratch & 15)))
     GS_FAIL(GS_ERR_ARG, "gs_embedding_bwd: the scratch is missing or not 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;

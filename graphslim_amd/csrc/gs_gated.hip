@@ -28,7 +28,8 @@ typedef const __attribute__((address_space(1))) void* gbl_ptr;
 
 constexpr int GF_PAD = 64;   // rows of laid-out operands are multiples of this many elements
 
-constexpr long GF_MAX_BLOCKS = 0xffffffL;   // of 256 threads that count their work in 32 bits
+constexpr long GF_MAX_THREADS = 0xffffffffL;   // of a launch
+constexpr long GF_MAX_BLOCKS = 0xffffffL;      // of 256 threads
 
 inline long gf_up(long n) { return (n + GF_PAD - 1) / GF_PAD * GF_PAD; }
 
@@ -893,9 +894,9 @@ int gf_lds(Kernel kern, int bytes, std::atomic<unsigned long long>& known) {
 }
 
 // Sets a product's slices; its tiles of BM x BN, or an error
-int gf_prepare(GatedGemm& q, const GatedSplit& sp, int BM, int BN, bool gated, float* part, long* tiles) {
+int gf_prepare(GatedGemm& q, const GatedSplit& sp, int BM, int BN, int threads, bool gated, float* part, long* tiles) {
   const long gx = (q.M + BM - 1) / BM, gy = (q.N + BN - 1) / BN;
-  if (gx * gy * sp.slices > 0x1fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", q.M, q.N);
+  if (gx * gy * sp.slices * threads > GF_MAX_THREADS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", q.M, q.N);
   q.gx = (int)gx;
   q.kslice = sp.kslice;
   if (sp.slices > 1) {
@@ -915,7 +916,7 @@ int gf_tile(GatedGemm q, const GatedSplit& sp, float* part, hipStream_t s) {
   static std::atomic<unsigned long long> known{0};
   GS_TRY(gf_lds(kern, LDS, known));
   long tiles;
-  GS_TRY(gf_prepare(q, sp, BM, BN, GATED, part, &tiles));
+  GS_TRY(gf_prepare(q, sp, BM, BN, WM * WN * 64, GATED, part, &tiles));
   kern<<<dim3((unsigned)tiles, (unsigned)sp.slices), dim3(WM * WN * 64), LDS, s>>>(q);
   GS_LAUNCH_CHECK();
   if (sp.slices > 1) {
@@ -948,12 +949,13 @@ int gf_pair_tile(GatedGemm a, GatedGemm b, const GatedPair& p, float* part, hipS
   static std::atomic<unsigned long long> known{0};
   GS_TRY(gf_lds(kern, LDS, known));
   long ta, tb;
-  GS_TRY(gf_prepare(a, p.dx, BM, BN, false, part, &ta));
-  GS_TRY(gf_prepare(b, p.dw, BM, BN, false, part + p.dx.part, &tb));
+  GS_TRY(gf_prepare(a, p.dx, BM, BN, WM * WN * 64, false, part, &ta));
+  GS_TRY(gf_prepare(b, p.dw, BM, BN, WM * WN * 64, false, part + p.dx.part, &tb));
+  if ((ta * p.dx.slices + tb * p.dw.slices) * WM * WN * 64 > GF_MAX_THREADS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", b.M, b.N);
   kern<<<dim3((unsigned)(ta * p.dx.slices + tb * p.dw.slices)), dim3(WM * WN * 64), LDS, s>>>(a, (unsigned)ta, (unsigned)(ta * p.dx.slices), b, (unsigned)tb);
   GS_LAUNCH_CHECK();
   const long ja = p.dx.slices > 1 ? gf_join_blocks(a) : 0, jb = p.dw.slices > 1 ? gf_join_blocks(b) : 0;
-  if (std::max(ja, jb) > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", b.M, b.N);
+  if (ja + jb > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated: %ld x %ld is beyond one launch", b.M, b.N);
   if (ja + jb) {
     gs_gated_join_pair_kernel<T><<<dim3((unsigned)(ja + jb)), dim3(256), 0, s>>>(a, p.dx.slices, (unsigned)ja, b, p.dw.slices);
     GS_LAUNCH_CHECK();
@@ -1021,6 +1023,7 @@ inline bool gf_few(long M, int type) { return M <= (type == GS_TYPE_F32 ? 24 : 4
 template <int T, int MB>
 int gf_rows(const GatedCall& c, hipStream_t s) {
   constexpr int RF = 2;
+  if ((c.F + 4 * RF - 1) / (4 * RF) > GF_MAX_BLOCKS) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated_fwd: weights of %ld rows are beyond one launch", c.F);
   GatedRows q = {c.x, c.wg, c.wu, c.ldx, c.ldw, c.M, c.D, c.F, c.ldh, c.h, c.saved, c.act};
   gs_gated_rows_kernel<T, MB, RF><<<dim3((unsigned)((c.F + 4 * RF - 1) / (4 * RF)), (unsigned)((c.M + MB - 1) / MB)), dim3(256), 0, s>>>(q);
   GS_LAUNCH_CHECK();
@@ -1085,17 +1088,16 @@ int gf_bwd(const GatedCall& c, hipStream_t s) {
 // dW = 0 where there are no tokens
 template <typename E>
 __global__ void gs_gated_zero_kernel(E* a, E* b, long R, long C, long ld) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= R * C) return;
-  a[i / C * ld + i % C] = (E)0.f;
-  b[i / C * ld + i % C] = (E)0.f;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < R * C; i += (long)gridDim.x * 256) {
+    a[i / C * ld + i % C] = (E)0.f;
+    b[i / C * ld + i % C] = (E)0.f;
+  }
 }
 
 template <int T>
 int gf_empty(const GatedCall& c, hipStream_t s) {
   typedef typename GsElt<T>::type E;
-  if ((c.F * c.D + 255) / 256 > 0x7fffffffL) GS_FAIL(GS_ERR_UNSUPPORTED, "gs_gated_bwd: weights of %ld x %ld are beyond one launch", c.F, c.D);
-  gs_gated_zero_kernel<E><<<dim3((unsigned)((c.F * c.D + 255) / 256)), dim3(256), 0, s>>>((E*)c.dwg, (E*)c.dwu, c.F, c.D, c.lddw);
+  gs_gated_zero_kernel<E><<<dim3((unsigned)std::min((c.F * c.D + 255) / 256, 65536L)), dim3(256), 0, s>>>((E*)c.dwg, (E*)c.dwu, c.F, c.D, c.lddw);
   GS_LAUNCH_CHECK();
   return GS_OK;
 }
