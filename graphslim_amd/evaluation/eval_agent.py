@@ -1,5 +1,7 @@
 """Evaluator of the reference (graphslim/evaluation/eval_agent.py:159-291) for the GCN evaluation model: `run_eval`
 seeded runs, each trains the GCN on the condensed graph (HIP ops) and tests on the full graph."""
+import copy
+
 import numpy as np
 from tqdm import trange
 
@@ -27,8 +29,10 @@ class Evaluator:
         k = int(getattr(args, "soft_label", 0) or 0)
         if getattr(args, "eval_loss", "CE") != "KLD" or k <= 0:
             return None
-        seed_everything(args.seed)              # the same teacher on every rank
-        model = _MODELS[model_type](data.feat_full.shape[1], args.hidden, data.nclass, evaluation_args(args), mode="eval")
+        seed_everything(args.seed)              # the same teacher on every rank, trained on the whole graph by each ...
+        own = copy.copy(evaluation_args(args))
+        own.eval_row_shard = None               # ... also after a row-sharded `evaluate` with these args
+        model = _MODELS[model_type](data.feat_full.shape[1], args.hidden, data.nclass, own, mode="eval")
         model.fit_with_val(data, train_iters=args.eval_epochs, normadj=True, verbose=verbose, setting=args.setting, reduced=False)
         return model.top_logits(data.feat_syn, data.adj_syn, k, float(getattr(args, "soft_tau", 1.0)))
 
