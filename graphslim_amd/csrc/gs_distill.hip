@@ -10,7 +10,7 @@
 namespace {
 
 constexpr int DS_MAX_TOP = 1024;
-constexpr float DS_LOG2E = 1.4426950408889634f;
+constexpr float DS_LOG2E = 1.4426950408889634f, DS_LOG2E_REST = (float)(1.4426950408889634 - (double)DS_LOG2E), DS_LN2 = 0.69314718055994531f;
 
 struct DistillArgs {
   const void* Z;
@@ -19,6 +19,7 @@ struct DistillArgs {
   const void* tv;
   const int* ti;
   float tau, inv_hi, inv_lo;   // 1 / tau as a sum of two floats: z / tau enters differences with the log-sum, whose error is absolute
+  float c_hi, c_lo;            // log2(e) / tau, too
   const float* lse_in;
   const float* w;
   float* loss;
@@ -27,7 +28,16 @@ struct DistillArgs {
   long ldd;
 };
 
-__device__ __forceinline__ float ds_exp(float x) { return __builtin_amdgcn_exp2f(x * DS_LOG2E); }
+// 2^(d (hi + lo)) for d <= 0.  FULL: with what the product d hi rounds away, up to 2^-24 |d hi| of the result; fp32 gradients show it,
+// 16-bit ones do not, and there the exponentials are half of the time.
+template <bool FULL>
+__device__ __forceinline__ float ds_pow(float d, float hi, float lo) {
+  const float t = d * hi, r = __builtin_amdgcn_exp2f(t);
+  if constexpr (!FULL) return r;
+  const float rest = fmaf(d, lo, fmaf(d, hi, -t));
+  return t < -160.f ? 0.f : fmaf(r, rest * DS_LN2, r);
+}
+__device__ __forceinline__ float ds_exp(float x) { return ds_pow<true>(x, DS_LOG2E, DS_LOG2E_REST); }
 
 // log q = z / tau - lse; a masked class (-inf) stays at -inf whatever the log-sum is
 __device__ __forceinline__ float ds_logq(const DistillArgs& a, float z, float lse) {
@@ -199,11 +209,10 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void gs_distill_regs_kernel(Dist
     for (int e = 0; e < N; ++e) m = fmaxf(m, (float)raw[i][e]);
   m = ds_reduce<G, true>(m, red[0]);
   if (m == -INFINITY) m = 0.f;
-  const float c = a.inv_hi * DS_LOG2E;                     // (x - m first: x c - m c would be off by an ulp of m c)
-  auto e_of = [&](float v) { return __builtin_amdgcn_exp2f((v - m) * c); };
+  constexpr bool KEEP = sizeof(E) == 4;
+  auto e_of = [&](float v) { return ds_pow<KEEP>(v - m, a.c_hi, a.c_lo); };   // (x - m first: x c - m c would be off by an ulp of m c)
   // fp32 rows keep the exponentials in place; 16-bit rows stay packed, half the registers, and are converted and raised again in each
   // pass (opaque in between, or the compiler keeps what it has seen, in 32 bits)
-  constexpr bool KEEP = sizeof(E) == 4;
   auto hide = [&] {
     if constexpr (!KEEP) {
 #pragma unroll
@@ -275,14 +284,14 @@ __global__ __launch_bounds__(G) void gs_distill_row_kernel(DistillArgs a) {
   if (!STATS) lse = a.lse_in[row];
   t.look(a, row, lane, first);
   const bool zero = GRAD && (!t.any || w == 0.f);
-  const float c = a.inv_hi * DS_LOG2E;
+  constexpr bool FULL = sizeof(E) == 4;
   float m = 0.f, s = 0.f, log_s = 0.f;
   if (STATS) {
     m = -INFINITY;
     auto add = [&](float mx, auto each) {                 // values whose maximum is mx
       mx = fmaxf(mx, m);
       const float ref = mx == -INFINITY ? 0.f : mx;
-      s *= __builtin_amdgcn_exp2f((m - ref) * c);
+      s *= ds_pow<FULL>(m - ref, a.c_hi, a.c_lo);
       each(ref);
       m = mx;
     };
@@ -303,23 +312,23 @@ __global__ __launch_bounds__(G) void gs_distill_row_kernel(DistillArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int e = 0; e < N; ++e) s += __builtin_amdgcn_exp2f(((float)r[u][e] - ref) * c);
+          for (int e = 0; e < N; ++e) s += ds_pow<FULL>((float)r[u][e] - ref, a.c_hi, a.c_lo);
       });
     }
     if (has_end) {
       const float v = (float)z[full * N + g];
-      add(v, [&](float ref) { s += __builtin_amdgcn_exp2f((v - ref) * c); });
+      add(v, [&](float ref) { s += ds_pow<FULL>(v - ref, a.c_hi, a.c_lo); });
     }
     float all = ds_reduce<G, true>(m, red[0]);
     if (all == -INFINITY) all = 0.f;
-    s = ds_reduce<G, false>(s * __builtin_amdgcn_exp2f((m - all) * c), red[1]);
+    s = ds_reduce<G, false>(s * ds_pow<FULL>(m - all, a.c_hi, a.c_lo), red[1]);
     m = all;
     log_s = logf(s);
     lse = m / a.tau + log_s;
   }
   auto q_of = [&](float v) {
-    if (STATS) return __builtin_amdgcn_exp2f((v - m) * c);
-    return ds_exp(fminf(ds_logq(a, v, lse), 0.f));        // (a log-sum of 1e38 in fp32 is off by more than any exponent)
+    if (STATS) return ds_pow<FULL>(v - m, a.c_hi, a.c_lo);
+    return ds_pow<FULL>(fminf(ds_logq(a, v, lse), 0.f), DS_LOG2E, DS_LOG2E_REST);        // (a log-sum of 1e38 in fp32 is off by more than any exponent)
   };
   const float over = STATS ? (s == 0.f ? 0.f : 1.f / s) : (lse == -INFINITY ? 0.f : (lse == lse ? 1.f : lse)), ws = w * over;
   if (first) {
@@ -439,6 +448,8 @@ int ds_run(const char* who, DistillArgs a, int type, long n, hipStream_t s) {
   if (clash) GS_FAIL(GS_ERR_ARG, "%s: an output lies on another operand (only dZ may, on all of Z)", who);
   a.inv_hi = 1.f / a.tau;
   a.inv_lo = (float)(1.0 / (double)a.tau - (double)a.inv_hi);
+  a.c_hi = (float)(1.4426950408889634 / (double)a.tau);
+  a.c_lo = (float)(1.4426950408889634 / (double)a.tau - (double)a.c_hi);
   if (type == GS_TYPE_F32) return ds_launch<GS_TYPE_F32>(a, s);
   if (type == GS_TYPE_F16) return ds_launch<GS_TYPE_F16>(a, s);
   return ds_launch<GS_TYPE_BF16>(a, s);
@@ -449,20 +460,20 @@ int ds_run(const char* who, DistillArgs a, int type, long n, hipStream_t s) {
 extern "C" int gs_distill_fwd(const void* Z, long ldz, int type, long n, int V, const void* top_val, const int* top_cls, int k, float tau,
                               float* loss, float* lse, gs_stream_t stream) {
   if (n > 0 && (!loss || !lse)) GS_FAIL(GS_ERR_ARG, "gs_distill_fwd: null pointer");
-  DistillArgs a = {Z, ldz, n, V, k, top_val, top_cls, tau, 0.f, 0.f, nullptr, nullptr, loss, lse, nullptr, 0};
+  DistillArgs a = {Z, ldz, n, V, k, top_val, top_cls, tau, 0.f, 0.f, 0.f, 0.f, nullptr, nullptr, loss, lse, nullptr, 0};
   return ds_run("gs_distill_fwd", a, type, n, (hipStream_t)stream);
 }
 
 extern "C" int gs_distill_bwd(const void* Z, long ldz, int type, long n, int V, const void* top_val, const int* top_cls, int k, float tau,
                               const float* lse, const float* d_loss, void* dZ, long ldd, gs_stream_t stream) {
   if (n > 0 && (!lse || !d_loss || !dZ)) GS_FAIL(GS_ERR_ARG, "gs_distill_bwd: null pointer");
-  DistillArgs a = {Z, ldz, n, V, k, top_val, top_cls, tau, 0.f, 0.f, lse, d_loss, nullptr, nullptr, dZ, ldd};
+  DistillArgs a = {Z, ldz, n, V, k, top_val, top_cls, tau, 0.f, 0.f, 0.f, 0.f, lse, d_loss, nullptr, nullptr, dZ, ldd};
   return ds_run("gs_distill_bwd", a, type, n, (hipStream_t)stream);
 }
 
 extern "C" int gs_distill_loss_grad(const void* Z, long ldz, int type, long n, int V, const void* top_val, const int* top_cls, int k,
                                     float tau, const float* d_loss, float* loss, void* dZ, long ldd, gs_stream_t stream) {
   if (n > 0 && (!d_loss || !loss || !dZ)) GS_FAIL(GS_ERR_ARG, "gs_distill_loss_grad: null pointer");
-  DistillArgs a = {Z, ldz, n, V, k, top_val, top_cls, tau, 0.f, 0.f, nullptr, d_loss, loss, nullptr, dZ, ldd};
+  DistillArgs a = {Z, ldz, n, V, k, top_val, top_cls, tau, 0.f, 0.f, 0.f, 0.f, nullptr, d_loss, loss, nullptr, dZ, ldd};
   return ds_run("gs_distill_loss_grad", a, type, n, (hipStream_t)stream);
 }

@@ -78,3 +78,24 @@ def test_infinite_logits(ops):
     assert torch.isnan(loss[1]) and torch.isnan(ops.distill(z.to(DEV), tv.to(DEV), ti.to(DEV), 0.5)[0][1])
     for t, was in ((loss, clean[0]), (grad, clean[1])):
         assert torch.equal(t[[0, 2]], was[[0, 2]])
+
+
+@pytest.mark.parametrize("V", ROWS)
+@pytest.mark.parametrize("tau", [1.0, 1.5])
+def test_small_probabilities_of_fp32_rows(ops, V, tau):
+    """One class at 0 and the others at -30 to -80, in quarters: the sum is 1 to 2^-24, differences are exact, and an exponential is off by its
+    own step of 2^-23 however small it is.  With the two roundings of w tau / s, the product and the sum: 12 of 2^-24."""
+    g = gen("small", V)
+    z = -torch.randint(120, 321, (4, V), generator=g).float() / 4 * tau
+    z[:, 0] = 0
+    tv, ti = torch.zeros(4, 1), torch.zeros(4, 1, dtype=torch.int32)
+    w = torch.rand(4, generator=g) + 0.5
+    q = torch.softmax(z.double() / tau, 1)[:, 1:]
+    want = q * w.double()[:, None] * tau
+    assert q.max() < 1e-12 and q.min() > 1e-36
+    args = z.to(DEV), tv.to(DEV), ti.to(DEV)
+    grad = ops.distill_loss_grad(*args, w.to(DEV), tau)[1][:, 1:]
+    close(grad, want, 12 * U * want, "gradient of the call for both")
+    # z / tau - lse is rounded once more, by 2^-24 of up to 80
+    grad = ops.distill_grad(*args, ops.distill(*args, tau)[1], w.to(DEV), tau)[:, 1:]
+    close(grad, want, (12 + 80) * U * want, "gradient")
