@@ -1036,7 +1036,10 @@ int gf_fwd(const GatedCall& c, hipStream_t s) {
   if (gf_few(c.M, T)) {
     if (c.M == 1) return gf_rows<T, 1>(c, s);
     if (c.M == 2) return gf_rows<T, 2>(c, s);
-    return c.M <= 4 ? gf_rows<T, 4>(c, s) : gf_rows<T, 8>(c, s);
+    if constexpr (T == GS_TYPE_F32) {
+      if (c.M > 4) return gf_rows<T, 8>(c, s);
+    }
+    return gf_rows<T, 4>(c, s);
   }
   const bool plain = gf_plain(c.x, c.ldx, c.wg, c.wu, c.ldw, c.D);
   const GatedPlan p = gf_plan(c.M, c.D, c.F, T, plain, false);
