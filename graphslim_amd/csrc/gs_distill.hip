@@ -37,7 +37,10 @@ __device__ __forceinline__ float ds_pow(float d, float hi, float lo) {
   const float rest = fmaf(d, lo, fmaf(d, hi, -t));
   return t < -160.f ? 0.f : fmaf(r, rest * DS_LN2, r);
 }
-__device__ __forceinline__ float ds_exp(float x) { return ds_pow<true>(x, DS_LOG2E, DS_LOG2E_REST); }
+template <typename E>
+__device__ __forceinline__ float ds_exp(float x) {
+  return ds_pow<sizeof(E) == 4>(x, DS_LOG2E, DS_LOG2E_REST);
+}
 
 // log q = z / tau - lse; a masked class (-inf) stays at -inf whatever the log-sum is
 __device__ __forceinline__ float ds_logq(const DistillArgs& a, float z, float lse) {
@@ -119,7 +122,7 @@ struct DistillTeacher {
     float s = 0.f;
     for (int j = lane; j < a.k; j += 64) {
       v[j] = (v[j] - top) / a.tau;                        // (in this order: t / tau may lie beyond fp32)
-      if (c[j] >= 0) s += ds_exp(v[j]);
+      if (c[j] >= 0) s += ds_exp<E>(v[j]);
     }
     const float log_sum = logf(gs_wave_sum(s));
     for (int j = lane; j < a.k; j += 64) v[j] -= log_sum;
@@ -131,7 +134,7 @@ struct DistillTeacher {
     float s = 0.f;
     for (int j = lane; j < a.k; j += 64)
       if (c[j] >= 0) {
-        const float p = ds_exp(v[j]);
+        const float p = ds_exp<E>(v[j]);
         const float zc = (float)z[c[j]], d = zc - m;
         float logq = fmaf(d, a.inv_lo, fmaf(d, a.inv_hi, -log_s));
         if (d == -INFINITY) logq = zc == -INFINITY ? zc : d - log_s;   // a masked class; a difference beyond fp32
@@ -156,7 +159,7 @@ struct DistillTeacher {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (cs[e] == cj) {
-              p += ds_exp(v[o + e]);
+              p += ds_exp<E>(v[o + e]);
               first &= o + e >= j;
             }
         }
