@@ -314,17 +314,28 @@ __device__ __forceinline__ E* gf_row(const GatedGemm& q, long m) {
 __device__ __forceinline__ f32x4 gf_mfma(h16x8 a, h16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 gf_mfma(b16x8 a, b16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// eight fp16 as bf16: what a bf16 holds of them, or the rest
-__device__ __forceinline__ b16x8 gf_part(b16x8 bits, bool rest) {
+// Eight fp16 as bf16: what a bf16 holds of them, or the 3 bits that are left.  In pairs, since one instruction rounds two; what is left is
+// exact, so a byte permutation packs it.
+template <bool REST>
+__device__ __forceinline__ b16x8 gf_part(b16x8 bits) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
   const h16x8 w = __builtin_bit_cast(h16x8, bits);
-  b16x8 r;
+  u32x4 r;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float f = (float)w[e];
-    r[e] = (__bf16)f;
-    if (rest) r[e] = (__bf16)(f - (float)r[e]);
+  for (int e = 0; e < 8; e += 2) {
+    const f32x2 v = {(float)w[e], (float)w[e + 1]};
+    const unsigned first = __builtin_bit_cast(unsigned, __builtin_convertvector(v, b16x2));
+    if (REST) {
+      const float lo = v[0] - __uint_as_float(first << 16), hi = v[1] - __uint_as_float(first & 0xffff0000u);
+      r[e / 2] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302);
+    } else {
+      r[e / 2] = first;
+    }
+    asm volatile("" : "+v"(r[e / 2]));   // (pair after pair: all at once would take more registers than there are)
   }
-  return r;
+  return __builtin_bit_cast(b16x8, r);
 }
 
 template <int N, typename Fn>
@@ -433,7 +444,7 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
   const P* srcA[ITA];
   int colA[ITA];
   int colB[ITB];        // of a chunk in its row
-  long srcB[ITB], endB[ITB];   // offsets from B's base; from that of the step with B's last rows, where they are fewer than BK
+  long srcB[ITB];       // offsets from B's base
 #pragma unroll
   for (int i = 0; i < ITA; ++i) {
     const int s = i * NT + tid, r = s / CA, c = (s % CA) ^ gf_swz<TA, BK>(r);
@@ -448,7 +459,6 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
     const long in_row = TB ? min(n0 + c * 8, q.bcols - 8) : (RAW ? 0 : c * 8);   // (RAW, k contiguous: the column comes with the step)
     colB[i] = c * 8;
     srcB[i] = (TB ? r * q.ldb : (long)(base + min(n, q.N - 1) * q.ldb - (const P*)q.B[0])) + in_row;
-    endB[i] = TB ? min((long)r, (q.brows - 1) % BK) * q.ldb + in_row : 0;
   }
   static_assert(!RAW || (!TA && !TB), "rows of k");
   // RAW: the chunks of the next tile on their way through registers.  A chunk that reaches behind its row's end is loaded from the
@@ -508,11 +518,16 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
         const P* at = srcA[i] + p * q.plane_a + (a_at + (TA ? k0 * q.lda : k0));
         __builtin_amdgcn_global_load_lds((gbl_ptr)at, (lds_ptr)(base + p * TILE_A + (i * NT + wave * 64) * 8), 16, 0, 0);
       }
+      auto load_b = [&](auto beyond) {
 #pragma unroll
-      for (int i = 0; i < ITB; ++i) {
-        const P* at = b0 + p * q.plane_b + (TB && end ? endB[i] : srcB[i]);
-        __builtin_amdgcn_global_load_lds((gbl_ptr)at, (lds_ptr)(base + NP * TILE_A + p * TILE_B + (i * NT + wave * 64) * 8), 16, 0, 0);
-      }
+        for (int i = 0; i < ITB; ++i) {
+          const P* at = b0 + p * q.plane_b + srcB[i] - beyond(i);
+          __builtin_amdgcn_global_load_lds((gbl_ptr)at, (lds_ptr)(base + NP * TILE_A + p * TILE_B + (i * NT + wave * 64) * 8), 16, 0, 0);
+        }
+      };
+      // (the step with B's last rows, where they are fewer than BK: the last one again for those that there are not)
+      if (TB && end) load_b([&](int i) { return max((i * NT + tid) / CB - (q.brows - 1) % BK, 0L) * q.ldb; });
+      else load_b([](int) { return 0; });
     }
   };
   auto land = [&](int buf) {
@@ -566,12 +581,12 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
       }
     });
     if constexpr (STRETCHES == 3) {
-      const bool rest = k0 >= q.stretch && k0 < 2 * q.stretch;
+      auto part = [&](auto rest) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        b[0][j] = gf_part(b[0][j], rest);
-        asm volatile("" : "+v"(b[0][j]));                          // (one after the other: all at once would take more registers than there are)
-      }
+        for (int j = 0; j < FN; ++j) b[0][j] = gf_part<decltype(rest)::value>(b[0][j]);
+      };
+      if (k0 >= q.stretch && k0 < 2 * q.stretch) part(std::true_type{});
+      else part(std::false_type{});
     }
   };
   auto multiply = [&] {
