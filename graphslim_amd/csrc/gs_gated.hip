@@ -35,18 +35,19 @@ inline long gf_up(long n) { return (n + GF_PAD - 1) / GF_PAD * GF_PAD; }
 
 // ---- activations: the value and its derivative ---------------------------------------------------------------------------------
 // Both tails keep their digits: Phi(g) = erfc(-g / sqrt 2) / 2 (1 + erf(g / sqrt 2) has none left below -5), and the sigmoid and what it
-// leaves of 1 come from e^-|g|, neither by a difference.
-template <int ACT>
+// leaves of 1 come from e^-|g|, neither by a difference.  16-bit types take the short exponential, off by 2^-23 |g| of itself (8192 x 2048 x
+// 8192 bf16, silu: 450 us, with the other one 473).
+template <int T, int ACT>
 __device__ __forceinline__ void gf_act(float g, float& a, float& da) {
   if constexpr (ACT == GS_ACT_RELU) {
     a = g > 0.f ? g : (g == g ? 0.f : g);
     da = g > 0.f ? 1.f : 0.f;
   } else if constexpr (ACT == GS_ACT_GELU) {
-    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g), x = -0.5f * g * g;
     a = g * cdf;
-    da = cdf + g * expf(-0.5f * g * g) * 0.39894228040143268f;
+    da = cdf + g * (T == GS_TYPE_F32 ? expf(x) : __expf(x)) * 0.39894228040143268f;
   } else {
-    const float e = expf(-fabsf(g)), one = 1.f / (1.f + e), zero = e * one;
+    const float x = -fabsf(g), e = T == GS_TYPE_F32 ? expf(x) : __expf(x), one = 1.f / (1.f + e), zero = e * one;
     const float sig = g >= 0.f ? one : zero, rest = g >= 0.f ? zero : one;
     a = ACT == GS_ACT_SILU ? g * sig : sig;
     da = ACT == GS_ACT_SILU ? sig * (1.f + g * rest) : sig * rest;
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(256) void gs_gated_slopes_kernel(int act, const typ
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float a, da;
-        gf_act<decltype(ac)::value>(g[j], a, da);
+        gf_act<T, decltype(ac)::value>(g[j], a, da);
         du[j] = d[j] * a;
         dg[j] = d[j] * u[j] * da;
       }
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(256) void gs_gated_rows_kernel(GatedRows q) {
         const long f = f0 + r;
         if (lane == m * RF + r && m0 + m < q.M && f < q.F) {
           float a, da;
-          gf_act<decltype(ac)::value>(acc[m][r], a, da);
+          gf_act<T, decltype(ac)::value>(acc[m][r], a, da);
           ((E*)q.h)[(m0 + m) * q.ldh + f] = (E)(a * acc[m][RF + r]);
           if (q.saved) {
             q.saved[(m0 + m) * q.F + f] = acc[m][r];
@@ -678,7 +679,7 @@ __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, u
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              gf_act<decltype(ac)::value>(g[e], h[e], da);
+              gf_act<T, decltype(ac)::value>(g[e], h[e], da);
               h[e] *= u[e];
             }
             gs_store<E, 4>((E*)q.C[0] + m * q.ldc + n, q.N - n, h);
@@ -761,7 +762,7 @@ __device__ __forceinline__ void gf_join(const GatedGemm& q, int slices, unsigned
       float da;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        gf_act<decltype(ac)::value>(g[e], g[e], da);
+        gf_act<T, decltype(ac)::value>(g[e], g[e], da);
         g[e] *= u[e];
       }
     });
