@@ -265,23 +265,26 @@ __global__ __launch_bounds__(256) void gs_gated_rows_kernel(GatedRows q) {
   for (int m = 0; m < MB; ++m)
 #pragma unroll
     for (int r = 0; r < 2 * RF; ++r) acc[m][r] = gs_wave_sum(acc[m][r]);
-  gf_with_act(q.act, [&](auto ac) {
+  float g = 0.f, u = 0.f;    // a lane finishes one result
 #pragma unroll
-    for (int m = 0; m < MB; ++m)
+  for (int m = 0; m < MB; ++m)
 #pragma unroll
-      for (int r = 0; r < RF; ++r) {
-        const long f = f0 + r;
-        if (lane == m * RF + r && m0 + m < q.M && f < q.F) {
-          float a, da;
-          gf_act<T, decltype(ac)::value>(acc[m][r], a, da);
-          ((E*)q.h)[(m0 + m) * q.ldh + f] = (E)(a * acc[m][RF + r]);
-          if (q.saved) {
-            q.saved[(m0 + m) * q.F + f] = acc[m][r];
-            q.saved[(q.M + m0 + m) * q.F + f] = acc[m][RF + r];
-          }
-        }
+    for (int r = 0; r < RF; ++r)
+      if (lane == m * RF + r) {
+        g = acc[m][r];
+        u = acc[m][RF + r];
       }
+  const long m = m0 + lane / RF, f = f0 + lane % RF;
+  if (lane >= MB * RF || m >= q.M || f >= q.F) return;
+  gf_with_act(q.act, [&](auto ac) {
+    float a, da;
+    gf_act<T, decltype(ac)::value>(g, a, da);
+    ((E*)q.h)[m * q.ldh + f] = (E)(a * u);
   });
+  if (q.saved) {
+    q.saved[m * q.F + f] = g;
+    q.saved[(q.M + m) * q.F + f] = u;
+  }
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------------------
