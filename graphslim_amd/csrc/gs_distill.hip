@@ -176,7 +176,7 @@ struct DistillTeacher {
 };
 
 // The row in registers, EP logits a thread: read once, written once.  Bound by HBM: 8192 x 32000 bf16, loss and gradient, 1.05 GB, 195 us
-// = 5.4 TB/s; 454 x 40 fp32 12.5 us, a launch and its host call.
+// = 5.4 TB/s (more than a copy's 4.9: the logits are read once and the gradient written once, both past the caches); 454 x 40 fp32 12.5 us, a launch and its host call.
 template <int T, int G, int EP, bool LOSS, bool GRAD, bool PAST>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void gs_distill_regs_kernel(DistillArgs a) {
   typedef typename GsElt<T>::type E;
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void gs_distill_regs_kernel(Dist
 
 // Rows of any length, a workgroup each.  STATS: the log-sum is taken from z (a running maximum and sum per thread, one pass), else it is
 // given.  Bound by HBM: losses, 2047 x 100003 fp16, 410 MB, 89 us = 4.6 TB/s; the gradient alone, 1024 x 50001 fp32, 411 MB,
-// 100 us = 4.1 TB/s (rows of odd length: three of four are read and written across cache lines).
+// 101 us = 4.1 TB/s (rows of odd length: three of four are read and written across cache lines).
 template <int T, int G, bool STATS, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(G) void gs_distill_row_kernel(DistillArgs a) {
   typedef typename GsElt<T>::type E;
@@ -373,8 +373,8 @@ void ds_regs(const DistillArgs& a, hipStream_t s) {
   constexpr int ROWS = G < 256 ? 256 / G : 1;
   const dim3 grid((unsigned)((a.n + ROWS - 1) / ROWS));
   if constexpr (GRAD && G >= 512) {
-    // A gradient that the 256 MB cache cannot keep beside the logits goes past it, and so do they (8192 x 32000 bf16: 225 -> 213 us;
-    // 2048 x 32000 fp32: 119 -> 112 us); a smaller one stays there for the products that read it next.
+    // A gradient that the 256 MB cache cannot keep beside the logits goes past it, and so do they (8192 x 32000 bf16: 217 us through
+    // the caches, 196 past them; 2048 x 32000 fp32: 116 and 104); a smaller one stays there for the products that read it next.
     if ((double)a.n * a.V * sizeof(typename GsElt<T>::type) > 128e6)
       return gs_distill_regs_kernel<T, G, EP, LOSS, GRAD, true><<<grid, dim3(G), ds_lds(a.k), s>>>(a);
   }
@@ -382,8 +382,8 @@ void ds_regs(const DistillArgs& a, hipStream_t s) {
 }
 
 // Rows that fit the registers are read once; a wave works on the shortest.  Where a choice is left, the fewest threads: several rows
-// on a compute unit overlap one's loads with another's arithmetic and barriers (8192 x 32000 bf16: 512 threads of 64 logits 222 us =
-// 4.7 TB/s, 1024 of 32 248 us; 2048 x 60000: 512 of 128 120 us, 1024 of 64 143 us).  Longer rows, and losses alone, which gain nothing
+// on a compute unit overlap one's loads with another's arithmetic and barriers (8192 x 32000 bf16: 512 threads of 64 logits
+// 196 us, 1024 of 32 238; 2048 x 60000: 512 of 128 109 us, 1024 of 64 160).  Longer rows, and losses alone, which gain nothing
 // from holding a long row, are walked (1024 x 131072 bf16, loss and gradient: 128 us held, 159 us walked twice).
 template <int T, bool LOSS, bool GRAD>
 void ds_stats(const DistillArgs& a, hipStream_t s) {

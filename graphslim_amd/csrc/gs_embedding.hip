@@ -11,7 +11,7 @@ namespace {
 // Bound by HBM: the distinct rows are read, all output rows written, and the scale costs nothing beside that.  One thread takes two 16-byte
 // pieces of output rows, half of all pieces apart, so that two dependent loads (id, row) are under way; the piece's row comes from a
 // 32-bit division, since one in 64 bits costs more than the piece's traffic.
-// 16383 ids, 50001 x 602 fp32: 11.3 us = 4.7 TB/s (a large copy reaches 4.9); 8 ids, 32000 x 1024 bf16: 7.6 us, a launch.
+// 16383 ids, 50001 x 602 fp32: 11.3 us = 4.7 TB/s (a large copy reaches 4.9); 8 ids, 32000 x 1024 bf16: 8 us, a launch and its host call.
 template <int T>
 __global__ __launch_bounds__(256) void gs_embedding_fwd_kernel(const typename GsElt<T>::type* __restrict__ W, long ldw, long V, int F,
                                                                const int* __restrict__ ids, unsigned total, float scale,
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void gs_embedding_fwd_kernel(const typename Gs
 //                cut into spans with a workgroup each, whose sums gs_embedding_join adds in the spans' order.
 constexpr int EM_TILE = 4096;      // ids per workgroup of the sort: four a thread, all loaded at once
 // Tokens of a bucket per workgroup: fewer make more partial sums, more a longer walk of a frequent row (bf16, 30000 ids on 300 x 2000:
-// 128, 256 and 512 tokens 62, 55 and 70 us; 32768 ids on 128000 x 2048: 169, 170 and 176).
+// 128, 256 and 512 tokens 62, 55 and 70 us; 32768 ids on 128000 x 2048: 169, 170 and 176 us).
 constexpr int EM_SPAN = 256;
 // Tiles up to which the sort's workgroups each add up all tiles' counts; beyond, a launch of its own makes prefix sums of them, since the
 // adding grows with the square of the tokens (32000 rows of 16, fp32: 140 000 tokens 32 us either way, 1 000 000 100 against 92,

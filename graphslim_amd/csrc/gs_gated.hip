@@ -36,7 +36,7 @@ inline long gf_up(long n) { return (n + GF_PAD - 1) / GF_PAD * GF_PAD; }
 // ---- activations: the value and its derivative ---------------------------------------------------------------------------------
 // Both tails keep their digits: Phi(g) = erfc(-g / sqrt 2) / 2 (1 + erf(g / sqrt 2) has none left below -5), and the sigmoid and what it
 // leaves of 1 come from e^-|g|, neither by a difference.  16-bit types take the short exponential, off by 2^-23 |g| of itself (8192 x 2048 x
-// 8192 bf16, silu: 450 us, with the other one 473).
+// 8192 bf16, silu: 470 us where the other one takes 493).
 template <int T, int ACT>
 __device__ __forceinline__ void gf_act(float g, float& a, float& da) {
   if constexpr (ACT == GS_ACT_RELU) {
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256) void gs_gated_slopes_kernel(int act, const typ
 // ---- few rows -------------------------------------------------------------------------------------------------------------------
 // For a few rows (eight at a time) the weights are all there is to read, and the vector units keep up: a wave takes RF rows of both weights,
 // its lanes 16 bytes each of a stretch of k, and adds across the lanes at the end.  Exact fp32 products for every type.  Bound by the
-// reading of the weights: one row, 2048 x 8192 bf16, 67 MB, 11.7 us = 5.7 TB/s (from the 256 MB cache when repeated, as here).
+// reading of the weights: one row, 2048 x 8192 bf16, 67 MB, 11.6 us = 5.8 TB/s (from the 256 MB cache when repeated, as here).
 struct GatedRows {
   const void *x, *wg, *wu;
   long ldx, ldw, M, D, F, ldh;
@@ -417,9 +417,10 @@ __device__ const int gf_zeros[4] __attribute__((aligned(16))) = {};   // a chunk
 // and the activation is applied in registers.
 // Bound by the matrix pipe where tiles are many: 16 FM x 16 FN results of a wave need FM + FN fragments from LDS a step for FM FN
 // instructions, so that 8 x 4 fragments (256 x 256 by eight waves) keep LDS reads below the pipe's time, and 4 x 4 do not quite.
-// 8192 x 2048 x 8192 bf16: forward 452 us = 1.22 PFLOP/s (a library's product of 8192^3 reaches 1.32), 516 with `saved` (537 MB more),
-// backward 2070 us = 1.06 PFLOP/s of the doubled products with the pass that makes [dg | du] (dg and du rounded to bf16: 1055).  fp32, six products of bf16 parts, 2708 x 500 x 1024: 150 us for
-// both passes = 111 TFLOP/s (the library: 153): the forward product has 176 large tiles for 256 compute units.
+// 8192 x 2048 x 8192 bf16: forward 470 us = 1.17 PFLOP/s (a library's product of 8192^3 reaches 1.32), 528 with `saved` (537 MB more),
+// backward 2040 us with the pass that makes [dg | du] = 1.08 PFLOP/s of the two parts' products (dg and du rounded to bf16: 1055 us); fp16
+// backward, three products and x and the weights split in registers, 3600 us.  fp32, six products of bf16 parts, 2708 x 500 x 1024: 152 us
+// for both passes = 109 TFLOP/s (the library: 153): the forward product has 176 large tiles for 256 compute units.
 template <int T, int PL, int WM, int WN, int FM, int FN, int BK, bool TA, bool TB, bool RAW, bool GATED>
 __device__ __forceinline__ void gf_product(const GatedGemm& q, unsigned block, unsigned slice, char* smem) {
   typedef typename GfPlane<T, PL>::type P;
@@ -1035,8 +1036,8 @@ int gf_operands(const GatedCall& c, const GatedPlan& p, GatedOperands* o, hipStr
   return GS_OK;
 }
 
-// Rows up to which the weights are read by gs_gated_rows_kernel.  2048 x 8192: bf16, 4 rows 16 us and 8 rows 25 us against 22 for the
-// matrix pipe; fp32, 24 rows 96 us against 115, of which laying out the split weights is most.
+// Rows up to which the weights are read by gs_gated_rows_kernel.  2048 x 8192: bf16, 4 rows 14 us (8 rows took 25), by the matrix pipe 5 to 8
+// rows 16; fp32, 24 rows 92 us and 25 by the matrix pipe 113, of which laying out the split weights is most.
 inline bool gf_few(long M, int type) { return M <= (type == GS_TYPE_F32 ? 24 : 4); }
 
 template <int T, int MB>
