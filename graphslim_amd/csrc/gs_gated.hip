@@ -9,7 +9,8 @@
 // type they would cost the gradients a second rounding as large as that of the result, and in fp16 dh u act'(g) can lie outside of the
 // type though the gradients do not.  The parts lie one behind the other along k, against the same weights or x a second time:
 //   bf16:  dg W = lo W + hi W;      fp16:  W = V + R, bf16 parts that hold all of its 11 bits, dg W = lo V + hi R + hi V
-// (lo R is below 2^-17 of the product and left out).
+// A rounded bf16 leaves at most 2^-8 of a value, the second part's rounding 2^-9 of that: dg is held to 2^-17.  lo R, at most 2^-8 2^-8 of the
+// product, is left out, so fp16's products are off by up to 2^-16 + 2^-17 of their terms; the result's own rounding is 2^-11.
 // The parts of fp32 operands, and [dg | du], are laid out in the caller's scratch first, rows padded with zeros to a multiple of 64;
 // so are 16-bit operands whose rows do not consist of whole, aligned chunks of 16 bytes, unless it is cheaper to read them as they are.
 #include <algorithm>
@@ -411,10 +412,10 @@ __device__ __forceinline__ void gf_tr_read4(unsigned addr, int first, Frag* x) {
 
 __device__ const int gf_zeros[4] __attribute__((aligned(16))) = {};   // a chunk behind the end of a row
 
-// T: type of the outputs (and of 16-bit operands), PL: parts (3: side by side; 2: those of A one behind the other along k), WM x WN waves of (16 FM) x (16 FN) results.  TA, TB: the operand's other
-// index is contiguous, not k.  RAW: x and the weights are read where they are though their rows begin or end inside a 16-byte chunk:
-// through registers, with zeros behind a row's end.  GATED: rows of B alternate between gate and up every 16, so that a lane holds both sums of its outputs
-// and the activation is applied in registers.
+// T: type of the outputs (and of 16-bit operands), PL: parts (3: side by side; 2: those of A one behind the other along k), WM x WN waves
+// of (16 FM) x (16 FN) results.  TA, TB: the operand's other index is contiguous, not k.  RAW: x and the weights are read where they are
+// though their rows begin or end inside a 16-byte chunk: through registers, with zeros behind a row's end.  GATED: rows of B alternate
+// between gate and up every 16, so that a lane holds both sums of its outputs and the activation is applied in registers.
 // Bound by the matrix pipe where tiles are many: 16 FM x 16 FN results of a wave need FM + FN fragments from LDS a step for FM FN
 // instructions, so that 8 x 4 fragments (256 x 256 by eight waves) keep LDS reads below the pipe's time, and 4 x 4 do not quite.
 // 8192 x 2048 x 8192 bf16: forward 470 us = 1.17 PFLOP/s (a library's product of 8192^3 reaches 1.32), 528 with `saved` (537 MB more),
@@ -821,8 +822,8 @@ GatedSplit gf_split_of(long M, long N, long K, bool gated, int pl) {
   return best;
 }
 
-// dx (M x D, k over 2 Fp) and dW (2 Fp x D, k over Mp), each in so many stretches: one launch of both, cut into pieces of about equal length, where that costs less
-// than one after the other (the same units, a launch about 3).
+// dx (M x D, k over 2 Fp) and dW (2 Fp x D, k over Mp), each in so many stretches: one launch of both, cut into pieces of about equal
+// length, where that costs less than one after the other (the same units, a launch about 3).
 struct GatedPair {
   bool together;
   GatedSplit dx, dw;

@@ -300,8 +300,8 @@ int gs_ot_divdiff_f32(float* K, const float* lam, const float* g, const float* g
 
 /* ---------------------------------------------------------------------------------------------
  * Training a student on a teacher's top logits: rows of a table by id and the table's gradient, the gated feed-forward block, the
- * distillation loss.  Rows are held in 32 or 16 bits (`type`: one of GS_TYPE_*); everything is computed and summed in fp32 and
- * rounded once when it is stored, and every sum has a fixed order (no float atomics: two runs are bitwise equal).  Row strides are in
+ * distillation loss.  Rows are held in 32 or 16 bits (`type`: one of GS_TYPE_*); everything is computed and summed in fp32, or in
+ * products of parts that say what they hold, and rounded once when it is stored, and every sum has a fixed order (no float atomics: two runs are bitwise equal).  Row strides are in
  * elements; rows may start at any element's address.  `scratch` is device memory of at least the bytes that the call's
  * *_scratch_bytes function names, 16-byte aligned; nothing in it is kept between calls, and calls that may run at the same time
  * (on different streams, or in different captured graphs) need scratch of their own.  No call allocates, synchronises or copies to
@@ -336,7 +336,8 @@ size_t gs_gated_fwd_scratch_bytes(long M, long D, long F, int type, int plain);
 int gs_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, long ldw, int type, long M, long D, long F, int act,
                  void* h, long ldh, float* saved, void* scratch, gs_stream_t stream);
 /* dg = dh * u * act'(g), du = dh * act(g); dx = dg Wg + du Wu, dw_gate = dg^T x, dw_up = du^T x.  For 16-bit types dg and du enter the
- * products as two bf16 parts: to 2^-17 of each and with fp32's range, so that a slope that fp16 does not hold leaves the gradients right.
+ * products as two bf16 parts: to 2^-17 of each (fp16: 2^-16 + 2^-17 of each product) and with fp32's range, so that a slope that fp16
+ * does not hold leaves the gradients right.
  * fp32 products (forward: of more than 24 rows) are six products of bf16 parts: as exact as fp32 (parts have a smallest step of 2^-133).
  * Operands that are not finite: what they enter by the formulas is not finite, nothing else is touched.  Where products are made of
  * parts (fp32, and the backward call in every type), or a size is no multiple of 64, it can be NaN where the formula gives an infinity,

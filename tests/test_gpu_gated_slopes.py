@@ -1,4 +1,4 @@
-"""dg and du of the gated block's backward pass keep fp32's range and 17 bits, whatever the operands' type: gradients against 64 bits under
+"""dg and du of the gated block's backward pass keep fp32's range and 16 bits, whatever the operands' type: gradients against 64 bits under
 bounds that count one rounding to the type, that of the result."""
 import pytest
 import torch
@@ -8,8 +8,10 @@ from test_gpu_ops import BF16, DEV, F16, gen, normal, ops, strided  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
-# dg, du as two bf16 parts are off by 2^-18; fp16 weights and x as two more, whose least product, 2^-9 2^-9, is left out.  Together 2^-17.
-PARTS = 2.0 ** -17
+# A rounded bf16 leaves at most 2^-8 of a value, a remainder whose exponent is at least 9 lower, and that one's rounding half a step of
+# 2^-7: dg, du as two parts are off by 2^-17.  fp16 weights and x are two more parts, exactly, whose product with the second part of dg, at
+# most 2^-8 2^-8, is left out.
+PARTS = {BF16: 2.0 ** -17, F16: 2.0 ** -17 + 2.0 ** -16}
 U = R.U
 
 
@@ -23,8 +25,8 @@ def gradients(d_h, x, wg, wu, saved, act):
     ea = 16 * U * (a.abs() + 1e-30) + (4 * U * g.abs() if act == "gelu" else 0)   # as for the forward pass
     eda = 16 * U * (1 + g.abs())
     dg, du = d * u * da, d * a
-    edg = d.abs() * u.abs() * eda + (PARTS + 3 * U) * dg.abs() + 2.0 ** -126
-    edu = d.abs() * ea + (PARTS + 3 * U) * du.abs() + 2.0 ** -126
+    edg = d.abs() * u.abs() * eda + (PARTS[dt] + 3 * U) * dg.abs() + 2.0 ** -126
+    edu = d.abs() * ea + (PARTS[dt] + 3 * U) * du.abs() + 2.0 ** -126
     adg, adu = dg.abs() + edg, du.abs() + edu
     M, F = dg.shape
     dx = dg @ wg + du @ wu
